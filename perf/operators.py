@@ -130,8 +130,7 @@ def prepare(case, seed):
             s.ws, s.ws_bytes = _workspace(s.cf.cf_fp8_grouped_gemm_workspace_bytes, s.total, c["experts"])
         elif c["kind"] == "grads":
             s.ws, s.ws_bytes = _workspace(s.cf.cf_grad_norm_workspace_bytes)
-            s.list, s.list_bytes = _grad_list(s.cf, s.grads)
-            s.out_list, _ = _grad_list(s.cf, s.clipped)
+            s.list, s.list_bytes = _grad_list(s.cf, s.grads, s.clipped)
     return s
 
 
@@ -335,15 +334,15 @@ def _prepare_grads(s, c, g):
     s.norm, s.coef = _one(), _one()
 
 
-def _grad_list(cf, tensors):
+def _grad_list(cf, tensors, out):
     """The device table of a list of gradients, made once: the buffers stay where they are from step to step."""
-    ptrs = torch.tensor([t.data_ptr() for t in tensors], dtype=torch.int64)
+    ptrs, outs = (torch.tensor([t.data_ptr() for t in ts], dtype=torch.int64) for ts in (tensors, out))
     counts = torch.tensor([t.numel() for t in tensors], dtype=torch.int64)
     types = torch.tensor([int(t.dtype == torch.float32) for t in tensors], dtype=torch.int32)
     n = ctypes.c_size_t(0)
     cf.cf_grad_list_bytes(counts, len(tensors), ctypes.byref(n))
     table = torch.empty(n.value, dtype=torch.uint8)
-    cf.cf_grad_list_fill(ptrs, counts, types, len(tensors), table, n.value)
+    cf.cf_grad_list_fill(ptrs, outs, counts, types, len(tensors), table, n.value)
     return table.to(DEV), n.value
 
 
@@ -352,7 +351,7 @@ def _named(out):
 
 
 def _own_grads(s, c, cf, st):
-    cf.cf_grad_norm_clip(s.list, s.out_list, s.list_bytes, float(c["max_norm"]), s.norm, s.coef, s.ws, s.ws_bytes, st)
+    cf.cf_grad_norm_clip(s.list, s.list_bytes, float(c["max_norm"]), s.norm, s.coef, s.ws, s.ws_bytes, st)
     return {"norm": s.norm, "coef": s.coef, **_named(s.out)}
 
 
