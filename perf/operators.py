@@ -326,7 +326,7 @@ def _prepare_grads(s, c, g):
     # two norm weights, q k v o, gate and up, their biases, down; back to back in one buffer for each type, as trainers keep them
     layer = [(h, small), (h, small), (4 * h * h, big), (h * i, big), (h * i, big), (i, small), (i, small), (h * i, big)]
     shapes = layer * c["layers"]
-    s.flat = {t: _normal(g, sum(n for n, u in shapes if u == t), sigma=1e-3, dtype=t) for t in {u for _, u in shapes}}
+    s.flat = {t: _normal(g, sum(n for n, u in shapes if u == t), sigma=1e-3, dtype=t) for t in sorted({u for _, u in shapes}, key=str)}
     s.out = {t: torch.zeros_like(f) for t, f in s.flat.items()}
     at = {t: [n for n, u in shapes if u == t] for t in s.flat}
     s.grads = [v for t, f in s.flat.items() for v in f.split(at[t])]
