@@ -2494,7 +2494,8 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     if (!d_counts || !d_offsets || !A || !B || !C || !a_descale || !b_descale || !d_workspace) return CF_ERR_INVALID_ARG;
     if (epilogue != EPI_NONE && epilogue != EPI_SILU_GATE) return CF_ERR_INVALID_ARG;
     if (epilogue == EPI_SILU_GATE && (!B_up || !b_up_descale)) return CF_ERR_INVALID_ARG;
-    if (scale_mode != SCALE_TENSOR && scale_mode != SCALE_ROWCOL) return CF_ERR_INVALID_ARG;
+    if (scale_mode != SCALE_TENSOR && scale_mode != SCALE_ROWCOL && scale_mode != SCALE_BLOCK) return CF_ERR_INVALID_ARG;
+    if (scale_mode == SCALE_BLOCK && (epilogue != EPI_NONE || a_is_e5m2)) return CF_ERR_UNSUPPORTED;
     // per-tensor descales would need one device scalar per expert for the weights: not built.  Rejected before
     // anything is launched, so a refused call leaves the workspace untouched.
     if (scale_mode == SCALE_TENSOR) return CF_ERR_UNSUPPORTED;
@@ -2506,7 +2507,7 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
         (epilogue == EPI_SILU_GATE && !aligned16(B_up)) || lda < K || ldc < N ||
         static_cast<size_t>(a_rows) * lda >= (1ull << 32) || static_cast<size_t>(N) * K >= (1ull << 32) ||
         (epilogue == EPI_SILU_GATE ? N % (BN / 2) != 0 : N % 8 != 0) || N < 8 || ldc % 8 != 0 || !aligned16(C) || !aligned16(b_descale) ||
-        (epilogue == EPI_SILU_GATE && !aligned16(b_up_descale)))
+        (epilogue == EPI_SILU_GATE && !aligned16(b_up_descale)) || (scale_mode == SCALE_BLOCK && K > kBlockMaxK))
         return CF_ERR_UNSUPPORTED;
     hipStream_t st = as_stream(stream);
     const int max_row_tiles = total_rows / BM + num_experts;
@@ -2523,10 +2524,11 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     p.a_row_index = d_a_row_index;
     p.a_rows = a_rows;
     p.b_expert_stride = static_cast<long long>(N) * K;
-    p.sb_expert_stride = scale_mode == SCALE_ROWCOL ? N : 0;
+    p.sb_expert_stride = scale_mode == SCALE_ROWCOL ? N : scale_mode == SCALE_BLOCK ? (N + 127) / 128 * (K / BK) : 0;
     const int out_bn = epilogue == EPI_SILU_GATE ? BN / 2 : BN;
     p.tiles_m = p.map_entries = max_row_tiles;
     p.tiles_n = (N + out_bn - 1) / out_bn;
+    if (scale_mode == SCALE_BLOCK) return grouped_gemm_nt_block(p, total_rows, num_experts, st);
     // Few rows per expert: the small-tile kernel, which walks an expert's rows 16 mb at a time, where its estimate is lower.
     // It is sized for half as many rows again as the bound's average, so that most experts take one pass over their weights;
     // beyond 40 rows that is more than its largest pass.  The counts are on the device, so the choice is for balanced experts: 64 of
@@ -2538,7 +2540,7 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
         const float direct = grouped_direct_estimate_us(total_rows, N, K, num_experts, gate, &shape);
         const int row_tiles = total_rows < num_experts ? total_rows : num_experts;
         if (direct < ring_estimate_us(row_tiles * BM, N, K, BM, out_bn, 0.95f, 6.0f)) {
-            const int rc = grouped_gemm_nt_direct(p, a_is_e5m2, epilogue, shape, st);
+            const int rc = grouped_gemm_nt_direct(p, a_is_e5m2, epilogue, scale_mode, shape, st);
             if (rc != CF_ERR_UNSUPPORTED) return rc;
         }
     }
@@ -2553,7 +2555,7 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
         if (direct < ring_estimate_us(num_experts * BM, N, K, BM, out_bn, gate ? 0.88f : 0.89f, gate ? 8.3f : 6.1f)) {
             GemmArgs q = p;
             q.tiles_m *= std::min(4, (total_rows + 64 * num_experts - 1) / (64 * num_experts) + 1);
-            const int rc = grouped_gemm_nt_direct(q, a_is_e5m2, epilogue, shape, st);
+            const int rc = grouped_gemm_nt_direct(q, a_is_e5m2, epilogue, scale_mode, shape, st);
             if (rc != CF_ERR_UNSUPPORTED) return rc;
         }
     }

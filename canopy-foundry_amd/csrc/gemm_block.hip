@@ -582,4 +582,10 @@ int gemm_nt_block_slim(GemmArgs p, hipStream_t st) {
     return launch_status();
 }
 
+// The small-tile kernel of gemm_direct.hip: 64 rows of an expert at a time; 32 where K leaves no room for the scales of 64.
+int grouped_gemm_nt_block(const GemmArgs& p, int total_rows, int num_experts, hipStream_t st) {
+    const int rc = grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, 3, st);
+    return rc != CF_ERR_UNSUPPORTED ? rc : grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, 7, st);
+}
+
 }  // namespace cf

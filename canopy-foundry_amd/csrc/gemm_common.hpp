@@ -12,6 +12,7 @@ enum { SCALE_TENSOR = 0, SCALE_ROWCOL = 1, SCALE_BLOCK = 2, SCALE_ROW = 3 };   /
 
 constexpr int BM = 256, BN = 256, BK = 128;       // tile of the persistent kernels; BK is every kernel's K-tile
 constexpr int kXcds = 8;
+constexpr int kBlockMaxK = 256 * BK;              // a tile's weight-block scales lie in LDS: 256 of them
 constexpr int kMapWords = 5;                      // words per entry of the row-tile table (build_tile_map), an entry being BM rows
 
 struct GemmArgs {
@@ -39,7 +40,7 @@ struct GemmArgs {
     const int* a_row_index;      // compact row r reads A row (and its descale) a_row_index[r]; null = r
     int a_rows;                  // rows of the A buffer (= M without a row index)
     long long b_expert_stride;   // bytes between the weight matrices of consecutive experts
-    int sb_expert_stride;        // elements between the channel descales of consecutive experts
+    int sb_expert_stride;        // elements between the channel or block descales of consecutive experts
     // term-split form (ring kernel, MX instantiation only): A's K axis is `K / b_k_period` terms laid side by side,
     // term t = the residual of the terms before it scaled by 16^t; every term multiplies the same b_k_period
     // columns of B, and the matrix cores scale its products by 2^(-4 t)
@@ -104,7 +105,7 @@ float direct_estimate_us(const GemmArgs& p, int epi, int scale_mode, int* shape)
 float grouped_direct_estimate_us(int total_rows, int N, int K, int num_experts, bool gate, int* shape);
 float grouped_direct_many_estimate_us(int total_rows, int N, int K, int num_experts, bool gate, int* shape);
 int gemm_nt_direct(const GemmArgs& p, int fmt, int epi, int scale_mode, int shape, hipStream_t st);
-int grouped_gemm_nt_direct(const GemmArgs& p, int fmt, int epi, int shape, hipStream_t st);
+int grouped_gemm_nt_direct(const GemmArgs& p, int fmt, int epi, int scale_mode, int shape, hipStream_t st);
 // gemm_half.hip: whether it takes a problem, its time, the launch
 bool half_ok(const GemmArgs& p, int fmt, int epi, int scale_mode);
 float half_estimate_us(const GemmArgs& p, int epi, bool shared);
@@ -120,6 +121,8 @@ int gemm_nt_block_wide(GemmArgs p, hipStream_t st);
 bool block_slim_ok(const GemmArgs& p);
 float block_slim_estimate_us(const GemmArgs& p);
 int gemm_nt_block_slim(GemmArgs p, hipStream_t st);
+// the grouped form over a row-tile table, arguments checked
+int grouped_gemm_nt_block(const GemmArgs& p, int total_rows, int num_experts, hipStream_t st);
 // gemm_accum.hip
 bool accum_wide_ok(const GemmArgs& p, int fmt, int epi, int scale_mode);
 float accum_wide_estimate_us(const GemmArgs& p);

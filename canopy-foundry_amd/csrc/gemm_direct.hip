@@ -109,9 +109,12 @@ void k_gemm_nt_direct(const GemmArgs p, const int rowcol, const int bias, const 
             // the tile's scales: [TM][groups] of the activations, [groups] of the weights
             for (int i = threadIdx.x; i < TM * kgroups; i += 64 * WK) {
                 const int r = i / kgroups, k = i - r * kgroups;
-                lds_sa[r * kpad + k] = p.sa[static_cast<size_t>(min(m0 + r, m_end - 1)) * kgroups + k];
+                int row = min(m0 + r, m_end - 1);
+                if (GROUPED && p.a_row_index) row = p.a_row_index[row];
+                lds_sa[r * kpad + k] = p.sa[static_cast<size_t>(row) * kgroups + k];
             }
-            for (int i = threadIdx.x; i < kgroups; i += 64 * WK) lds_sb[i] = p.sb[static_cast<size_t>(n0 / 128) * kgroups + i];
+            const float* sb = p.sb + static_cast<size_t>(expert) * p.sb_expert_stride + static_cast<size_t>(n0 / 128) * kgroups;
+            for (int i = threadIdx.x; i < kgroups; i += 64 * WK) lds_sb[i] = sb[i];
             __syncthreads();
         }
 
@@ -479,8 +482,9 @@ int gemm_nt_direct(const GemmArgs& p, int fmt, int epi, int scale_mode, int shap
     return fmt == 1 ? launch_plain<1, false, false>(p, epi, scale_mode, shape, st)
          : fmt == 0 ? launch_plain<0, false, false>(p, epi, scale_mode, shape, st) : CF_ERR_UNSUPPORTED;
 }
-int grouped_gemm_nt_direct(const GemmArgs& p, int fmt, int epi, int shape, hipStream_t st) {
+int grouped_gemm_nt_direct(const GemmArgs& p, int fmt, int epi, int scale_mode, int shape, hipStream_t st) {
     if (epi == EPI_SILU_GATE) return fmt == 0 ? launch_gate<true>(p, SCALE_ROWCOL, shape, st) : CF_ERR_UNSUPPORTED;
+    if (scale_mode == SCALE_BLOCK) return launch_plain<0, true, true>(p, epi, scale_mode, shape, st);
     return fmt == 1 ? launch_plain<1, false, true>(p, epi, SCALE_ROWCOL, shape, st)
                     : launch_plain<0, false, true>(p, epi, SCALE_ROWCOL, shape, st);
 }

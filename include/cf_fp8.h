@@ -211,6 +211,74 @@ int cf_rmsnorm_clip_quantize_record(const uint16_t* d_x, const uint16_t* d_scale
                                     float* d_rms, void* d_q, const float* d_qscale,
                                     float* d_amax, cf_stream_t stream);
 
+/* ---- the residual layer around the products --------------------------------
+ * The residual addition, RMS norm and quantize of a pre-norm layer in one pass, and its gradient; the reference adds,
+ * normalises and quantizes in separate launches (src/trainer.cu:6281-6304) and its backward of them is outside this library's path.
+ * The residual stream is bf16, or fp32 with stream_is_f32: d_residual, d_sum, d_grad_sum and d_grad_residual are then float*.
+ *     h = T(r + x)            T: the stream's type; x bf16, null = nothing is added
+ *     rms = sqrt(mean(h^2) + eps),   y = h / rms * scale      of h as it is stored, y in fp32
+ * d_sum [rows, H] receives h and may be d_residual; d_normed [rows, H] receives bf16(y) and may be d_x; d_rms [rows] is what the
+ * backward pass takes.  All three may be null.  The 8-bit output is made from the fp32 y: y is rounded once on that way, where
+ * cf_rmsnorm_clip_quantize_rows rounds it to bf16 first, as the reference's launches do.  A maximum leaves NaNs out; a NaN is NaN in
+ * the output.  eps is above 0, or no row is all zeros.  H <= 16384, else CF_ERR_UNSUPPORTED; otherwise any H and any alignment
+ * that the elements have.  Rows are contiguous. */
+
+/* Per-row scales: scale = 448 (57344: is_e5m2) / max(max|y|, 1e-12), descale its inverse, as cf_fp8_quantize_rows
+ * (kernels/fp8.cu:37-39,49). */
+int cf_add_rmsnorm_quantize_rows(const void* d_residual, const uint16_t* d_x, int stream_is_f32, const uint16_t* d_scale, int rows, int H,
+                                 float eps, int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_rms, void* d_q, float* d_row_scale,
+                                 float* d_row_descale, cf_stream_t stream);
+/* E4M3 with a scale for each 128 elements of a row, [rows, ceil(H/128)], the activation operand of the CF_SCALE_BLOCK_128 products; the
+ * formula of kernels/fp8.cu:37-39,49 per group. */
+int cf_add_rmsnorm_quantize_block_1x128(const void* d_residual, const uint16_t* d_x, int stream_is_f32, const uint16_t* d_scale, int rows,
+                                        int H, float eps, void* d_sum, uint16_t* d_normed, float* d_rms, void* d_q, float* d_group_scale,
+                                        float* d_group_descale, cf_stream_t stream);
+/* Delayed scaling: quantize with *d_qscale and raise *d_amax to max|y| (the caller zeroes it), as fp8_quantize_e4m3_record does
+ * (kernels/fp8.cu:67-103). */
+int cf_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, int stream_is_f32, const uint16_t* d_scale, int rows, int H,
+                                   float eps, int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_rms, void* d_q, const float* d_qscale,
+                                   float* d_amax, cf_stream_t stream);
+
+/* The gradient of the three (the quantize counts as the identity); no counterpart in the reference's fp8 path.  With dy = d_grad_normed [rows, H] bf16 (the gradient of
+ * y), h = d_sum and rms as the forward pass left them, dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
+ *     xh = h / rms,  g = dy * scale,  d_grad_residual = T(dh + (g - xh * mean(g * xh)) / rms)
+ * which is the gradient of r and, as bf16 or 8 bits, of x;   d_grad_scale [H] fp32 = (accumulate ? itself : 0) + sum over rows of dy * xh,
+ * the rows added in an order that follows from rows and H alone.  d_grad_residual may be d_grad_sum.  rows = 0 leaves zeros in d_grad_scale
+ * unless it accumulates.  d_workspace: 16-byte aligned, cf_add_rmsnorm_backward_workspace_bytes() bytes; it belongs to the call. */
+int cf_add_rmsnorm_backward_workspace_bytes(int rows, int H, size_t* bytes);
+int cf_add_rmsnorm_backward(const uint16_t* d_grad_normed, const void* d_sum, int stream_is_f32, const uint16_t* d_scale, const float* d_rms,
+                            const void* d_grad_sum, int rows, int H, void* d_grad_residual, float* d_grad_scale, int accumulate,
+                            void* d_workspace, size_t workspace_bytes, cf_stream_t stream);
+/* The same plus the gradient's E5M2 bytes for the products of the layer before, from the fp32 value: d_grad8 = e5m2(gradient * *d_qscale),
+ * *d_amax raised to its maximum (the caller zeroes it), as cf_cross_entropy_fwd_bwd_chunk_quant_e5m2 (kernels/fp8.cu:86-103). */
+int cf_add_rmsnorm_backward_quant_e5m2(const uint16_t* d_grad_normed, const void* d_sum, int stream_is_f32, const uint16_t* d_scale,
+                                       const float* d_rms, const void* d_grad_sum, int rows, int H, void* d_grad_residual,
+                                       float* d_grad_scale, int accumulate, void* d_grad8, const float* d_qscale, float* d_amax,
+                                       void* d_workspace, size_t workspace_bytes, cf_stream_t stream);
+
+/* ---- global norm of a list of gradients, and clipping by it: no counterpart in the reference's kernel library ------
+ *     norm = sqrt(sum over all elements of all tensors of g^2),  coef = norm > max_norm ? max_norm / norm : 1,  out = T(g * coef)
+ * The sum is taken in 64 bits, in an order that follows from the list alone.  A norm that is not finite (in fp32) is returned as it is and
+ * the gradients stay as they are (coef = 1): the caller who finds it skips the step.
+ * The list is a table of the tensors' addresses and sizes, made once for buffers that stay where they are: cf_grad_list_bytes gives its
+ * size, cf_grad_list_fill writes it to host memory (d_tensors, d_out, counts, types and list are host arrays), the caller copies it to
+ * the device, 16-byte aligned, and passes that and its size to the calls below.  d_out: where the clipped gradients go, null = in place;
+ * an output is its own input or overlaps no tensor.  Tensors need no more than their elements' alignment; a count of 0 takes no address. */
+#define CF_GRAD_BF16 0
+#define CF_GRAD_F32  1
+int cf_grad_list_bytes(const size_t* counts, int num_tensors, size_t* bytes);
+int cf_grad_list_fill(void* const* d_tensors, void* const* d_out, const size_t* counts, const int* types, int num_tensors, void* list,
+                      size_t list_bytes);
+/* The norm alone (no counterpart, as above).  d_workspace: 16-byte aligned, this many bytes for any list; it belongs to the call. */
+int cf_grad_norm_workspace_bytes(size_t* bytes);
+int cf_grad_norm(const void* d_list, size_t list_bytes, float* d_norm, void* d_workspace, size_t workspace_bytes, cf_stream_t stream);
+/* Clips by a norm the caller has (no counterpart, as above; over several GPUs: the root of the sum of their squares).  max_norm >= 0, infinity = leave them;
+ * d_coef may be null and is not d_norm. */
+int cf_grad_clip(const void* d_list, size_t list_bytes, float max_norm, const float* d_norm, float* d_coef, cf_stream_t stream);
+/* Both (no counterpart, as above): the same norm and the same bits as the two calls. */
+int cf_grad_norm_clip(const void* d_list, size_t list_bytes, float max_norm, float* d_norm, float* d_coef, void* d_workspace,
+                      size_t workspace_bytes, cf_stream_t stream);
+
 /* ---- loss head: chunked cross-entropy, fused with the quantize of its gradient ---------
  * The FP8 head (src/trainer.cu:8015-8060) projects a chunk of rows onto the vocabulary with the NT GEMM above,
  * runs cross-entropy forward + backward in place, and quantizes the bf16 gradient to E5M2 for the input-gradient
@@ -392,7 +460,7 @@ int cf_moe_scale_accumulate_bf16(uint16_t* d_mixed, const uint16_t* d_term,
 int cf_fp8_grouped_gemm_workspace_bytes(int total_rows, int num_experts, size_t* bytes);
 
 /* For each expert e: C[offsets[e] .. +counts[e], :] = A_rows . B[e]^T with the per-token x
- * per-channel scales and epilogues of cf_fp8_gemm_nt_bf16_ex (replaces the per-expert
+ * per-channel or block scales and epilogues of cf_fp8_gemm_nt_bf16_ex (replaces the per-expert
  * lt_gemm_fp8_nt calls at src/trainer.cu:6893-6931).  A row r of the compact output reads A row
  * d_a_row_index[r] (and its descale) when the index is given, so the token permute
  * (moe_gather_rows_u8, kernels/moe.cu:720-728) is fused into the operand fetch; null = row r.
@@ -400,7 +468,9 @@ int cf_fp8_grouped_gemm_workspace_bytes(int total_rows, int num_experts, size_t*
  * bound rows * top_k; counts / offsets stay on the device.  a_rows is the number of rows of d_A
  * (every row index is below it; total_rows without an index).  Needs K % 128 == 0, K >= 256,
  * N a multiple of 8 (of 128 with the SiLU-gate epilogue), ldc % 8 == 0, 16-byte aligned operands,
- * descales and C, and a_rows * lda, N * K below 2^32. */
+ * descales and C, and a_rows * lda, N * K below 2^32.
+ * scale_mode: CF_SCALE_ROW_COL, or CF_SCALE_BLOCK_128 with a_descale [a_rows, K/128] (the row index applies to its rows), b_descale
+ * [num_experts, ceil(N/128), K/128], no fused epilogue and K <= 32768. */
 int cf_fp8_grouped_gemm_nt_bf16_ex(int total_rows, int N, int K, int num_experts,
                                    const int* d_counts, const int* d_offsets, const void* d_A,
                                    int a_rows, int lda, const int* d_a_row_index, const float* d_a_descale,
