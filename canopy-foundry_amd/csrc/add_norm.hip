@@ -7,6 +7,8 @@
 // Backward, per row:  xh = h / rms,  g = dy * w,  c = mean(g * xh),  dr = dh + (g - xh * c) / rms;  over the rows:  dw = sum(dy * xh).
 #include "common.hpp"
 
+#include <type_traits>
+
 namespace cf {
 namespace {
 
@@ -27,8 +29,9 @@ struct AddNormArgs {
     float* descale;
     const float* qscale;      // Q_RECORD
     float* amax;
-    int H;
+    int rows, H;
     float eps;
+    int e5m2;
 };
 
 template <bool F32>
@@ -59,61 +62,305 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
     return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
 }
 
-// One workgroup per row, the row in LDS as fp32.
-template <bool F32, int QMODE, bool E5M2>
-__global__ __launch_bounds__(kThreads) void k_add_norm(const AddNormArgs p) {
-    extern __shared__ float ys[];
-    __shared__ float sh[4];
-    const int t = threadIdx.x, H = p.H;
-    const size_t base = static_cast<size_t>(blockIdx.x) * H;
-    float ss = 0.0f;
-    for (int i = t; i < H; i += kThreads) {
-        float h = load_stream<F32>(p.residual, base + i);
-        if (p.x) {
-            h += bf16_to_f32(p.x[base + i]);
-            if constexpr (!F32) h = bf16_to_f32(f32_to_bf16(h));
+// Eight elements at any alignment that one element has: gfx950 moves them in one instruction all the same.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// A row's last chunk, n < 8 elements (TAIL), is loaded whole where enough follows and cut afterwards: element by element the loads of the
+// last lane kept a row waiting for eight of them in turn (8192 x 4095: 88 us, 4096 43).  `whole`: the eight elements lie in the tensor.
+template <bool F32, bool TAIL>
+__device__ __forceinline__ void load8(const void* p, size_t at, int n, bool whole, float (&v)[8]) {
+    if (!TAIL || n >= 8 || whole) {
+        if constexpr (F32) {
+            const f32x4_any* q = reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + at);
+            const f32x4_any a = q[0], b = q[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        } else {
+            const u32x4_any a = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(a[i]); v[2 * i + 1] = bf16_hi(a[i]); }
         }
-        if (p.sum) store_stream<F32>(p.sum, base + i, h);
-        ys[i] = h;
-        ss = __builtin_fmaf(h, h, ss);
-    }
-    const float rms = sqrtf(block_sum(ss, sh) / static_cast<float>(H) + p.eps);
-    if (t == 0 && p.rms) p.rms[blockIdx.x] = rms;
-    const float inv = 1.0f / rms;
-    float amax = 0.0f;
-    for (int i = t; i < H; i += kThreads) {
-        const float y = ys[i] * inv * bf16_to_f32(p.weight[i]);
-        ys[i] = y;
-        amax = fmaxf(amax, fabsf(y));
-        if (p.normed) p.normed[base + i] = f32_to_bf16(y);
-    }
-    constexpr float F = E5M2 ? 57344.0f : 448.0f;
-    if constexpr (QMODE == Q_BLOCK) {
-        __syncthreads();
-        const int groups = (H + 127) / 128, wave = t >> 6, lane = t & 63;
-        for (int g = wave; g < groups; g += kThreads / kWave) {
-            const int i0 = g * 128 + lane, i1 = i0 + 64;
-            const float a0 = i0 < H ? ys[i0] : 0.0f, a1 = i1 < H ? ys[i1] : 0.0f;
-            const float a = fmaxf(wave_max(fmaxf(fabsf(a0), fabsf(a1))), 1e-12f), s = F / a;
-            if (lane == 0) {
-                p.scale[static_cast<size_t>(blockIdx.x) * groups + g] = s;
-                p.descale[static_cast<size_t>(blockIdx.x) * groups + g] = a / F;
-            }
-            if (i0 < H) p.q[base + i0] = cvt1_fp8<E5M2>(a0 * s);
-            if (i1 < H) p.q[base + i1] = cvt1_fp8<E5M2>(a1 * s);
+        if constexpr (TAIL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.0f;
         }
     } else {
-        amax = block_max(amax, sh);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? load_stream<F32>(p, at + i) : 0.0f;
+    }
+}
+// Eight weights as bf16 pairs.  A last chunk is the end of the eight elements that the weight ends with, moved down.
+template <bool TAIL>
+__device__ __forceinline__ u32x4_any load_weight(const uint16_t* w, int at, int n, int H) {
+    if (!TAIL || n >= 8) return *reinterpret_cast<const u32x4_any*>(w + at);
+    u32x4_any v = {0, 0, 0, 0};
+    if (H >= 8) {
+        v = *reinterpret_cast<const u32x4_any*>(w + H - 8);
+        const int down = 8 - n;
+        if (down & 4) v = u32x4_any{v[2], v[3], 0, 0};
+        if (down & 2) v = u32x4_any{v[1], v[2], v[3], 0};
+        if (down & 1) v = u32x4_any{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) v[i >> 1] |= static_cast<uint32_t>(w[at + i]) << (16 * (i & 1));
+    }
+    return v;
+}
+// Streaming stores, which leave through the L2 (plain ones: 8192 x 4096 45.4 us instead of 42.9, 16384 x 1024 25.3 instead of 21.6).  A last chunk
+// goes in pieces of four, two and one elements.
+template <bool TAIL>
+__device__ __forceinline__ void store8_bf16(uint16_t* p, size_t at, int n, const float (&v)[8]) {
+    u32x4_any o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2_hw(v[2 * i], v[2 * i + 1]);
+    if (!TAIL || n >= 8) {
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4_any*>(p + at));
+    } else {
+        typedef uint32_t u32_any __attribute__((aligned(2)));
+        uint16_t* q = p + at;
+        if (n & 4) {
+            reinterpret_cast<u32_any*>(q)[0] = o[0];
+            reinterpret_cast<u32_any*>(q)[1] = o[1];
+        }
+        if (n & 2) *reinterpret_cast<u32_any*>(q + (n & 4)) = (n & 4) ? o[2] : o[0];
+        if (n & 1) q[n - 1] = static_cast<uint16_t>(n == 1 ? o[0] : n == 3 ? o[1] : n == 5 ? o[2] : o[3]);
+    }
+}
+template <bool F32, bool TAIL>
+__device__ __forceinline__ void store8_stream(void* p, size_t at, int n, const float (&v)[8]) {
+    if constexpr (!F32) {
+        store8_bf16<TAIL>(static_cast<uint16_t*>(p), at, n, v);
+    } else {
+        f32x4_any* q = reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + at);
+        const f32x4_any a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+        if (!TAIL || n >= 4) __builtin_nontemporal_store(a, q);
+        if (!TAIL || n >= 8) {
+            __builtin_nontemporal_store(b, q + 1);
+        } else {
+            float* r = static_cast<float*>(p) + at;
+#pragma unroll
+            for (int i = 0; i < 7; ++i)
+                if (i >= (n & 4) && i < n) r[i] = v[i];
+        }
+    }
+}
+template <bool TAIL>
+__device__ __forceinline__ void store8_fp8(uint8_t* p, size_t at, int n, bool e5m2, bool finite, const float (&v)[8]) {
+    u32x2_any o;
+    if (finite) {
+        o.x = e5m2 ? cvt4_fp8_finite<true>(v[0], v[1], v[2], v[3]) : cvt4_fp8_finite<false>(v[0], v[1], v[2], v[3]);
+        o.y = e5m2 ? cvt4_fp8_finite<true>(v[4], v[5], v[6], v[7]) : cvt4_fp8_finite<false>(v[4], v[5], v[6], v[7]);
+    } else {
+        o.x = e5m2 ? cvt4_fp8<true>(v[0], v[1], v[2], v[3]) : cvt4_fp8<false>(v[0], v[1], v[2], v[3]);
+        o.y = e5m2 ? cvt4_fp8<true>(v[4], v[5], v[6], v[7]) : cvt4_fp8<false>(v[4], v[5], v[6], v[7]);
+    }
+    if (!TAIL || n >= 8) {
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x2_any*>(p + at));
+    } else {
+        typedef uint32_t u32_byte __attribute__((aligned(1)));
+        typedef uint16_t u16_byte __attribute__((aligned(1)));
+        uint8_t* q = p + at;
+        uint32_t rest = o.x;
+        if (n & 4) {
+            *reinterpret_cast<u32_byte*>(q) = o.x;
+            rest = o.y;
+            q += 4;
+        }
+        if (n & 2) {
+            *reinterpret_cast<u16_byte*>(q) = static_cast<uint16_t>(rest);
+            rest >>= 16;
+            q += 2;
+        }
+        if (n & 1) *q = static_cast<uint8_t>(rest);
+    }
+}
+
+// What a value is after the lanes of a group of 16 have exchanged it, by DPP: quad, half row, row.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    v = max(v, dpp<0xb1>(v));           // lane ^ 1
+    v = max(v, dpp<0x4e>(v));           // lane ^ 2
+    v = max(v, dpp<0x141>(v));          // the other quad of the half row
+    return max(v, dpp<0x140>(v));       // the other half of the row
+}
+__device__ __forceinline__ float add16(float v) {
+    v += __uint_as_float(dpp<0xb1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x4e>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
+    return v + __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+}
+// Over a row's threads, the same in each.  A row of more than one wavefront is a workgroup's only one; `sh` holds a word for each of its
+// wavefronts, at most 16, and is not used again.
+template <bool ONE_WAVE>
+__device__ __forceinline__ float row_sum(float v, float* sh) {
+    v = add16(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    if constexpr (!ONE_WAVE) {
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int w = threadIdx.x & 15;
+        v = add16(w < static_cast<int>(blockDim.x >> 6) ? sh[w] : 0.0f);
+    }
+    return v;
+}
+template <bool ONE_WAVE>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* sh) {
+    v = max16(v);
+    v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16, kWave)));
+    v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32, kWave)));
+    if constexpr (!ONE_WAVE) {
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int w = threadIdx.x & 15;
+        v = max16(w < static_cast<int>(blockDim.x >> 6) ? sh[w] : 0u);
+    }
+    return v;
+}
+
+constexpr uint32_t kInf = 0x7f800000u;
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// A row is held in registers, V chunks of eight elements a thread, chunk c by thread c % T: one read and one write of everything.  Sixteen
+// threads next to each other hold a scale group of 128.  TAIL: H is no multiple of 8, the last chunk is a part.
+// What bounds it: HBM, and for few rows the chain load - sum - maximum - store.  Both want a row on as many threads as it has chunks.  Threads a row x
+// chunks a thread, one row a workgroup (64: four rows), us:
+//     rows x H                        512 x 1   256 x 2   128 x 4    64 x 8   1024 x 1
+//     1 x 4096, bf16                    3.4       3.8       5.0       7.0       3.6
+//     512 x 4096                        4.6       4.8       6.2       8.7       5.4
+//     8192 x 4096                      42.0      44.0      46.4      56.8      57.0
+//     4000 x 7168, 1x128 scales           (512 x 2: 39.1)            100.0     38.4
+//     8192 x 4096, fp32, bf16 rows     79.6      82.4      90.8     107.5      74.8
+// So V = 1 up to H = 8192 and 2 beyond, with as many wavefronts as that takes; below 512 elements four rows share a workgroup.
+// Maxima are taken of the bits of |y|: they order like the values, with NaN above infinity, so one maximum also says whether
+// anything needs the slow conversion, which keeps NaN codes.
+template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
+__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNormArgs p) {
+    __shared__ float sh_sum[16];
+    __shared__ uint32_t sh_max[2][16];
+    const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
+    int row = blockIdx.x, t = threadIdx.x;
+    if constexpr (ONE_WAVE) {
+        row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+        t &= 63;
+        if (row >= p.rows) return;
+    }
+    const int chunks = TAIL ? (H + 7) / 8 : H / 8;
+    const size_t base = static_cast<size_t>(row) * H;
+    auto left = [&](int j) { return TAIL ? H - (t + j * T) * 8 : 8; };      // elements from chunk j of this thread on
+    auto has = [&](int j) { return t + j * T < chunks; };
+    const bool follows = static_cast<size_t>(p.rows - 1 - row) * H >= 7;         // elements behind this row, as many as a last chunk lacks
+
+    float h[V][8];
+    u32x4_any w[V];
+    {
+        float x[V][8];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j][i] = x[j][i] = 0.0f;
+            if (has(j)) {
+                load8<F32, TAIL>(p.residual, base + (t + j * T) * 8, left(j), follows, h[j]);
+                if (p.x) load8<false, TAIL>(p.x, base + (t + j * T) * 8, left(j), follows, x[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            w[j] = u32x4_any{0, 0, 0, 0};
+            if (has(j)) w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
+        }
+        if (p.x) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    h[j][i] += x[j][i];
+                    if constexpr (!F32) h[j][i] = round_bf16_hw(h[j][i]);
+                }
+        }
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (p.sum && has(j)) store8_stream<F32, TAIL>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
+        float part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[j][i], h[j][i], part);
+        ss += part;
+    }
+    const float rms = sqrtf(row_sum<ONE_WAVE>(ss, sh_sum) / static_cast<float>(H) + p.eps);
+    if (t == 0 && p.rms) p.rms[row] = rms;
+    const float inv = 1.0f / rms;
+
+    const float F = p.e5m2 ? 57344.0f : 448.0f;
+    uint32_t top[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        top[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            h[j][i] = h[j][i] * inv * ((i & 1) ? bf16_hi(w[j][i >> 1]) : bf16_lo(w[j][i >> 1]));        // y from here on
+            top[j] = max(top[j], abs_bits(h[j][i]));
+        }
+        if (p.normed && has(j)) store8_bf16<TAIL>(p.normed, base + (t + j * T) * 8, left(j), h[j]);
+    }
+    // the largest |y| of a chunk without its NaNs
+    auto number = [&](int j) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(h[j][i]));
+        return __float_as_uint(m);
+    };
+    auto quantize = [&](int j, float s, bool finite) {
+        if (!has(j)) return;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = h[j][i] * s;
+        store8_fp8<TAIL>(p.q, base + (t + j * T) * 8, left(j), p.e5m2, finite, v);
+    };
+    if constexpr (QMODE == Q_BLOCK) {
+        const int groups = (H + 127) >> 7;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            uint32_t m = max16(top[j]);
+            const bool finite = __all(m < kInf);
+            if (!finite) m = max16(number(j));
+            const float a = fmaxf(__uint_as_float(m), 1e-12f), s = F / a;
+            const int c = t + j * T;
+            if ((c & 15) == 0 && has(j)) {
+                p.scale[static_cast<size_t>(row) * groups + (c >> 4)] = s;
+                p.descale[static_cast<size_t>(row) * groups + (c >> 4)] = a / F;
+            }
+            quantize(j, s, finite);
+        }
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = max(m, top[j]);
+        m = row_max<ONE_WAVE>(m, sh_max[0]);
+        bool finite = m < kInf;
+        if (!finite) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) n = max(n, number(j));
+            m = row_max<ONE_WAVE>(n, sh_max[1]);
+        }
         float s;
         if constexpr (QMODE == Q_ROWS) {
-            const float a = fmaxf(amax, 1e-12f);
+            const float a = fmaxf(__uint_as_float(m), 1e-12f);
             s = F / a;
-            if (t == 0) { p.scale[blockIdx.x] = s; p.descale[blockIdx.x] = a / F; }
+            if (t == 0) { p.scale[row] = s; p.descale[row] = a / F; }
         } else {
             s = *p.qscale;
-            if (t == 0) atomic_max_nonneg(p.amax, amax);
+            if (t == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
+            finite = finite && abs_bits(s) < kInf;         // 0 times infinity
         }
-        for (int i = t; i < H; i += kThreads) p.q[base + i] = cvt1_fp8<E5M2>(ys[i] * s);
+#pragma unroll
+        for (int j = 0; j < V; ++j) quantize(j, s, finite);
     }
 }
 
@@ -184,15 +431,23 @@ int check_shape(int rows, int H) {
 }
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
+template <bool F32, int QMODE, bool TAIL>
+int launch_add_norm(const AddNormArgs& p, hipStream_t st) {
+    const int chunks = (p.H + 7) / 8;
+    const auto waves = [&](int v) { return (chunks + kWave * v - 1) / (kWave * v) * kWave; };
+    if (chunks <= kWave) k_add_norm<F32, QMODE, TAIL, true, 1><<<ceil_div(p.rows, 4), 256, 0, st>>>(p);
+    else if (chunks <= 1024) k_add_norm<F32, QMODE, TAIL, false, 1><<<p.rows, waves(1), 0, st>>>(p);
+    else k_add_norm<F32, QMODE, TAIL, false, 2><<<p.rows, waves(2), 0, st>>>(p);
+    return launch_status();
+}
+
 template <int QMODE>
-int add_norm(const AddNormArgs& p, bool f32, bool e5m2, int rows, cf_stream_t stream) {
+int add_norm(AddNormArgs p, bool f32, bool e5m2, int rows, cf_stream_t stream) {
     hipStream_t st = as_stream(stream);
-    auto go = [&](auto kernel) {
-        kernel<<<rows, kThreads, static_cast<size_t>(p.H) * 4, st>>>(p);
-        return launch_status();
-    };
-    if (f32) return e5m2 ? go(k_add_norm<true, QMODE, true>) : go(k_add_norm<true, QMODE, false>);
-    return e5m2 ? go(k_add_norm<false, QMODE, true>) : go(k_add_norm<false, QMODE, false>);
+    p.rows = rows;
+    p.e5m2 = e5m2;
+    if (p.H % 8 != 0) return f32 ? launch_add_norm<true, QMODE, true>(p, st) : launch_add_norm<false, QMODE, true>(p, st);
+    return f32 ? launch_add_norm<true, QMODE, false>(p, st) : launch_add_norm<false, QMODE, false>(p, st);
 }
 
 // what the three forward entry points ask of the arguments they share
