@@ -13,7 +13,6 @@ namespace cf {
 namespace {
 
 constexpr int kMaxH = 16384;
-constexpr int kThreads = 256;
 
 enum { Q_ROWS = 0, Q_BLOCK = 1, Q_RECORD = 2 };
 
@@ -34,62 +33,46 @@ struct AddNormArgs {
     int e5m2;
 };
 
-template <bool F32>
-__device__ __forceinline__ float load_stream(const void* p, size_t i) {
-    if constexpr (F32) return static_cast<const float*>(p)[i];
-    else return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
-}
-template <bool F32>
-__device__ __forceinline__ void store_stream(void* p, size_t i, float v) {
-    if constexpr (F32) static_cast<float*>(p)[i] = v;
-    else static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
-}
-
-// sum (or maximum) over the workgroup of four wavefronts, the same in every thread
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
-}
-__device__ __forceinline__ float block_max(float v, float* sh) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-}
-
 // Eight elements at any alignment that one element has: gfx950 moves them in one instruction all the same.
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-// A row's last chunk, n < 8 elements (TAIL), is loaded whole where enough follows and cut afterwards: element by element the loads of the
-// last lane kept a row waiting for eight of them in turn (8192 x 4095: 88 us, 4096 43).  `whole`: the eight elements lie in the tensor.
+// Eight elements as they lie in memory; converted where they are used, so that a load on its way is not waited for.
+template <bool F32>
+struct Raw8 {
+    u32x4_any v[F32 ? 2 : 1];
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (F32) return __uint_as_float(v[i >> 2][i & 3]);
+        else return (i & 1) ? bf16_hi(v[0][i >> 1]) : bf16_lo(v[0][i >> 1]);
+    }
+};
+// A row's last chunk, n < 8 elements (TAIL), is loaded whole where enough follows, and cut when it is used: element by element the loads of the
+// last lane kept a row waiting for eight of them in turn (8192 x 4095: 88 us, now 55; 4096 43).  `whole`: the eight elements lie in the tensor.
 template <bool F32, bool TAIL>
-__device__ __forceinline__ void load8(const void* p, size_t at, int n, bool whole, float (&v)[8]) {
+__device__ __forceinline__ void load8(const void* p, size_t at, int n, bool whole, Raw8<F32>& r) {
     if (!TAIL || n >= 8 || whole) {
-        if constexpr (F32) {
-            const f32x4_any* q = reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + at);
-            const f32x4_any a = q[0], b = q[1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-        } else {
-            const u32x4_any a = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(a[i]); v[2 * i + 1] = bf16_hi(a[i]); }
-        }
-        if constexpr (TAIL) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.0f;
-        }
+        const u32x4_any* q = F32 ? reinterpret_cast<const u32x4_any*>(static_cast<const float*>(p) + at)
+                                 : reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(p) + at);
+        r.v[0] = q[0];
+        if constexpr (F32) r.v[1] = q[1];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? load_stream<F32>(p, at + i) : 0.0f;
+        for (int i = 0; i < 8; ++i)
+            if (i < n) {
+                if constexpr (F32) r.v[i >> 2][i & 3] = static_cast<const uint32_t*>(p)[at + i];
+                else r.v[0][i >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p)[at + i]) << (16 * (i & 1));
+            }
     }
+}
+template <bool F32>
+__device__ __forceinline__ void clear8(Raw8<F32>& r) {
+    r.v[0] = u32x4_any{0, 0, 0, 0};
+    if constexpr (F32) r.v[1] = u32x4_any{0, 0, 0, 0};
+}
+template <bool F32, bool TAIL>
+__device__ __forceinline__ float value8(const Raw8<F32>& r, int i, int n) {
+    return !TAIL || i < n ? r.at(i) : 0.0f;
 }
 // Eight weights as bf16 pairs.  A last chunk is the end of the eight elements that the weight ends with, moved down.
 template <bool TAIL>
@@ -225,6 +208,19 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* sh) {
 constexpr uint32_t kInf = 0x7f800000u;
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// Raising one maximum from every row.  Atomics on one address take turns, and the rows that run first all find the value they start from: with an
+// atomic from each row that finds its own the larger, 1000 rows of 4096 took 15.8 us, 7.8 with a scale a row; 8192 (fp32) 94 and 78, 32768 x 1024 86 and 51.  So one
+// row in 128 raises it as soon as it knows its own; the others look again behind their stores and a microsecond and a half: 10.8, 84 and 61 us.
+__device__ __forceinline__ void raise_first(float* amax, uint32_t m, int row, float& before) {
+    before = atomic_load_agent(amax);
+    if (row % 128 == 0 && __uint_as_float(m) > before) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
+}
+__device__ __forceinline__ void raise_last(float* amax, uint32_t m, int row, float before) {
+    if (row % 128 == 0 || __uint_as_float(m) <= before) return;
+    __builtin_amdgcn_s_sleep(48);           // 3072 cycles
+    if (__uint_as_float(m) > atomic_load_agent(amax)) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
+}
+
 // A row is held in registers, V chunks of eight elements a thread, chunk c by thread c % T: one read and one write of everything.  Sixteen
 // threads next to each other hold a scale group of 128.  TAIL: H is no multiple of 8, the last chunk is a part.
 // What bounds it: HBM, and for few rows the chain load - sum - maximum - store.  Both want a row on as many threads as it has chunks.  Threads a row x
@@ -258,30 +254,29 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNor
     float h[V][8];
     u32x4_any w[V];
     {
-        float x[V][8];
+        Raw8<F32> r[V];
+        Raw8<false> x[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) h[j][i] = x[j][i] = 0.0f;
+            clear8(r[j]);
+            clear8(x[j]);
+            w[j] = u32x4_any{0, 0, 0, 0};
             if (has(j)) {
-                load8<F32, TAIL>(p.residual, base + (t + j * T) * 8, left(j), follows, h[j]);
+                load8<F32, TAIL>(p.residual, base + (t + j * T) * 8, left(j), follows, r[j]);
                 if (p.x) load8<false, TAIL>(p.x, base + (t + j * T) * 8, left(j), follows, x[j]);
+                w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
             }
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            w[j] = u32x4_any{0, 0, 0, 0};
-            if (has(j)) w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
-        }
-        if (p.x) {
+        for (int j = 0; j < V; ++j)
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    h[j][i] += x[j][i];
+            for (int i = 0; i < 8; ++i) {
+                h[j][i] = value8<F32, TAIL>(r[j], i, left(j));
+                if (p.x) {
+                    h[j][i] += value8<false, TAIL>(x[j], i, left(j));
                     if constexpr (!F32) h[j][i] = round_bf16_hw(h[j][i]);
                 }
-        }
+            }
     }
     float ss = 0.0f;
 #pragma unroll
@@ -349,18 +344,21 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNor
             for (int j = 0; j < V; ++j) n = max(n, number(j));
             m = row_max<ONE_WAVE>(n, sh_max[1]);
         }
-        float s;
+        float s, before = 0.0f;
         if constexpr (QMODE == Q_ROWS) {
             const float a = fmaxf(__uint_as_float(m), 1e-12f);
             s = F / a;
             if (t == 0) { p.scale[row] = s; p.descale[row] = a / F; }
         } else {
             s = *p.qscale;
-            if (t == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
+            if (t == 0) raise_first(p.amax, m, row, before);
             finite = finite && abs_bits(s) < kInf;         // 0 times infinity
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) quantize(j, s, finite);
+        if constexpr (QMODE == Q_RECORD) {
+            if (t == 0) raise_last(p.amax, m, row, before);
+        }
     }
 }
 
@@ -372,55 +370,166 @@ struct AddNormGradArgs {
     const void* dh;           // [rows, H] the residual stream's gradient, or null
     void* dr;                 // [rows, H]
     float* partial;           // [parts, H]
+    float* part_amax;         // [parts]
     uint8_t* q;               // [rows, H] E5M2, or null
     const float* qscale;
     float* amax;
     int rows, H;
 };
 
-// Workgroup b takes rows b, b + parts, ... and leaves its share of dw, gathered in LDS, in partial[b].
-template <bool F32>
-__global__ __launch_bounds__(kThreads) void k_add_norm_grad(const AddNormGradArgs p) {
-    extern __shared__ float dw[];
-    __shared__ float sh[4];
-    const int t = threadIdx.x, H = p.H;
-    for (int i = t; i < H; i += kThreads) dw[i] = 0.0f;
-    float amax = 0.0f;
-    const float s = p.q ? *p.qscale : 0.0f;
-    for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+// Workgroup b takes rows b, b + parts, ... as k_add_norm holds one, loads the next row's operands before it works on one, and leaves its share of
+// dw in partial[b].  ONE_WAVE: four rows at a time, one a wavefront, whose shares are added in LDS.
+template <bool F32, bool QUANT, bool TAIL, bool ONE_WAVE, int V>
+__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm_grad(const AddNormGradArgs p) {
+    __shared__ float sh[2][16];
+    __shared__ float sh_dw[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
+    const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
+    const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
+    const int first = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
+    const int step = ONE_WAVE ? gridDim.x * 4 : gridDim.x;
+    const int chunks = TAIL ? (H + 7) / 8 : H / 8;
+    auto left = [&](int j) { return TAIL ? H - (t + j * T) * 8 : 8; };
+    auto has = [&](int j) { return t + j * T < chunks; };
+
+    struct Row {
+        Raw8<false> dy[V];
+        Raw8<F32> h[V], dh[V];
+        float rms;
+    };
+    auto load = [&](Row& r, int row) {
         const size_t base = static_cast<size_t>(row) * H;
-        const float inv = 1.0f / p.rms[row];
-        float dot = 0.0f;
-        for (int i = t; i < H; i += kThreads) {
-            const float xh = load_stream<F32>(p.sum, base + i) * inv, dy = bf16_to_f32(p.dy[base + i]);
-            dw[i] = __builtin_fmaf(dy, xh, dw[i]);
-            dot = __builtin_fmaf(dy * bf16_to_f32(p.weight[i]), xh, dot);
+        const bool follows = static_cast<size_t>(p.rows - 1 - row) * H >= 7;
+        r.rms = p.rms[row];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            clear8(r.dy[j]);
+            clear8(r.h[j]);
+            clear8(r.dh[j]);
+            if (has(j)) {
+                load8<false, TAIL>(p.dy, base + (t + j * T) * 8, left(j), follows, r.dy[j]);
+                load8<F32, TAIL>(p.sum, base + (t + j * T) * 8, left(j), follows, r.h[j]);
+                if (p.dh) load8<F32, TAIL>(p.dh, base + (t + j * T) * 8, left(j), follows, r.dh[j]);
+            }
         }
-        const float c = block_sum(dot, sh) / static_cast<float>(H);
-        for (int i = t; i < H; i += kThreads) {
-            const float xh = load_stream<F32>(p.sum, base + i) * inv, g = bf16_to_f32(p.dy[base + i]) * bf16_to_f32(p.weight[i]);
-            const float d = __builtin_fmaf(__builtin_fmaf(-xh, c, g), inv, p.dh ? load_stream<F32>(p.dh, base + i) : 0.0f);
-            store_stream<F32>(p.dr, base + i, d);
-            if (p.q) {
-                p.q[base + i] = cvt1_fp8<true>(d * s);
-                amax = fmaxf(amax, fabsf(d));
+    };
+    u32x4_any w[V];
+    float dw[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w[j] = u32x4_any{0, 0, 0, 0};
+        if (has(j)) w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[j][i] = 0.0f;
+    }
+    const float s = QUANT ? *p.qscale : 0.0f;
+    const bool s_finite = abs_bits(s) < kInf;
+    float amax = 0.0f;
+    constexpr bool AHEAD = V == 1;          // 1024 threads have 128 registers each, too few for two rows of two chunks
+    Row r, next;
+    if (AHEAD && first < p.rows) load(next, first);
+    int turn = 0;
+    for (int row = first; row < p.rows; row += step, turn ^= 1) {
+        if constexpr (AHEAD) {
+            r = next;
+            if (row + step < p.rows) load(next, row + step);
+        } else {
+            load(r, row);
+        }
+        const size_t base = static_cast<size_t>(row) * H;
+        const float inv = 1.0f / r.rms;
+        float dot = 0.0f;
+        float xh[V][8], g[V][8];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float dy = value8<false, TAIL>(r.dy[j], i, left(j));
+                xh[j][i] = value8<F32, TAIL>(r.h[j], i, left(j)) * inv;
+                dw[j][i] = __builtin_fmaf(dy, xh[j][i], dw[j][i]);
+                g[j][i] = dy * ((i & 1) ? bf16_hi(w[j][i >> 1]) : bf16_lo(w[j][i >> 1]));
+                dot = __builtin_fmaf(g[j][i], xh[j][i], dot);
+            }
+        const float c = row_sum<ONE_WAVE>(dot, sh[turn]) / static_cast<float>(H);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float d[8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                d[i] = __builtin_fmaf(__builtin_fmaf(-xh[j][i], c, g[j][i]), inv, value8<F32, TAIL>(r.dh[j], i, left(j)));
+                if constexpr (QUANT) {
+                    amax = fmaxf(amax, fabsf(d[i]));
+                    top = max(top, abs_bits(d[i]));
+                }
+            }
+            if (has(j)) store8_stream<F32, TAIL>(p.dr, base + (t + j * T) * 8, left(j), d);
+            if constexpr (QUANT) {
+                const bool finite = __all(top < kInf) && s_finite;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] *= s;
+                if (has(j)) store8_fp8<TAIL>(p.q, base + (t + j * T) * 8, left(j), true, finite, d);
             }
         }
     }
-    if (p.q) {
-        amax = block_max(amax, sh);
-        if (t == 0) atomic_max_nonneg(p.amax, amax);
+    float* part = p.partial + static_cast<size_t>(blockIdx.x) * H;
+    if constexpr (ONE_WAVE) {
+        static_assert(V == 1);
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sh_dw[wave][t * 8 + i] = dw[0][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < H; i += 256) part[i] = (sh_dw[0][i] + sh_dw[1][i]) + (sh_dw[2][i] + sh_dw[3][i]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (has(j)) {
+                const int at = (t + j * T) * 8;
+                if (!TAIL || left(j) >= 8) {
+                    reinterpret_cast<f32x4_any*>(part + at)[0] = f32x4_any{dw[j][0], dw[j][1], dw[j][2], dw[j][3]};
+                    reinterpret_cast<f32x4_any*>(part + at)[1] = f32x4_any{dw[j][4], dw[j][5], dw[j][6], dw[j][7]};
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < left(j)) part[at + i] = dw[j][i];
+                }
+            }
     }
-    for (int i = t; i < H; i += kThreads) p.partial[static_cast<size_t>(blockIdx.x) * H + i] = dw[i];
+    if constexpr (QUANT) {
+        __syncthreads();
+        const uint32_t m = row_max<false>(__float_as_uint(amax), reinterpret_cast<uint32_t*>(sh[0]));
+        if (threadIdx.x == 0) p.part_amax[blockIdx.x] = __uint_as_float(m);
+    }
 }
 
-// dw[i] = (dw[i] +) the parts' shares, in their order
-__global__ __launch_bounds__(kThreads) void k_sum_parts(const float* partial, float* dw, int H, int parts, int accumulate) {
-    const int i = blockIdx.x * kThreads + threadIdx.x;
-    if (i >= H) return;
+// dw[i] = (dw[i] +) the parts' shares: 32 columns a workgroup, 32 threads to a column that take every 32nd part and are added in order.
+// The workgroup behind them raises *amax to the parts' maxima.
+constexpr int kSumColumns = 32, kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void k_sum_parts(const float* __restrict__ partial, float* __restrict__ dw, int H, int parts, int accumulate,
+                                                           const float* __restrict__ part_amax, float* __restrict__ amax) {
+    constexpr int kGroups = kSumThreads / kSumColumns;
+    __shared__ float sh[kSumThreads];
+    const int t = threadIdx.x;
+    if (static_cast<int>(blockIdx.x) * kSumColumns >= H) {
+        uint32_t m = 0;
+        for (int b = t; b < parts; b += kSumThreads) m = max(m, __float_as_uint(part_amax[b]));
+        m = row_max<false>(m, reinterpret_cast<uint32_t*>(sh));
+        if (t == 0) atomic_max_nonneg(amax, __uint_as_float(m));
+        return;
+    }
+    const int column = blockIdx.x * kSumColumns + t % kSumColumns, group = t / kSumColumns;
     float v = 0.0f;
-    for (int b = 0; b < parts; ++b) v += partial[static_cast<size_t>(b) * H + i];
-    dw[i] = accumulate ? dw[i] + v : v;
+    if (column < H) {
+#pragma unroll 8
+        for (int b = group; b < parts; b += kGroups) v += partial[static_cast<size_t>(b) * H + column];
+    }
+    sh[t] = v;
+    __syncthreads();
+    if (group == 0 && column < H) {
+        v = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) v += sh[g * kSumColumns + t];
+        dw[column] = accumulate ? dw[column] + v : v;
+    }
 }
 
 // 0: run, 1: nothing to do, < 0: error
@@ -431,13 +540,15 @@ int check_shape(int rows, int H) {
 }
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
+// threads of a row, V chunks each
+constexpr int row_threads(int H, int V) { return ((H + 7) / 8 + kWave * V - 1) / (kWave * V) * kWave; }
+constexpr int kOneWaveH = 8 * kWave, kOneChunkH = 8 * 1024;
+
 template <bool F32, int QMODE, bool TAIL>
 int launch_add_norm(const AddNormArgs& p, hipStream_t st) {
-    const int chunks = (p.H + 7) / 8;
-    const auto waves = [&](int v) { return (chunks + kWave * v - 1) / (kWave * v) * kWave; };
-    if (chunks <= kWave) k_add_norm<F32, QMODE, TAIL, true, 1><<<ceil_div(p.rows, 4), 256, 0, st>>>(p);
-    else if (chunks <= 1024) k_add_norm<F32, QMODE, TAIL, false, 1><<<p.rows, waves(1), 0, st>>>(p);
-    else k_add_norm<F32, QMODE, TAIL, false, 2><<<p.rows, waves(2), 0, st>>>(p);
+    if (p.H <= kOneWaveH) k_add_norm<F32, QMODE, TAIL, true, 1><<<ceil_div(p.rows, 4), 4 * kWave, 0, st>>>(p);
+    else if (p.H <= kOneChunkH) k_add_norm<F32, QMODE, TAIL, false, 1><<<p.rows, row_threads(p.H, 1), 0, st>>>(p);
+    else k_add_norm<F32, QMODE, TAIL, false, 2><<<p.rows, row_threads(p.H, 2), 0, st>>>(p);
     return launch_status();
 }
 
@@ -469,7 +580,26 @@ AddNormArgs forward_args(const void* d_residual, const uint16_t* d_x, const uint
     return p;
 }
 
-int grad_parts(int rows) { return rows < 1024 ? rows : 1024; }
+// Workgroups of the backward pass, each with a share of dw that is written and read once more: eight wavefronts a CU, which keep HBM busy with
+// the next row's operands on their way, and a workgroup on each of 256 CUs at least.  8192 x 4096 bf16, 8 wavefronts a workgroup: 256 57.9 us, 512 62.5, 1024 66.0;
+// 32768 x 1024, 2 of them: 256 101, 512 67.6, 1024 58.0, 2048 66.5; 65536 x 512, 4 rows a workgroup: 256 70.4, 512 58.2, 1024 64.2.
+// But four turns each, or the shares cost more than the rows: 1000 x 1000 with a workgroup a row 14.3, with 256 8.8.
+int grad_parts(int rows, int H) {
+    const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kOneChunkH ? 1 : 2) / kWave;
+    const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;
+    int parts = waves < 8 ? 2048 / waves : 256;
+    parts = parts < turns / 4 ? parts : turns / 4;
+    parts = parts > 256 ? parts : 256;
+    return parts < turns ? parts : turns;
+}
+size_t grad_workspace(int rows, int H) { return static_cast<size_t>(grad_parts(rows, H)) * (static_cast<size_t>(H) + 1) * 4; }
+
+template <bool F32, bool QUANT, bool TAIL>
+void launch_grad(const AddNormGradArgs& p, int parts, hipStream_t st) {
+    if (p.H <= kOneWaveH) k_add_norm_grad<F32, QUANT, TAIL, true, 1><<<parts, 4 * kWave, 0, st>>>(p);
+    else if (p.H <= kOneChunkH) k_add_norm_grad<F32, QUANT, TAIL, false, 1><<<parts, row_threads(p.H, 1), 0, st>>>(p);
+    else k_add_norm_grad<F32, QUANT, TAIL, false, 2><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+}
 
 int add_norm_grad(AddNormGradArgs p, int f32, float* d_grad_scale, int accumulate, void* d_workspace, size_t workspace_bytes,
                   cf_stream_t stream) {
@@ -477,7 +607,7 @@ int add_norm_grad(AddNormGradArgs p, int f32, float* d_grad_scale, int accumulat
     if (!d_grad_scale || misaligned(d_grad_scale, 4)) return CF_ERR_INVALID_ARG;
     if (p.rows == 0) {              // no rows: their sum is zero
         if (accumulate) return CF_OK;
-        k_sum_parts<<<ceil_div(p.H, kThreads), kThreads, 0, as_stream(stream)>>>(nullptr, d_grad_scale, p.H, 0, 0);
+        k_sum_parts<<<ceil_div(p.H, kSumColumns), kSumThreads, 0, as_stream(stream)>>>(nullptr, d_grad_scale, p.H, 0, 0, nullptr, nullptr);
         return launch_status();
     }
     if (!p.dy || !p.sum || !p.weight || !p.rms || !p.dr || !d_workspace) return CF_ERR_INVALID_ARG;
@@ -485,14 +615,19 @@ int add_norm_grad(AddNormGradArgs p, int f32, float* d_grad_scale, int accumulat
     if (misaligned(p.dy, 2) || misaligned(p.sum, el) || misaligned(p.weight, 2) || misaligned(p.rms, 4) || misaligned(p.dh, el) ||
         misaligned(p.dr, el) || misaligned(d_workspace, 16))
         return CF_ERR_INVALID_ARG;
-    const int parts = grad_parts(p.rows);
-    if (workspace_bytes < static_cast<size_t>(parts) * p.H * 4) return CF_ERR_INVALID_ARG;
+    const int parts = grad_parts(p.rows, p.H);
+    if (workspace_bytes < grad_workspace(p.rows, p.H)) return CF_ERR_INVALID_ARG;
     p.partial = static_cast<float*>(d_workspace);
+    p.part_amax = p.partial + static_cast<size_t>(parts) * p.H;
     hipStream_t st = as_stream(stream);
-    const size_t lds = static_cast<size_t>(p.H) * 4;
-    if (f32) k_add_norm_grad<true><<<parts, kThreads, lds, st>>>(p);
-    else k_add_norm_grad<false><<<parts, kThreads, lds, st>>>(p);
-    k_sum_parts<<<ceil_div(p.H, kThreads), kThreads, 0, st>>>(p.partial, d_grad_scale, p.H, parts, accumulate);
+    auto go = [&](auto stream_f32, auto quant) {
+        constexpr bool F32 = decltype(stream_f32)::value, QUANT = decltype(quant)::value;
+        if (p.H % 8 != 0) launch_grad<F32, QUANT, true>(p, parts, st);
+        else launch_grad<F32, QUANT, false>(p, parts, st);
+    };
+    if (f32) p.q ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+    else p.q ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
+    k_sum_parts<<<ceil_div(p.H, kSumColumns) + (p.q ? 1 : 0), kSumThreads, 0, st>>>(p.partial, d_grad_scale, p.H, parts, accumulate, p.part_amax, p.amax);
     return launch_status();
 }
 
@@ -542,7 +677,7 @@ int cf_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, 
 int cf_add_rmsnorm_backward_workspace_bytes(int rows, int H, size_t* bytes) {
     if (rows < 0 || H < 0 || !bytes) return CF_ERR_INVALID_ARG;
     if (H > kMaxH) return CF_ERR_UNSUPPORTED;
-    *bytes = static_cast<size_t>(grad_parts(rows)) * H * 4;
+    *bytes = grad_workspace(rows, H);
     return CF_OK;
 }
 
