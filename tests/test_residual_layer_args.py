@@ -75,6 +75,32 @@ def test_gradient_list(cf):
     assert fill(outs=(P, 0, 0)) == -1 and fill(outs=(P + 2, 0, P)) == -1 and fill(outs=(P, 0, P)) == 0
 
 
+def test_gradient_list_stays_in_its_bytes(cf):
+    """Whatever the alignment cuts a tensor's first entry to: the bytes that the size names are written, those behind them are not."""
+    for count in (1, 7, 8, 4095, 8191, 16377, 16378, 16383, 16384, 16385, 32768, 32769, 49145, 49152, 100_000):
+        for kind, el in ((0, 2), (1, 4)):
+            for shift in range(0, 16, el):
+                n = ctypes.c_size_t(0)
+                counts, types = torch.tensor([count, count], dtype=torch.int64), torch.tensor([kind, kind], dtype=torch.int32)
+                ptrs = torch.tensor([P + shift, P + shift], dtype=torch.int64)
+                assert cf.raw_cf_grad_list_bytes(counts.data_ptr(), 2, ctypes.byref(n)) == 0
+                image = torch.full((n.value + 4096,), 0xa5, dtype=torch.uint8)
+                assert cf.raw_cf_grad_list_fill(ptrs.data_ptr(), None, counts.data_ptr(), types.data_ptr(), 2, image.data_ptr(), n.value) == 0
+                assert bool((image[n.value:] == 0xa5).all())
+                # every element of both tensors once, in order, and nothing else: (address, address, count, type, 0) an entry
+                at, seen = [P + shift, P + shift], 0
+                entries = image[:n.value].view(torch.int64).view(-1, 4)
+                for src, dst, what, pad in entries.tolist():
+                    length, f32 = what & 0xffffffff, what >> 32
+                    if length == 0:
+                        continue
+                    which = 0 if seen < count else 1
+                    assert src == dst == at[which] and f32 == kind and pad == 0
+                    at[which] += length * el
+                    seen += length
+                assert seen == 2 * count
+
+
 def test_gradient_norm_refusals(cf):
     n = ctypes.c_size_t(0)
     assert cf.raw_cf_grad_norm_workspace_bytes(ctypes.byref(n)) == 0 and cf.raw_cf_grad_norm_workspace_bytes(None) == -1
