@@ -2512,7 +2512,7 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     hipStream_t st = as_stream(stream);
     const int max_row_tiles = total_rows / BM + num_experts;
     int* tile_map = static_cast<int*>(d_workspace);
-    if (build_map) k_build_tile_map<<<1, 64, 0, st>>>(d_counts, d_offsets, num_experts, max_row_tiles, total_rows, tile_map);
+    if (build_map && scale_mode != SCALE_BLOCK) k_build_tile_map<<<1, 64, 0, st>>>(d_counts, d_offsets, num_experts, max_row_tiles, total_rows, tile_map);
     GemmArgs p{};
     p.M = total_rows; p.N = N; p.K = K;
     p.A = static_cast<const uint8_t*>(A); p.lda = lda;
@@ -2528,7 +2528,7 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     const int out_bn = epilogue == EPI_SILU_GATE ? BN / 2 : BN;
     p.tiles_m = p.map_entries = max_row_tiles;
     p.tiles_n = (N + out_bn - 1) / out_bn;
-    if (scale_mode == SCALE_BLOCK) return grouped_gemm_nt_block(p, total_rows, num_experts, st);
+    if (scale_mode == SCALE_BLOCK) return grouped_gemm_nt_block(p, d_counts, d_offsets, total_rows, num_experts, st);
     // Few rows per expert: the small-tile kernel, which walks an expert's rows 16 mb at a time, where its estimate is lower.
     // It is sized for half as many rows again as the bound's average, so that most experts take one pass over their weights;
     // beyond 40 rows that is more than its largest pass.  The counts are on the device, so the choice is for balanced experts: 64 of

@@ -30,9 +30,90 @@ constexpr int kWideOut = kWideSb + 2 * 2 * kWideMaxKb * 4;      // 2 KiB per wav
 constexpr int kWideLds = kWideOut + 8 * 2048;           // 153,600 bytes
 constexpr int kWideWaitVm0 = 0x0f70;                    // s_waitcnt vmcnt(0) only
 
+// ---- the grouped form's table of row tiles ----
+// Word 0: the number of tiles of `rows` rows; then three words per expert, its first row, the row behind its last and its first tile; then
+// the expert of each tile.  It fits the bytes of the table of build_tile_map for tiles of 128 or 256 rows.
+constexpr int kExpertWords = 3;
+constexpr int kTableThreads = 256;
+__global__ __launch_bounds__(kTableThreads) void k_build_block_table(const int* __restrict__ counts, const int* __restrict__ offsets, int num_experts,
+                                                                     int total_rows, int tile_rows, int max_tiles, int* __restrict__ table) {
+    __shared__ int sh_first[kTableThreads], sh_tiles[kTableThreads], sh_wave[kTableThreads / kWave], sh_written;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int* const experts = table + 1;
+    int* const tiles = table + 1 + kExpertWords * num_experts;
+    int carry = 0;
+    if (t == 0) sh_written = 0;
+    for (int e0 = 0; e0 < num_experts; e0 += kTableThreads) {
+        const int e = e0 + t;
+        int first = 0, kept = 0;
+        if (e < num_experts) {
+            first = offsets[e];
+            kept = first >= 0 && first < total_rows ? max(0, min(counts[e], total_rows - first)) : 0;
+        }
+        const int n = (kept + tile_rows - 1) / tile_rows;
+        int incl = n;
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const int v = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += v;
+        }
+        if (lane == 63) sh_wave[wave] = incl;
+        __syncthreads();
+        int before = carry;
+        for (int w = 0; w < wave; ++w) before += sh_wave[w];
+        const int at = before + incl - n;
+        sh_first[t] = at;
+        // always all of them when the experts' ranges do not overlap; otherwise the ones that fit come first and the table ends with them
+        sh_tiles[t] = at + n <= max_tiles ? n : 0;
+        if (sh_tiles[t] > 0) atomicMax(&sh_written, at + n);
+        if (e < num_experts) {
+            experts[kExpertWords * e] = first;
+            experts[kExpertWords * e + 1] = first + kept;
+            experts[kExpertWords * e + 2] = at;
+        }
+        int all = carry;
+        for (int w = 0; w < kTableThreads / kWave; ++w) all += sh_wave[w];
+        __syncthreads();
+        for (int i = wave; i < kTableThreads; i += kTableThreads / kWave)
+            for (int k = lane; k < sh_tiles[i]; k += kWave) tiles[sh_first[i] + k] = e0 + i;
+        carry = all;
+        __syncthreads();
+    }
+    if (t == 0) table[0] = sh_written;
+}
+
+// Where the tile at `lin` of the walk lies.  Dense: the patches of tile_coords.  Grouped: an expert's tiles in groups of four column tiles, its row
+// tiles varying fastest.
+struct Spot { int m0, m_end, n0, expert; };
+template <bool GROUPED, int TM, int TN>
+__device__ __forceinline__ Spot locate(const GemmArgs& p, int lin) {
+    Spot s;
+    if constexpr (GROUPED) {
+        constexpr int GN = 4;
+        const int* const experts = p.tile_map + 1;
+        s.expert = __builtin_amdgcn_readfirstlane(experts[kExpertWords * p.map_entries + lin / p.tiles_n]);
+        const int* const e = experts + kExpertWords * s.expert;
+        const int first = __builtin_amdgcn_readfirstlane(e[0]), last = __builtin_amdgcn_readfirstlane(e[1]);
+        const int local = lin - __builtin_amdgcn_readfirstlane(e[2]) * p.tiles_n, n = (last - first + TM - 1) / TM;
+        const int g = local / (n * GN), within = local - g * (n * GN);
+        s.m0 = first + within % n * TM;
+        s.m_end = last;
+        s.n0 = (g * GN + within / n) * TN;
+    } else {
+        int tm, tn;
+        tile_coords(lin, p.tiles_m, p.tiles_n, tm, tn);
+        s.m0 = tm * TM;
+        s.m_end = p.M;
+        s.n0 = tn * TN;
+        s.expert = 0;
+    }
+    return s;
+}
+
 // 16-byte pieces of a row are xor-swizzled: the 16-lane groups of a ds_read_b128 meet 16 different slots (the pattern repeats every 16 rows)
 __device__ __forceinline__ int swz_rows16(int row) { return (row ^ ((row >> 3) & 1)) & 7; }
 
+template <bool GROUPED>
 __global__ __launch_bounds__(kWideThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_gemm_nt_block_wide(const GemmArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -40,7 +121,7 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);      // 0..7
     const int wm = wave & 3, wn = wave >> 2;              // 64 rows x 128 columns: the four wavefronts of a wn share a column block
     const int ktiles = p.K / BK;          // >= 3, checked by the launcher; also the number of scale groups along K
-    const int total_tiles = p.tiles_m * p.tiles_n;
+    const int total_tiles = (GROUPED ? __builtin_amdgcn_readfirstlane(p.tile_map[0]) : p.tiles_m) * p.tiles_n;
     int my_tiles, lin0, lstep;
     if (gridDim.x % kXcds == 0) {
         const int per = (total_tiles + kXcds - 1) / kXcds;
@@ -55,29 +136,45 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
         lin0 = blockIdx.x;
     }
     if (my_tiles <= 0) return;
-    auto tile_at = [&](int seq, int& m0, int& n0) {
-        int tm, tn;
-        tile_coords(lin0 + seq * lstep, p.tiles_m, p.tiles_n, tm, tn);
-        m0 = tm * BM;
-        n0 = tn * BN;
-    };
+    auto spot = [&](int seq) { return locate<GROUPED, BM, BN>(p, lin0 + seq * lstep); };
 
     // ---- global -> LDS: wavefront w copies rows [32 w, 32 w + 32) of both operands and the scales of those activation rows ----
     const int lrow = lane >> 3, lslot = lane & 7;
     uint32_t xoff[4], woff[4], saoff = 0;              // per-lane byte offsets
     const uint8_t* sbsrc = nullptr;                    // the tile's rows of weight-block scales
+    const uint8_t* wbase = p.B;                        // the weights of the tile the copy stream is in
+    // The rows a tile gathers are asked for ahead of the stream's turn to it, in the drain of a tile before.
+    Spot ahead;
+    int ahead_seq = -1, ahead_row[4], ahead_srow = 0;
+    auto look_ahead = [&](int seq) {
+        ahead = spot(seq);
+        ahead_seq = seq;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = min(ahead.m0 + wave * 32 + j * 8 + lrow, ahead.m_end - 1);
+            ahead_row[j] = GROUPED && p.a_row_index ? p.a_row_index[r] : r;
+        }
+        const int r = min(ahead.m0 + wave * 32 + (lane & 31), ahead.m_end - 1);
+        ahead_srow = GROUPED && p.a_row_index ? p.a_row_index[r] : r;
+    };
     auto aim = [&](int seq) {
-        int m0, n0;
-        tile_at(seq, m0, n0);
+        if (!GROUPED || ahead_seq != seq) look_ahead(seq);
+        const int n0 = ahead.n0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int row = wave * 32 + j * 8 + lrow;
             const uint32_t chunk = (lslot ^ swz_rows16(row)) * 16;
-            xoff[j] = static_cast<uint32_t>(min(m0 + row, p.M - 1)) * static_cast<uint32_t>(p.lda) + chunk;
-            woff[j] = static_cast<uint32_t>(n0 + row) * static_cast<uint32_t>(p.ldb) + chunk;        // N % 256 == 0
+            xoff[j] = static_cast<uint32_t>(ahead_row[j]) * static_cast<uint32_t>(p.lda) + chunk;
+            const int n = GROUPED ? min(n0 + row, p.N - 1) : n0 + row;          // dense: N % BN == 0
+            woff[j] = static_cast<uint32_t>(n) * static_cast<uint32_t>(p.ldb) + chunk;
         }
-        saoff = static_cast<uint32_t>(min(m0 + wave * 32 + (lane & 31), p.M - 1)) * static_cast<uint32_t>(ktiles) * 4u;
-        sbsrc = reinterpret_cast<const uint8_t*>(p.sb + static_cast<size_t>((n0 >> 7) + (wave & 1)) * ktiles);
+        saoff = static_cast<uint32_t>(ahead_srow) * static_cast<uint32_t>(ktiles) * 4u;
+        int block = (n0 >> 7) + (wave & 1);
+        if constexpr (GROUPED) {
+            wbase = p.B + ahead.expert * p.b_expert_stride;
+            block = min(block, (p.N - 1) >> 7);
+        }
+        sbsrc = reinterpret_cast<const uint8_t*>(p.sb + static_cast<size_t>(ahead.expert) * p.sb_expert_stride + static_cast<size_t>(block) * ktiles);
     };
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
     auto dma16 = [&](uint32_t dst, uint32_t voff, const uint8_t* base) {
@@ -96,7 +193,7 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
     auto copy_one = [&](int stage, int kt, auto jc) {
         constexpr int J = decltype(jc)::value;
         if constexpr (J < 4)      dma16(lds0 + stage + (wave * 32 + J * 8) * BK, xoff[J], p.A + kt * BK);
-        else if constexpr (J < 8) dma16(lds0 + stage + BM * BK + (wave * 32 + (J - 4) * 8) * BK, woff[J - 4], p.B + kt * BK);
+        else if constexpr (J < 8) dma16(lds0 + stage + BM * BK + (wave * 32 + (J - 4) * 8) * BK, woff[J - 4], wbase + kt * BK);
         else dma4_lo32(lds0 + kWideSa + (stage ? BM * 4 : 0) + wave * 128, saoff, reinterpret_cast<const uint8_t*>(p.sa + kt));
     };
     // the weight-block scales of the tile the stream has just turned to, by wavefronts 0 and 1 (one per column block), into the half of
@@ -247,13 +344,13 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
         static_for<29, 32>([&](auto nc) { fold(nc); });
         // The sums leave as bf16.  A lane holds four consecutive columns of one row per block; 16 rows x 64 columns at a time are
         // turned round in LDS (128-byte rows, 16-byte pieces xor-swizzled by row) and stored as whole lines, eight rows per instruction.
-        int m0, n0;
-        tile_at(seq, m0, n0);
+        const Spot here = spot(seq);
+        if (GROUPED && dseq + 1 < my_tiles && ahead_seq <= dseq) look_ahead(dseq + 1);
         int lane_d = lane;
         asm volatile("" : "+v"(lane_d));        // the drain's per-lane constants are worked out here, not kept through the K loop
         const int row = lane_d & 15, cq = lane_d >> 4, rr = lane_d >> 3, rc = lane_d & 7;
         typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        uint16_t* cp = p.C + static_cast<size_t>(m0 + wm * 64) * p.ldc + n0 + wn * 128;
+        uint16_t* cp = p.C + static_cast<size_t>(here.m0 + wm * 64) * p.ldc + here.n0 + wn * 128;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -270,7 +367,7 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
                 for (int t = 0; t < 2; ++t) {
                     const int r = rr + 8 * t;
                     const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + ((rc ^ ((r >> 1) & 7)) << 4));
-                    if (m0 + wm * 64 + j * 16 + r < p.M) {
+                    if (here.m0 + wm * 64 + j * 16 + r < here.m_end && (!GROUPED || here.n0 + wn * 128 + h * 64 + rc * 8 < p.N)) {
                         const u32x4 vv = {v.x, v.y, v.z, v.w};
                         __builtin_nontemporal_store(vv, reinterpret_cast<u32x4*>(cp + static_cast<size_t>(j * 16 + r) * p.ldc + h * 64 + rc * 8));
                     }
@@ -298,6 +395,7 @@ constexpr int kSlimLds = kSlimOut + 8 * 2048;           // 151,552 bytes
 // five copy instructions per wavefront and K-tile (2 activations, 2 weights, 1 scales)
 constexpr int kSlimWaitVm10 = 0x0f7a, kSlimWaitVm15 = 0x0f7f;
 
+template <bool GROUPED>
 __global__ __launch_bounds__(kWideThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_gemm_nt_block_slim(const GemmArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -305,7 +403,7 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);      // 0..7
     const int wm = wave & 3, wn = wave >> 2;              // 32 rows x 64 columns
     const int ktiles = p.K / BK;          // >= 4, checked by the launcher
-    const int total_tiles = p.tiles_m * p.tiles_n;
+    const int total_tiles = (GROUPED ? __builtin_amdgcn_readfirstlane(p.tile_map[0]) : p.tiles_m) * p.tiles_n;
     int my_tiles, lin0, lstep;
     if (gridDim.x % kXcds == 0) {
         const int per = (total_tiles + kXcds - 1) / kXcds;
@@ -320,29 +418,45 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
         lin0 = blockIdx.x;
     }
     if (my_tiles <= 0) return;
-    auto tile_at = [&](int seq, int& m0, int& n0) {
-        int tm, tn;
-        tile_coords(lin0 + seq * lstep, p.tiles_m, p.tiles_n, tm, tn);
-        m0 = tm * kSlimEdge;
-        n0 = tn * kSlimEdge;
-    };
+    auto spot = [&](int seq) { return locate<GROUPED, kSlimEdge, kSlimEdge>(p, lin0 + seq * lstep); };
 
     // ---- global -> LDS: wavefront w copies rows [16 w, 16 w + 16) of both operands and the scales of those activation rows ----
     const int lrow = lane >> 3, lslot = lane & 7;
     uint32_t xoff[2], woff[2], saoff = 0;
     const uint8_t* sbsrc = nullptr;
+    const uint8_t* wbase = p.B;                        // the weights of the tile the copy stream is in
+    // The rows a tile gathers are asked for ahead of the stream's turn to it, in the drain of a tile before.
+    Spot ahead;
+    int ahead_seq = -1, ahead_row[2], ahead_srow = 0;
+    auto look_ahead = [&](int seq) {
+        ahead = spot(seq);
+        ahead_seq = seq;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = min(ahead.m0 + wave * 16 + j * 8 + lrow, ahead.m_end - 1);
+            ahead_row[j] = GROUPED && p.a_row_index ? p.a_row_index[r] : r;
+        }
+        const int r = min(ahead.m0 + wave * 16 + (lane & 15), ahead.m_end - 1);
+        ahead_srow = GROUPED && p.a_row_index ? p.a_row_index[r] : r;
+    };
     auto aim = [&](int seq) {
-        int m0, n0;
-        tile_at(seq, m0, n0);
+        if (!GROUPED || ahead_seq != seq) look_ahead(seq);
+        const int n0 = ahead.n0;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int row = wave * 16 + j * 8 + lrow;
             const uint32_t chunk = (lslot ^ swz_rows16(row)) * 16;
-            xoff[j] = static_cast<uint32_t>(min(m0 + row, p.M - 1)) * static_cast<uint32_t>(p.lda) + chunk;
-            woff[j] = static_cast<uint32_t>(n0 + row) * static_cast<uint32_t>(p.ldb) + chunk;        // N % 128 == 0
+            xoff[j] = static_cast<uint32_t>(ahead_row[j]) * static_cast<uint32_t>(p.lda) + chunk;
+            const int n = GROUPED ? min(n0 + row, p.N - 1) : n0 + row;          // dense: N % kSlimEdge == 0
+            woff[j] = static_cast<uint32_t>(n) * static_cast<uint32_t>(p.ldb) + chunk;
         }
-        saoff = static_cast<uint32_t>(min(m0 + wave * 16 + (lane & 15), p.M - 1)) * static_cast<uint32_t>(ktiles) * 4u;
-        sbsrc = reinterpret_cast<const uint8_t*>(p.sb + static_cast<size_t>(n0 >> 7) * ktiles);
+        saoff = static_cast<uint32_t>(ahead_srow) * static_cast<uint32_t>(ktiles) * 4u;
+        int block = n0 >> 7;
+        if constexpr (GROUPED) {
+            wbase = p.B + ahead.expert * p.b_expert_stride;
+            block = min(block, (p.N - 1) >> 7);
+        }
+        sbsrc = reinterpret_cast<const uint8_t*>(p.sb + static_cast<size_t>(ahead.expert) * p.sb_expert_stride + static_cast<size_t>(block) * ktiles);
     };
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
     auto dma16 = [&](uint32_t dst, uint32_t voff, const uint8_t* base) {
@@ -361,7 +475,7 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
     auto copy_one = [&](int stage, int kt, auto jc) {
         constexpr int J = decltype(jc)::value;
         if constexpr (J < 2)      dma16(lds0 + stage + (wave * 16 + J * 8) * BK, xoff[J], p.A + kt * BK);
-        else if constexpr (J < 4) dma16(lds0 + stage + kSlimEdge * BK + (wave * 16 + (J - 2) * 8) * BK, woff[J - 2], p.B + kt * BK);
+        else if constexpr (J < 4) dma16(lds0 + stage + kSlimEdge * BK + (wave * 16 + (J - 2) * 8) * BK, woff[J - 2], wbase + kt * BK);
         else dma4_lo16(lds0 + kSlimSa + (stage >> 6) + wave * 64, saoff, reinterpret_cast<const uint8_t*>(p.sa + kt));
     };
     auto copy_sb = [&](int parity) {
@@ -484,13 +598,13 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
         }
         static_for<5, 8>([&](auto nc) { fold(nc); });
         // out as in the kernel above
-        int m0, n0;
-        tile_at(seq, m0, n0);
+        const Spot here = spot(seq);
+        if (GROUPED && dseq + 1 < my_tiles && ahead_seq <= dseq) look_ahead(dseq + 1);
         int lane_d = lane;
         asm volatile("" : "+v"(lane_d));
         const int row = lane_d & 15, cq = lane_d >> 4, rr = lane_d >> 3, rc = lane_d & 7;
         typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-        uint16_t* cp = p.C + static_cast<size_t>(m0 + wm * 32) * p.ldc + n0 + wn * 64;
+        uint16_t* cp = p.C + static_cast<size_t>(here.m0 + wm * 32) * p.ldc + here.n0 + wn * 64;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -505,7 +619,7 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
             for (int t = 0; t < 2; ++t) {
                 const int r = rr + 8 * t;
                 const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + ((rc ^ ((r >> 1) & 7)) << 4));
-                if (m0 + wm * 32 + j * 16 + r < p.M) {
+                if (here.m0 + wm * 32 + j * 16 + r < here.m_end && (!GROUPED || here.n0 + wn * 64 + rc * 8 < p.N)) {
                     const u32x4 vv = {v.x, v.y, v.z, v.w};
                     __builtin_nontemporal_store(vv, reinterpret_cast<u32x4*>(cp + static_cast<size_t>(j * 16 + r) * p.ldc + rc * 8));
                 }
@@ -542,12 +656,12 @@ int gemm_nt_block_wide(GemmArgs p, hipStream_t st) {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_wide), hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds);
+        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_wide<false>), hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds);
     });
     if (err != hipSuccess) return static_cast<int>(err);
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = p.N / BN;
-    k_gemm_nt_block_wide<<<persistent_grid(p.tiles_m * p.tiles_n, num_cus()), kWideThreads, kWideLds, st>>>(p);
+    k_gemm_nt_block_wide<false><<<persistent_grid(p.tiles_m * p.tiles_n, num_cus()), kWideThreads, kWideLds, st>>>(p);
     return launch_status();
 }
 
@@ -573,17 +687,44 @@ int gemm_nt_block_slim(GemmArgs p, hipStream_t st) {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds);
+        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim<false>), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds);
     });
     if (err != hipSuccess) return static_cast<int>(err);
     p.tiles_m = (p.M + kSlimEdge - 1) / kSlimEdge;
     p.tiles_n = p.N / kSlimEdge;
-    k_gemm_nt_block_slim<<<persistent_grid(p.tiles_m * p.tiles_n, num_cus()), kWideThreads, kSlimLds, st>>>(p);
+    k_gemm_nt_block_slim<false><<<persistent_grid(p.tiles_m * p.tiles_n, num_cus()), kWideThreads, kSlimLds, st>>>(p);
     return launch_status();
 }
 
-// The small-tile kernel of gemm_direct.hip: 64 rows of an expert at a time; 32 where K leaves no room for the scales of 64.
-int grouped_gemm_nt_block(const GemmArgs& p, int total_rows, int num_experts, hipStream_t st) {
+namespace {
+template <int TM, int TN, class Kernel>
+int launch_grouped(Kernel kernel, int lds, GemmArgs p, const int* counts, const int* offsets, int total_rows, int num_experts, hipStream_t st) {
+    const int max_tiles = total_rows / TM + num_experts;          // every expert has less than a tile more than its rows fill
+    const int busy = total_rows / TM + (num_experts < total_rows ? num_experts : total_rows);
+    int* table = const_cast<int*>(p.tile_map);
+    p.map_entries = num_experts;
+    p.tiles_n = (p.N + TN - 1) / TN;
+    k_build_block_table<<<1, kTableThreads, 0, st>>>(counts, offsets, num_experts, total_rows, TM, max_tiles, table);
+    kernel<<<persistent_grid(busy * p.tiles_n, num_cus()), kWideThreads, lds, st>>>(p);
+    return launch_status();
+}
+}  // namespace
+
+int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offsets, int total_rows, int num_experts, hipStream_t st) {
+    static std::once_flag once;
+    static hipError_t err = hipSuccess;
+    std::call_once(once, [] {
+        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_wide<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds);
+        if (err == hipSuccess)
+            err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds);
+    });
+    if (err != hipSuccess) return static_cast<int>(err);
+    const int ktiles = p.K / BK;
+    /*SELECT*/
+    if (total_rows > 256 * num_experts && ktiles >= 3) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, counts, offsets, total_rows, num_experts, st);
+    if (total_rows > 64 * num_experts && ktiles >= kSlimStages)
+        return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, counts, offsets, total_rows, num_experts, st);
+    build_tile_map(counts, offsets, num_experts, p.map_entries, total_rows, const_cast<int*>(p.tile_map), st);
     const int rc = grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, 3, st);
     return rc != CF_ERR_UNSUPPORTED ? rc : grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, 7, st);
 }

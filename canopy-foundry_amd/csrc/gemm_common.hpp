@@ -121,8 +121,8 @@ int gemm_nt_block_wide(GemmArgs p, hipStream_t st);
 bool block_slim_ok(const GemmArgs& p);
 float block_slim_estimate_us(const GemmArgs& p);
 int gemm_nt_block_slim(GemmArgs p, hipStream_t st);
-// the grouped form over a row-tile table, arguments checked
-int grouped_gemm_nt_block(const GemmArgs& p, int total_rows, int num_experts, hipStream_t st);
+// the grouped form; p.tile_map is the workspace, of cf_fp8_grouped_gemm_workspace_bytes, that it builds its own table in
+int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offsets, int total_rows, int num_experts, hipStream_t st);
 // gemm_accum.hip
 bool accum_wide_ok(const GemmArgs& p, int fmt, int epi, int scale_mode);
 float accum_wide_estimate_us(const GemmArgs& p);
