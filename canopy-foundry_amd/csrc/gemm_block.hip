@@ -28,7 +28,7 @@ constexpr int kWideSb = kWideSa + 2 * BM * 4;           // weight-block scales: 
 constexpr int kWideMaxKb = 256;
 constexpr int kWideOut = kWideSb + 2 * 2 * kWideMaxKb * 4;      // 2 KiB per wavefront in which the output is turned round
 constexpr int kWideLds = kWideOut + 8 * 2048;           // 153,600 bytes
-constexpr int kWideWaitVm0 = 0x0f70;                    // s_waitcnt vmcnt(0) only
+constexpr int kWideWaitVm0 = 0x0f70, kWideWaitVm16 = 0x4f70;      // s_waitcnt vmcnt(0), vmcnt(16) only
 
 // ---- the grouped form's table of row tiles ----
 // Word 0: the number of tiles of `rows` rows; then three words per expert, its first row, the row behind its last and its first tile; then
@@ -119,7 +119,9 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);      // 0..7
-    const int wm = wave & 3, wn = wave >> 2;              // 64 rows x 128 columns: the four wavefronts of a wn share a column block
+    // 64 rows x 128 columns: the four wavefronts of a wn share a column block.  Grouped: of the two wavefronts of a SIMD (w and w + 4) one is in the
+    // upper half of the rows and one in the lower, one in the left half of the columns and one in the right (see `busy`).
+    const int wn = wave >> 2, wm = GROUPED ? (wave + 2 * wn) & 3 : wave & 3;
     const int ktiles = p.K / BK;          // >= 3, checked by the launcher; also the number of scale groups along K
     const int total_tiles = (GROUPED ? __builtin_amdgcn_readfirstlane(p.tile_map[0]) : p.tiles_m) * p.tiles_n;
     int my_tiles, lin0, lstep;
@@ -140,12 +142,16 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
 
     // ---- global -> LDS: wavefront w copies rows [32 w, 32 w + 32) of both operands and the scales of those activation rows ----
     const int lrow = lane >> 3, lslot = lane & 7;
-    uint32_t xoff[4], woff[4], saoff = 0;              // per-lane byte offsets
+    uint32_t xoff[4], woff[GROUPED ? 2 : 4], saoff = 0;              // per-lane byte offsets
     const uint8_t* sbsrc = nullptr;                    // the tile's rows of weight-block scales
     const uint8_t* wbase = p.B;                        // the weights of the tile the copy stream is in
     // The rows a tile gathers are asked for ahead of the stream's turn to it, in the drain of a tile before.
     Spot ahead;
     int ahead_seq = -1, ahead_row[4], ahead_srow = 0;
+    // An expert's last row tile, and the last column tile, may be nearly empty: a wavefront without an output in the tile works on none of its
+    // K-tiles (`busy`, for the tile the stream has turned to), rows that are not there are not copied.
+    bool busy = true, copies_x = true;
+    int weight_rows = 0;                               // of this wavefront's 32: a multiple of 8, as N is
     auto look_ahead = [&](int seq) {
         ahead = spot(seq);
         ahead_seq = seq;
@@ -165,13 +171,16 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
             const int row = wave * 32 + j * 8 + lrow;
             const uint32_t chunk = (lslot ^ swz_rows16(row)) * 16;
             xoff[j] = static_cast<uint32_t>(ahead_row[j]) * static_cast<uint32_t>(p.lda) + chunk;
-            const int n = GROUPED ? min(n0 + row, p.N - 1) : n0 + row;          // dense: N % BN == 0
-            woff[j] = static_cast<uint32_t>(n) * static_cast<uint32_t>(p.ldb) + chunk;
+            // grouped: copies j and j + 2 share an offset, 16 rows apart; dense: N % 256 == 0
+            if (!GROUPED || j < 2) woff[j] = static_cast<uint32_t>(n0 + row) * static_cast<uint32_t>(p.ldb) + chunk;
         }
         saoff = static_cast<uint32_t>(ahead_srow) * static_cast<uint32_t>(ktiles) * 4u;
         int block = (n0 >> 7) + (wave & 1);
         if constexpr (GROUPED) {
             wbase = p.B + ahead.expert * p.b_expert_stride;
+            busy = ahead.m0 + wm * 64 < ahead.m_end && n0 + wn * 128 < p.N;
+            copies_x = ahead.m0 + wave * 32 < ahead.m_end;
+            weight_rows = p.N - n0 - wave * 32;
             block = min(block, (p.N - 1) >> 7);
         }
         sbsrc = reinterpret_cast<const uint8_t*>(p.sb + static_cast<size_t>(ahead.expert) * p.sb_expert_stride + static_cast<size_t>(block) * ktiles);
@@ -192,7 +201,9 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
     // copy J (0..8) of the K-tile at position kt of its tile into the stage at `stage` (0 or kWideStage)
     auto copy_one = [&](int stage, int kt, auto jc) {
         constexpr int J = decltype(jc)::value;
+        if (GROUPED && !(J >= 4 && J < 8 ? (J - 4) * 8 < weight_rows : copies_x)) return;
         if constexpr (J < 4)      dma16(lds0 + stage + (wave * 32 + J * 8) * BK, xoff[J], p.A + kt * BK);
+        else if constexpr (J < 8 && GROUPED) dma16(lds0 + stage + BM * BK + (wave * 32 + (J - 4) * 8) * BK, woff[J & 1], wbase + kt * BK + ((J - 4) >> 1) * 16 * static_cast<size_t>(p.ldb));
         else if constexpr (J < 8) dma16(lds0 + stage + BM * BK + (wave * 32 + (J - 4) * 8) * BK, woff[J - 4], wbase + kt * BK);
         else dma4_lo32(lds0 + kWideSa + (stage ? BM * 4 : 0) + wave * 128, saoff, reinterpret_cast<const uint8_t*>(p.sa + kt));
     };
@@ -260,6 +271,8 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
             fn[j] = *reinterpret_cast<const float*>(smem + kWideSa + (stage ? BM * 4 : 0) + (wm * 64 + j * 16 + r16) * 4) * sbv;
     };
 
+    // Grouped: the tile before was a whole one, whose sixteen stores, the last memory operations before, need not be waited for with the copies.
+    bool whole_tile = false;
     int s0 = 0;                   // stage of the current K-tile; the other one holds, or receives, the next
     // One K-tile.  FIRST: a tile's first (nothing is left to fold).  (nkt, npar): position and tile parity of the K-tile after it,
     // dkt: position of the one after that, whose copies start behind the barrier.
@@ -284,7 +297,8 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
         mfma(std::integral_constant<int, 24>{});
         fold(std::integral_constant<int, 21>{});
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(kWideWaitVm0);
+        if (GROUPED && FIRST && whole_tile) __builtin_amdgcn_s_waitcnt(kWideWaitVm16);
+        else                                __builtin_amdgcn_s_waitcnt(kWideWaitVm0);
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
         static_for<25, 32>([&](auto nc) {
@@ -306,6 +320,22 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
         copy_one(s0, dkt, std::integral_constant<int, 7>{});
         copy_one(s0, dkt, std::integral_constant<int, 8>{});
         __builtin_amdgcn_sched_barrier(0);
+        s0 = s1;
+    };
+
+    // A K-tile of a tile that this wavefront has no output in: the barrier and the copies.  `turn`: the next K-tile is another tile's first, whose
+    // operands are read.
+    auto ktile_idle = [&](bool turn, int npar, int dkt) {
+        const int s1 = s0 ^ kWideStage;
+        __builtin_amdgcn_s_waitcnt(kWideWaitVm0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<0, 9>([&](auto jc) { copy_one(s0, dkt, jc); });
+        if (turn) {
+            static_for<0, 4>([&](auto rc) { read_w(s1, std::integral_constant<int, 0>{}, rc); });
+            static_for<0, 8>([&](auto rc) { read_x(s1, rc); });
+            read_factors(s1, npar, 0);
+        }
         s0 = s1;
     };
 
@@ -334,6 +364,15 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
     uint8_t* stg = smem + kWideOut + wave * 2048;
     for (int seq = 0; seq < my_tiles; ++seq) {
         const int parity = seq & 1;
+        if (GROUPED && !busy) {
+            whole_tile = false;
+            for (int kt = 0; kt < ktiles; ++kt) {
+                ktile_idle(kt + 1 == ktiles, parity ^ 1, dkt);
+                advance_copy();
+            }
+            if (dseq + 1 < my_tiles && ahead_seq <= dseq) look_ahead(dseq + 1);
+            continue;
+        }
         ktile(std::integral_constant<int, 1>{}, 1, parity, dkt);
         advance_copy();
         for (int kt = 1; kt < ktiles; ++kt) {
@@ -345,6 +384,7 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
         // The sums leave as bf16.  A lane holds four consecutive columns of one row per block; 16 rows x 64 columns at a time are
         // turned round in LDS (128-byte rows, 16-byte pieces xor-swizzled by row) and stored as whole lines, eight rows per instruction.
         const Spot here = spot(seq);
+        whole_tile = GROUPED && here.m0 + wm * 64 + 64 <= here.m_end && here.n0 + wn * 128 + 128 <= p.N;
         if (GROUPED && dseq + 1 < my_tiles && ahead_seq <= dseq) look_ahead(dseq + 1);
         int lane_d = lane;
         asm volatile("" : "+v"(lane_d));        // the drain's per-lane constants are worked out here, not kept through the K loop
@@ -719,14 +759,53 @@ int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offse
             err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds);
     });
     if (err != hipSuccess) return static_cast<int>(err);
+    const float rows = static_cast<float>(total_rows), experts = static_cast<float>(num_experts < total_rows ? num_experts : total_rows);
     const int ktiles = p.K / BK;
-    /*SELECT*/
-    if (total_rows > 256 * num_experts && ktiles >= 3) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, counts, offsets, total_rows, num_experts, st);
-    if (total_rows > 64 * num_experts && ktiles >= kSlimStages)
-        return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, counts, offsets, total_rows, num_experts, st);
-    build_tile_map(counts, offsets, num_experts, p.map_entries, total_rows, const_cast<int*>(p.tile_map), st);
-    const int rc = grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, 3, st);
-    return rc != CF_ERR_UNSUPPORTED ? rc : grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, 7, st);
+    // Microseconds, table and launches aside, for rows that lie evenly: rounds of workgroups or tiles over the CUs, fitted to 3200 sizes of more than 24 rows an
+    // expert (of which 10 % then ran over 1.1 times the best, 4 % over 1.25).  An expert has 0.6 of a small tile (0.5 of
+    // a large one) more than its rows fill, and one at least.  Measured us, chosen first (rows, experts, N, K: 32 x 64, 64 x 64, 128 x 128, 256 x 256 tiles):
+    //     96    64  1408 x 2048     31.7    47.7    48.2    67.7         1000  16  1536 x 4096    48.4    40.5    32.3    56.3
+    //     1280  64  1408 x 2048     43.1    64.5    57.3    72.2         4000  16  2048 x 7168       .    234     141     120
+    //     2560  64  1408 x 2048     64.4    71.2    55.6    75.1         500    8  1024 x 2048    18.3    14.1    21.4    34.3
+    //     8000  64  1408 x 2048     145     143     76.5    83.0         2000   8  1024 x 2048    34.1    28.3    22.6    35.4
+    //     98304 64  1408 x 2048       .    1157     462     365          32768  8  1024 x 2048       .    273     118     96.8
+    const auto busy_entries = [&](int edge) { return total_rows / edge + (num_experts < total_rows ? num_experts : total_rows); };      // row tiles at most
+    const auto tiles = [&](float edge, float more) { return rows / edge + more * experts > experts ? rows / edge + more * experts : experts; };
+    const auto rounds = [&](float n) { const float r = n / static_cast<float>(num_cus()); return static_cast<float>(static_cast<int>(r) + 1); };
+    const float k = static_cast<float>(p.K);
+    const int columns64 = (p.N + 63) / 64;
+    // 64 rows at a time, side by side; the LDS of the small-tile kernel holds the scales of that many rows up to K = 16000
+    float best = 1e30f;
+    int shape = 7;                  // of the small-tile kernel, or the tile edge.  (Two or three K-tiles for four wavefronts: 16809 rows, 128 experts of 1536 x 256 67 us, in 64 x 64 157)
+    const float passes = tiles(64.0f, 0.6f) * static_cast<float>(columns64) / static_cast<float>(num_cus());
+    if (ktiles >= 4 && ktiles <= 120) {
+        best = (passes > 0.8f ? passes + 0.5f : 1.0f) * (5.6f + k * 128.0f / 51e3f);
+        shape = 3;
+    }
+    if (ktiles >= kSlimStages) {
+        const float r = rounds(tiles(kSlimEdge, 0.6f) * static_cast<float>((p.N + kSlimEdge - 1) / kSlimEdge));
+        const float t = (r > 1.0f ? r : 1.25f) * (static_cast<float>(ktiles) * 0.50f + 6.0f);
+        if (t < best) { best = t; shape = kSlimEdge; }
+    }
+    if (ktiles >= 3) {
+        const float t = rounds(tiles(BM, 0.5f) * static_cast<float>((p.N + BN - 1) / BN)) * (static_cast<float>(ktiles) * 1.3f + 11.7f);
+        if (t < best) { best = t; shape = BM; }
+    }
+    // Up to 24 rows an expert most have one pass of 32 x 64: their weights are read once, which is all of the time (4.6 TB/s).  Where that leaves CUs without
+    // one, fewer columns and up to 32 rows (8 experts of 1024 x 2048, 200 rows: 11.8 us and 13.8), and few rows besides (12 rows, 64 experts of
+    // 256 x 6144: 16 x 16 12.9, 32 x 32 13, 32 x 64 16.3; 16 rows, 2 of 512 x 4096: 9.2, 10.7, 12).
+    const bool fills = experts * static_cast<float>(columns64) >= static_cast<float>(num_cus());
+    if (rows <= (fills ? 24.0f : 32.0f) * static_cast<float>(num_experts)) shape = fills ? 7 : rows <= 10.0f * experts ? 0 : 1;
+    if (shape == BM) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, counts, offsets, total_rows, num_experts, st);
+    if (shape == kSlimEdge) return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, counts, offsets, total_rows, num_experts, st);
+    GemmArgs q = p;
+    q.tiles_m = q.map_entries = busy_entries(BM);
+    build_tile_map(counts, offsets, num_experts, q.map_entries, total_rows, const_cast<int*>(q.tile_map), st);
+    if (shape == 3) {
+        const long long each = (static_cast<long long>(total_rows) + 64LL * num_experts - 1) / (64LL * num_experts);
+        q.tiles_m *= each < 3 ? static_cast<int>(each) + 1 : 4;           // workgroups for the passes of an entry of 256 rows
+    }
+    return grouped_gemm_nt_direct(q, 0, EPI_NONE, SCALE_BLOCK, shape, st);
 }
 
 }  // namespace cf
