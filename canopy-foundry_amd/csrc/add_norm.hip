@@ -29,6 +29,7 @@ struct AddNormArgs {
     const float* qscale;      // Q_RECORD
     float* amax;
     int rows, H;
+    unsigned row0;            // the launch's first row
     float eps;
     int e5m2;
 };
@@ -211,11 +212,11 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // Raising one maximum from every row.  Atomics on one address take turns, and the rows that run first all find the value they start from: with an
 // atomic from each row that finds its own the larger, 1000 rows of 4096 took 15.8 us, 7.8 with a scale a row; 8192 (fp32) 94 and 78, 32768 x 1024 86 and 51.  So one
 // row in 128 raises it as soon as it knows its own; the others look again behind their stores and a microsecond and a half: 10.8, 84 and 61 us.
-__device__ __forceinline__ void raise_first(float* amax, uint32_t m, int row, float& before) {
+__device__ __forceinline__ void raise_first(float* amax, uint32_t m, unsigned row, float& before) {
     before = atomic_load_agent(amax);
     if (row % 128 == 0 && __uint_as_float(m) > before) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
 }
-__device__ __forceinline__ void raise_last(float* amax, uint32_t m, int row, float before) {
+__device__ __forceinline__ void raise_last(float* amax, uint32_t m, unsigned row, float before) {
     if (row % 128 == 0 || __uint_as_float(m) <= before) return;
     __builtin_amdgcn_s_sleep(48);           // 3072 cycles
     if (__uint_as_float(m) > atomic_load_agent(amax)) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
@@ -239,11 +240,12 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNor
     __shared__ float sh_sum[16];
     __shared__ uint32_t sh_max[2][16];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
-    int row = blockIdx.x, t = threadIdx.x;
+    unsigned row = p.row0 + blockIdx.x;
+    int t = threadIdx.x;
     if constexpr (ONE_WAVE) {
-        row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+        row = __builtin_amdgcn_readfirstlane(p.row0 + blockIdx.x * 4 + (threadIdx.x >> 6));
         t &= 63;
-        if (row >= p.rows) return;
+        if (row >= static_cast<unsigned>(p.rows)) return;
     }
     const int chunks = TAIL ? (H + 7) / 8 : H / 8;
     const size_t base = static_cast<size_t>(row) * H;
@@ -385,8 +387,8 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm_grad(const A
     __shared__ float sh_dw[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
-    const int first = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
-    const int step = ONE_WAVE ? gridDim.x * 4 : gridDim.x;
+    const unsigned first = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
+    const unsigned step = ONE_WAVE ? gridDim.x * 4 : gridDim.x, rows = p.rows;
     const int chunks = TAIL ? (H + 7) / 8 : H / 8;
     auto left = [&](int j) { return TAIL ? H - (t + j * T) * 8 : 8; };
     auto has = [&](int j) { return t + j * T < chunks; };
@@ -396,9 +398,9 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm_grad(const A
         Raw8<F32> h[V], dh[V];
         float rms;
     };
-    auto load = [&](Row& r, int row) {
+    auto load = [&](Row& r, unsigned row) {
         const size_t base = static_cast<size_t>(row) * H;
-        const bool follows = static_cast<size_t>(p.rows - 1 - row) * H >= 7;
+        const bool follows = static_cast<size_t>(rows - 1 - row) * H >= 7;
         r.rms = p.rms[row];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -426,12 +428,12 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm_grad(const A
     float amax = 0.0f;
     constexpr bool AHEAD = V == 1;          // 1024 threads have 128 registers each, too few for two rows of two chunks
     Row r, next;
-    if (AHEAD && first < p.rows) load(next, first);
+    if (AHEAD && first < rows) load(next, first);
     int turn = 0;
-    for (int row = first; row < p.rows; row += step, turn ^= 1) {
+    for (unsigned row = first; row < rows; row += step, turn ^= 1) {
         if constexpr (AHEAD) {
             r = next;
-            if (row + step < p.rows) load(next, row + step);
+            if (row + step < rows) load(next, row + step);
         } else {
             load(r, row);
         }
@@ -544,11 +546,16 @@ bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintpt
 constexpr int row_threads(int H, int V) { return ((H + 7) / 8 + kWave * V - 1) / (kWave * V) * kWave; }
 constexpr int kOneWaveH = 8 * kWave, kOneChunkH = 8 * 1024;
 
+constexpr unsigned kLaunchRows = 1u << 21;             // a launch has fewer than 2^32 threads
+
 template <bool F32, int QMODE, bool TAIL>
-int launch_add_norm(const AddNormArgs& p, hipStream_t st) {
-    if (p.H <= kOneWaveH) k_add_norm<F32, QMODE, TAIL, true, 1><<<ceil_div(p.rows, 4), 4 * kWave, 0, st>>>(p);
-    else if (p.H <= kOneChunkH) k_add_norm<F32, QMODE, TAIL, false, 1><<<p.rows, row_threads(p.H, 1), 0, st>>>(p);
-    else k_add_norm<F32, QMODE, TAIL, false, 2><<<p.rows, row_threads(p.H, 2), 0, st>>>(p);
+int launch_add_norm(AddNormArgs p, hipStream_t st) {
+    for (; p.row0 < static_cast<unsigned>(p.rows); p.row0 += kLaunchRows) {
+        const unsigned left = static_cast<unsigned>(p.rows) - p.row0, n = left < kLaunchRows ? left : kLaunchRows;
+        if (p.H <= kOneWaveH) k_add_norm<F32, QMODE, TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
+        else if (p.H <= kOneChunkH) k_add_norm<F32, QMODE, TAIL, false, 1><<<n, row_threads(p.H, 1), 0, st>>>(p);
+        else k_add_norm<F32, QMODE, TAIL, false, 2><<<n, row_threads(p.H, 2), 0, st>>>(p);
+    }
     return launch_status();
 }
 

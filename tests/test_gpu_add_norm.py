@@ -300,3 +300,20 @@ def test_gradient_against_differences(cf, dev):
         mine = (got["dr"].double() * v).sum() + (got["dw"].double() * u).sum()
         size = (got["dr"].double() * v).abs().sum() + (got["dw"].double() * u).abs().sum()
         assert abs(mine - slope) <= 2e-6 * size
+
+
+def test_more_rows_than_one_launch_holds(cf, dev):
+    """Rows of eight, 2^21 and a few: the last ones are as the first."""
+    rows, H = (1 << 21) + 7, 8
+    case(f"add-norm {rows} rows of {H}")
+    r = torch.randn(rows, H, device=dev).to(torch.bfloat16)
+    x, w = torch.zeros_like(r), torch.ones(H, device=dev).to(torch.bfloat16)
+    total, q = torch.zeros_like(r), torch.zeros(rows, H, dtype=torch.uint8, device=dev)
+    rms, s, d = (torch.zeros(rows, device=dev) for _ in range(3))
+    cf.cf_add_rmsnorm_quantize_rows(r, x, 0, w, rows, H, EPS, 0, total, None, rms, q, s, d, stream())
+    torch.cuda.synchronize()
+    assert torch.equal(total, r)
+    tail = slice(rows - 4000, rows)
+    check_forward({"sum": total[tail].cpu(), "rms": rms[tail].cpu(), "normed": None, "q": q[tail].cpu(), "scale": s[tail].cpu(), "descale": d[tail].cpu()},
+                  r[tail].cpu(), x[tail].cpu(), w.cpu(), "rows", 0)
+    assert bool((s > 0).all())

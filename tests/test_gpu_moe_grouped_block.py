@@ -108,6 +108,23 @@ def test_block_scaled_experts(cf, dev, counts, N, K, gather):
     b.check(b.run(cf))
 
 
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("counts,N,K", [
+    ([40] * 300, 256, 512),                          # more experts than the table's workgroup has threads
+    ([3, 0] * 200, 136, 384),
+    ([1536, 1500, 1600, 30, 2000, 257] * 3, 1416, 640),     # last row and column tiles nearly empty, several tiles a workgroup
+    ([2500] * 8, 1024 + 8, 384),                     # three K-tiles; eight columns in the last tile
+    ([5000, 4000, 6000], 1920, 512),                 # four
+    ([300, 420], 264, 32768),                        # all of the weight-block scales' LDS
+    ([900, 1, 129, 128, 127, 0, 700] * 4, 1408, 896),
+    ([20000], 392, 256),
+], ids=lambda v: str(v) if not isinstance(v, list) else f"{len(v)}x{max(v)}")
+def test_block_scaled_experts_of_many_rows(cf, dev, counts, N, K, gather):
+    case(f"grouped block GEMM counts={counts[:8]} of {len(counts)} N={N} K={K} gather={gather}")
+    b = Experts(dev, counts, N, K, gather, seed=N * 3 + K)
+    b.check(b.run(cf))
+
+
 def test_strides_and_rows_behind_the_last_expert(cf, dev):
     """Row strides larger than the rows, a bound above the sum of the counts: the rows behind are left alone."""
     for counts, total in (([3, 0, 5], 64), ([130, 20, 70], 700), ([400, 0, 300, 90], 2000)):
