@@ -2528,7 +2528,10 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     const int out_bn = epilogue == EPI_SILU_GATE ? BN / 2 : BN;
     p.tiles_m = p.map_entries = max_row_tiles;
     p.tiles_n = (N + out_bn - 1) / out_bn;
-    if (scale_mode == SCALE_BLOCK) return grouped_gemm_nt_block(p, d_counts, d_offsets, total_rows, num_experts, st);
+    if (scale_mode == SCALE_BLOCK) {
+        p.counts = d_counts; p.offsets = d_offsets; p.num_experts = num_experts;
+        return grouped_gemm_nt_block(p, st);
+    }
     // Few rows per expert: the small-tile kernel, which walks an expert's rows 16 mb at a time, where its estimate is lower.
     // It is sized for half as many rows again as the bound's average, so that most experts take one pass over their weights;
     // beyond 40 rows that is more than its largest pass.  The counts are on the device, so the choice is for balanced experts: 64 of

@@ -30,27 +30,19 @@ constexpr int kWideOut = kWideSb + 2 * 2 * kWideMaxKb * 4;      // 2 KiB per wav
 constexpr int kWideLds = kWideOut + 8 * 2048;           // 153,600 bytes
 constexpr int kWideWaitVm0 = 0x0f70, kWideWaitVm16 = 0x4f70;      // s_waitcnt vmcnt(0), vmcnt(16) only
 
-// ---- the grouped form's table of row tiles ----
-// Word 0: the number of tiles of `rows` rows; then three words per expert, its first row, the row behind its last and its first tile; then
-// the expert of each tile.  It fits the bytes of the table of build_tile_map for tiles of 128 or 256 rows.
-constexpr int kExpertWords = 3;
-constexpr int kTableThreads = 256;
-__global__ __launch_bounds__(kTableThreads) void k_build_block_table(const int* __restrict__ counts, const int* __restrict__ offsets, int num_experts,
-                                                                     int total_rows, int tile_rows, int max_tiles, int* __restrict__ table) {
-    __shared__ int sh_first[kTableThreads], sh_tiles[kTableThreads], sh_wave[kTableThreads / kWave], sh_written;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    int* const experts = table + 1;
-    int* const tiles = table + 1 + kExpertWords * num_experts;
-    int carry = 0;
-    if (t == 0) sh_written = 0;
-    for (int e0 = 0; e0 < num_experts; e0 += kTableThreads) {
-        const int e = e0 + t;
-        int first = 0, kept = 0;
-        if (e < num_experts) {
-            first = offsets[e];
-            kept = first >= 0 && first < total_rows ? max(0, min(counts[e], total_rows - first)) : 0;
-        }
-        const int n = (kept + tile_rows - 1) / tile_rows;
+// ---- the grouped form's row tiles ----
+// A workgroup counts the experts' row tiles into LDS before it begins (a kernel of its own for the table took 6 to 10 us and its launch): `first_tile` [experts + 1]
+// is the number of tiles before each expert's.
+constexpr int kMostExperts = 2048;
+constexpr int kTilesLds = (kMostExperts + 1 + 8) * 4;
+template <int TM>
+__device__ __forceinline__ int count_tiles(const GemmArgs& p, int* first_tile) {
+    int* const sh_wave = first_tile + kMostExperts + 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int total = 0;
+    for (int e0 = 0; e0 < p.num_experts; e0 += kWideThreads) {
+        const int e = e0 + tid;
+        const int n = e < p.num_experts ? (expert_rows(p, e).rows + TM - 1) / TM : 0;
         int incl = n;
 #pragma unroll
         for (int off = 1; off < kWave; off <<= 1) {
@@ -59,45 +51,49 @@ __global__ __launch_bounds__(kTableThreads) void k_build_block_table(const int* 
         }
         if (lane == 63) sh_wave[wave] = incl;
         __syncthreads();
-        int before = carry;
-        for (int w = 0; w < wave; ++w) before += sh_wave[w];
-        const int at = before + incl - n;
-        sh_first[t] = at;
-        // always all of them when the experts' ranges do not overlap; otherwise the ones that fit come first and the table ends with them
-        sh_tiles[t] = at + n <= max_tiles ? n : 0;
-        if (sh_tiles[t] > 0) atomicMax(&sh_written, at + n);
-        if (e < num_experts) {
-            experts[kExpertWords * e] = first;
-            experts[kExpertWords * e + 1] = first + kept;
-            experts[kExpertWords * e + 2] = at;
+        int before = total;
+#pragma unroll
+        for (int w = 0; w < kWideThreads / kWave; ++w) {
+            before += w < wave ? sh_wave[w] : 0;
+            total += sh_wave[w];
         }
-        int all = carry;
-        for (int w = 0; w < kTableThreads / kWave; ++w) all += sh_wave[w];
-        __syncthreads();
-        for (int i = wave; i < kTableThreads; i += kTableThreads / kWave)
-            for (int k = lane; k < sh_tiles[i]; k += kWave) tiles[sh_first[i] + k] = e0 + i;
-        carry = all;
+        if (e < p.num_experts) first_tile[e] = before + incl - n;
         __syncthreads();
     }
-    if (t == 0) table[0] = sh_written;
+    if (tid == 0) first_tile[p.num_experts] = total;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(total);
+}
+
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // Where the tile at `lin` of the walk lies.  Dense: the patches of tile_coords.  Grouped: an expert's tiles in groups of four column tiles, its row
 // tiles varying fastest.
 struct Spot { int m0, m_end, n0, expert; };
 template <bool GROUPED, int TM, int TN>
-__device__ __forceinline__ Spot locate(const GemmArgs& p, int lin) {
+__device__ __forceinline__ Spot locate(const GemmArgs& p, const int* first_tile, int lin) {
     Spot s;
     if constexpr (GROUPED) {
         constexpr int GN = 4;
-        const int* const experts = p.tile_map + 1;
-        s.expert = __builtin_amdgcn_readfirstlane(experts[kExpertWords * p.map_entries + lin / p.tiles_n]);
-        const int* const e = experts + kExpertWords * s.expert;
-        const int first = __builtin_amdgcn_readfirstlane(e[0]), last = __builtin_amdgcn_readfirstlane(e[1]);
-        const int local = lin - __builtin_amdgcn_readfirstlane(e[2]) * p.tiles_n, n = (last - first + TM - 1) / TM;
+        const int tile = lin / p.tiles_n;
+        int lo = 0, hi = p.num_experts - 1;                 // the last expert whose first tile is not behind it: the one that has it
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (__builtin_amdgcn_readfirstlane(first_tile[mid]) <= tile) lo = mid;
+            else hi = mid - 1;
+        }
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        const int before = __builtin_amdgcn_readfirstlane(first_tile[lo]), n = __builtin_amdgcn_readfirstlane(first_tile[lo + 1]) - before;
+        const ExpertRows r = expert_rows(p, lo);
+        const int first = __builtin_amdgcn_readfirstlane(r.first), local = lin - before * p.tiles_n;
         const int g = local / (n * GN), within = local - g * (n * GN);
+        s.expert = lo;
         s.m0 = first + within % n * TM;
-        s.m_end = last;
+        s.m_end = first + __builtin_amdgcn_readfirstlane(r.rows);
         s.n0 = (g * GN + within / n) * TN;
     } else {
         int tm, tn;
@@ -123,7 +119,9 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
     // upper half of the rows and one in the lower, one in the left half of the columns and one in the right (see `busy`).
     const int wn = wave >> 2, wm = GROUPED ? (wave + 2 * wn) & 3 : wave & 3;
     const int ktiles = p.K / BK;          // >= 3, checked by the launcher; also the number of scale groups along K
-    const int total_tiles = (GROUPED ? __builtin_amdgcn_readfirstlane(p.tile_map[0]) : p.tiles_m) * p.tiles_n;
+    int* const first_tile = reinterpret_cast<int*>(smem + kWideLds);         // grouped
+    int total_tiles = p.tiles_m * p.tiles_n;
+    if constexpr (GROUPED) total_tiles = count_tiles<BM>(p, first_tile) * p.tiles_n;
     int my_tiles, lin0, lstep;
     if (gridDim.x % kXcds == 0) {
         const int per = (total_tiles + kXcds - 1) / kXcds;
@@ -138,7 +136,7 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
         lin0 = blockIdx.x;
     }
     if (my_tiles <= 0) return;
-    auto spot = [&](int seq) { return locate<GROUPED, BM, BN>(p, lin0 + seq * lstep); };
+    auto spot = [&](int seq) { return locate<GROUPED, BM, BN>(p, first_tile, lin0 + seq * lstep); };
 
     // ---- global -> LDS: wavefront w copies rows [32 w, 32 w + 32) of both operands and the scales of those activation rows ----
     const int lrow = lane >> 3, lslot = lane & 7;
@@ -443,7 +441,9 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);      // 0..7
     const int wm = wave & 3, wn = wave >> 2;              // 32 rows x 64 columns
     const int ktiles = p.K / BK;          // >= 4, checked by the launcher
-    const int total_tiles = (GROUPED ? __builtin_amdgcn_readfirstlane(p.tile_map[0]) : p.tiles_m) * p.tiles_n;
+    int* const first_tile = reinterpret_cast<int*>(smem + kSlimLds);
+    int total_tiles = p.tiles_m * p.tiles_n;
+    if constexpr (GROUPED) total_tiles = count_tiles<kSlimEdge>(p, first_tile) * p.tiles_n;
     int my_tiles, lin0, lstep;
     if (gridDim.x % kXcds == 0) {
         const int per = (total_tiles + kXcds - 1) / kXcds;
@@ -458,7 +458,7 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
         lin0 = blockIdx.x;
     }
     if (my_tiles <= 0) return;
-    auto spot = [&](int seq) { return locate<GROUPED, kSlimEdge, kSlimEdge>(p, lin0 + seq * lstep); };
+    auto spot = [&](int seq) { return locate<GROUPED, kSlimEdge, kSlimEdge>(p, first_tile, lin0 + seq * lstep); };
 
     // ---- global -> LDS: wavefront w copies rows [16 w, 16 w + 16) of both operands and the scales of those activation rows ----
     const int lrow = lane >> 3, lslot = lane & 7;
@@ -522,7 +522,8 @@ void k_gemm_nt_block_slim(const GemmArgs p) {
         if (wave == 0) {
             for (int c = 0; c * 64 < ktiles; ++c) {
                 const uint32_t v = static_cast<uint32_t>(min(c * 64 + lane, ktiles - 1)) * 4u;
-                dma4(lds0 + kSlimSb + parity * (kWideMaxKb * 4) + c * 256, v, sbsrc);
+                // (grouped, the compiler may have parked the address in vector registers)
+                dma4(lds0 + kSlimSb + parity * (kWideMaxKb * 4) + c * 256, v, GROUPED ? uniform(sbsrc) : sbsrc);
             }
         }
     };
@@ -737,26 +738,24 @@ int gemm_nt_block_slim(GemmArgs p, hipStream_t st) {
 }
 
 namespace {
+static_assert(kWideLds + kTilesLds <= 160 * 1024 && kSlimLds + kTilesLds <= 160 * 1024);
 template <int TM, int TN, class Kernel>
-int launch_grouped(Kernel kernel, int lds, GemmArgs p, const int* counts, const int* offsets, int total_rows, int num_experts, hipStream_t st) {
-    const int max_tiles = total_rows / TM + num_experts;          // every expert has less than a tile more than its rows fill
-    const int busy = total_rows / TM + (num_experts < total_rows ? num_experts : total_rows);
-    int* table = const_cast<int*>(p.tile_map);
-    p.map_entries = num_experts;
+int launch_grouped(Kernel kernel, int lds, GemmArgs p, hipStream_t st) {
+    const int busy = p.M / TM + (p.num_experts < p.M ? p.num_experts : p.M);        // row tiles at most
     p.tiles_n = (p.N + TN - 1) / TN;
-    k_build_block_table<<<1, kTableThreads, 0, st>>>(counts, offsets, num_experts, total_rows, TM, max_tiles, table);
-    kernel<<<persistent_grid(busy * p.tiles_n, num_cus()), kWideThreads, lds, st>>>(p);
+    kernel<<<persistent_grid(busy * p.tiles_n, num_cus()), kWideThreads, lds + kTilesLds, st>>>(p);
     return launch_status();
 }
 }  // namespace
 
-int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offsets, int total_rows, int num_experts, hipStream_t st) {
+int grouped_gemm_nt_block(GemmArgs p, hipStream_t st) {
+    const int total_rows = p.M, num_experts = p.num_experts;
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_wide<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds);
+        err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_wide<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kWideLds + kTilesLds);
         if (err == hipSuccess)
-            err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds);
+            err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds + kTilesLds);
     });
     if (err != hipSuccess) return static_cast<int>(err);
     const float rows = static_cast<float>(total_rows), experts = static_cast<float>(num_experts < total_rows ? num_experts : total_rows);
@@ -769,7 +768,6 @@ int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offse
     //     2560  64  1408 x 2048     64.4    71.2    55.6    75.1         500    8  1024 x 2048    18.3    14.1    21.4    34.3
     //     8000  64  1408 x 2048     145     143     76.5    83.0         2000   8  1024 x 2048    34.1    28.3    22.6    35.4
     //     98304 64  1408 x 2048       .    1157     462     365          32768  8  1024 x 2048       .    273     118     96.8
-    const auto busy_entries = [&](int edge) { return total_rows / edge + (num_experts < total_rows ? num_experts : total_rows); };      // row tiles at most
     const auto tiles = [&](float edge, float more) { return rows / edge + more * experts > experts ? rows / edge + more * experts : experts; };
     const auto rounds = [&](float n) { const float r = n / static_cast<float>(num_cus()); return static_cast<float>(static_cast<int>(r) + 1); };
     const float k = static_cast<float>(p.K);
@@ -782,12 +780,12 @@ int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offse
         best = (passes > 0.8f ? passes + 0.5f : 1.0f) * (5.6f + k * 128.0f / 51e3f);
         shape = 3;
     }
-    if (ktiles >= kSlimStages) {
+    if (ktiles >= kSlimStages && num_experts <= kMostExperts) {
         const float r = rounds(tiles(kSlimEdge, 0.6f) * static_cast<float>((p.N + kSlimEdge - 1) / kSlimEdge));
         const float t = (r > 1.0f ? r : 1.25f) * (static_cast<float>(ktiles) * 0.50f + 6.0f);
         if (t < best) { best = t; shape = kSlimEdge; }
     }
-    if (ktiles >= 3) {
+    if (ktiles >= 3 && num_experts <= kMostExperts) {
         const float t = rounds(tiles(BM, 0.5f) * static_cast<float>((p.N + BN - 1) / BN)) * (static_cast<float>(ktiles) * 1.3f + 11.7f);
         if (t < best) { best = t; shape = BM; }
     }
@@ -796,16 +794,14 @@ int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offse
     // 256 x 6144: 16 x 16 12.9, 32 x 32 13, 32 x 64 16.3; 16 rows, 2 of 512 x 4096: 9.2, 10.7, 12).
     const bool fills = experts * static_cast<float>(columns64) >= static_cast<float>(num_cus());
     if (rows <= (fills ? 24.0f : 32.0f) * static_cast<float>(num_experts)) shape = fills ? 7 : rows <= 10.0f * experts ? 0 : 1;
-    if (shape == BM) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, counts, offsets, total_rows, num_experts, st);
-    if (shape == kSlimEdge) return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, counts, offsets, total_rows, num_experts, st);
-    GemmArgs q = p;
-    q.tiles_m = q.map_entries = busy_entries(BM);
-    build_tile_map(counts, offsets, num_experts, q.map_entries, total_rows, const_cast<int*>(q.tile_map), st);
+    if (shape == BM) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, st);
+    if (shape == kSlimEdge) return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, st);
+    p.tiles_m = total_rows / BM + (num_experts < total_rows ? num_experts : total_rows);
     if (shape == 3) {
         const long long each = (static_cast<long long>(total_rows) + 64LL * num_experts - 1) / (64LL * num_experts);
-        q.tiles_m *= each < 3 ? static_cast<int>(each) + 1 : 4;           // workgroups for the passes of an entry of 256 rows
+        p.tiles_m *= each < 3 ? static_cast<int>(each) + 1 : 4;           // workgroups for the passes of 256 rows
     }
-    return grouped_gemm_nt_direct(q, 0, EPI_NONE, SCALE_BLOCK, shape, st);
+    return grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, shape, st);
 }
 
 }  // namespace cf

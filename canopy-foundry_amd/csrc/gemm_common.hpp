@@ -37,6 +37,8 @@ struct GemmArgs {
     // grouped (per-expert) form, ring and small-tile kernels; all null / 0 for a dense GEMM
     const int* tile_map;         // [0] = number of row tiles, then kMapWords words per row tile: expert, its first row, end row, first tile, tiles
     int map_entries;             // small-tile kernel: row tiles the table has room for (tiles_m may be several times that: workgroups that share an entry)
+    const int *counts, *offsets; // block scales: the experts' rows themselves
+    int num_experts;
     const int* a_row_index;      // compact row r reads A row (and its descale) a_row_index[r]; null = r
     int a_rows;                  // rows of the A buffer (= M without a row index)
     long long b_expert_stride;   // bytes between the weight matrices of consecutive experts
@@ -46,6 +48,13 @@ struct GemmArgs {
     // columns of B, and the matrix cores scale its products by 2^(-4 t)
     int b_k_period;
 };
+
+// An expert's rows in the compact buffers, cut at the rows those hold (p.M).
+struct ExpertRows { int first, rows; };
+__device__ __forceinline__ ExpertRows expert_rows(const GemmArgs& p, int e) {
+    const int first = p.offsets[e];
+    return {first, first >= 0 && first < p.M ? max(0, min(p.counts[e], p.M - first)) : 0};
+}
 
 template <int I, int N, class F>
 __device__ __forceinline__ void static_for(F&& f) {
@@ -121,8 +130,8 @@ int gemm_nt_block_wide(GemmArgs p, hipStream_t st);
 bool block_slim_ok(const GemmArgs& p);
 float block_slim_estimate_us(const GemmArgs& p);
 int gemm_nt_block_slim(GemmArgs p, hipStream_t st);
-// the grouped form; p.tile_map is the workspace, of cf_fp8_grouped_gemm_workspace_bytes, that it builds its own table in
-int grouped_gemm_nt_block(const GemmArgs& p, const int* counts, const int* offsets, int total_rows, int num_experts, hipStream_t st);
+// the grouped form, which goes by the counts and offsets themselves and needs no table
+int grouped_gemm_nt_block(GemmArgs p, hipStream_t st);
 // gemm_accum.hip
 bool accum_wide_ok(const GemmArgs& p, int fmt, int epi, int scale_mode);
 float accum_wide_estimate_us(const GemmArgs& p);

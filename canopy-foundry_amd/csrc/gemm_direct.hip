@@ -50,17 +50,50 @@ void k_gemm_nt_direct(const GemmArgs p, const int rowcol, const int bias, const 
         // A table entry is up to 256 rows of an expert, walked TM at a time.  Where the rows lie on few experts there are fewer entries
         // than workgroups to a column of tiles: those beyond the last entry take every second, third, ... pass of the entries
         // before.  (64 experts of 2 x 1408 x 2048, 1280 rows all on one: 53 us with its entries walked by a workgroup each.)
-        const int* e = p.tile_map + 1 + kMapWords * min(tm, p.map_entries - 1);            // the usual one, read beside the number of entries
-        int number = e[0], first = e[1], last = e[2], first_tile = e[3];
-        const int entries = __builtin_amdgcn_readfirstlane(min(p.tile_map[0], p.map_entries));
+        // With block scales the entries are counted here instead, an expert a lane, by every wavefront for itself: a table of 64 experts took 3 us
+        // and its launch, and reading it as long as counting does.
+        int number = 0, first = 0, last = 0, first_tile = 0, entries;
+        auto find = [&](int entry) {
+            if constexpr (BLOCK) {
+                int before = 0;
+                for (int e0 = 0; e0 < p.num_experts; e0 += kWave) {
+                    const int e = e0 + lane;
+                    ExpertRows r = {0, 0};
+                    if (e < p.num_experts) r = expert_rows(p, e);
+                    const int n = (r.rows + BM - 1) / BM;
+                    int incl = n;
+#pragma unroll
+                    for (int off = 1; off < kWave; off <<= 1) {
+                        const int v = __shfl_up(incl, off, kWave);
+                        if (lane >= off) incl += v;
+                    }
+                    incl += before;
+                    const unsigned long long behind = __ballot(entry < incl);
+                    const int all = __shfl(incl, 63, kWave);
+                    if (entry >= before && behind) {
+                        const int at = __ffsll(behind) - 1;
+                        number = e0 + at;
+                        first = __shfl(r.first, at, kWave);
+                        last = first + __shfl(r.rows, at, kWave);
+                        first_tile = __shfl(incl - n, at, kWave);
+                    }
+                    before = all;
+                }
+                entries = __builtin_amdgcn_readfirstlane(before);
+            } else {
+                const int* e = p.tile_map + 1 + kMapWords * min(entry, p.map_entries - 1);            // the usual one, read beside the number of entries
+                number = e[0]; first = e[1]; last = e[2]; first_tile = e[3];
+                entries = __builtin_amdgcn_readfirstlane(min(p.tile_map[0], p.map_entries));
+            }
+        };
+        find(tm);
         if (entries <= 0) return;
         int entry = tm, part = 0, parts = tm + entries < p.tiles_m ? 2 : 1;
         if (tm >= entries || 2 * entries < p.tiles_m) {
             part = tm / entries;
             entry = tm - part * entries;
             parts = (p.tiles_m - 1 - entry) / entries + 1;
-            e = p.tile_map + 1 + kMapWords * entry;
-            number = e[0]; first = e[1]; last = e[2]; first_tile = e[3];
+            find(entry);
         }
         expert = __builtin_amdgcn_readfirstlane(number);
         m_first = __builtin_amdgcn_readfirstlane(first) + (entry - __builtin_amdgcn_readfirstlane(first_tile)) * BM;
