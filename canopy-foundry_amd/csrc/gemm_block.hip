@@ -759,48 +759,48 @@ int grouped_gemm_nt_block(GemmArgs p, hipStream_t st) {
     });
     if (err != hipSuccess) return static_cast<int>(err);
     const float rows = static_cast<float>(total_rows), experts = static_cast<float>(num_experts < total_rows ? num_experts : total_rows);
-    const int ktiles = p.K / BK;
-    // Microseconds, table and launches aside, for rows that lie evenly: rounds of workgroups or tiles over the CUs, fitted to 3200 sizes of more than 24 rows an
-    // expert (of which 10 % then ran over 1.1 times the best, 4 % over 1.25).  An expert has 0.6 of a small tile (0.5 of
-    // a large one) more than its rows fill, and one at least.  Measured us, chosen first (rows, experts, N, K: 32 x 64, 64 x 64, 128 x 128, 256 x 256 tiles):
-    //     96    64  1408 x 2048     31.7    47.7    48.2    67.7         1000  16  1536 x 4096    48.4    40.5    32.3    56.3
-    //     1280  64  1408 x 2048     43.1    64.5    57.3    72.2         4000  16  2048 x 7168       .    234     141     120
-    //     2560  64  1408 x 2048     64.4    71.2    55.6    75.1         500    8  1024 x 2048    18.3    14.1    21.4    34.3
-    //     8000  64  1408 x 2048     145     143     76.5    83.0         2000   8  1024 x 2048    34.1    28.3    22.6    35.4
-    //     98304 64  1408 x 2048       .    1157     462     365          32768  8  1024 x 2048       .    273     118     96.8
+    const int ktiles = p.K / BK, columns64 = (p.N + 63) / 64;
+    // Microseconds for rows that lie evenly: rounds of workgroups or tiles over the CUs.  An expert has half of a tile (0.6 of a small one) more than its rows
+    // fill, and one at least.  Fitted to 5200 sizes, of which 10 % run over 1.1 times the best kernel, 3 % over 1.25; some of them, us:
+    //     rows  experts N x K     32 x 64  64 x 64  128 x 128  256 x 256        rows  experts N x K     32 x 64  64 x 64  128 x 128  256 x 256
+    //     96    64  1408 x 2048     28.5     45       38         52             1000  16  1536 x 4096     46.3     38.8     25.9       38.5
+    //     1280  64  1408 x 2048     41.3     64.9     46.8       56.0           4000  16  2048 x 7168       .      241      134        114
+    //     2560  64  1408 x 2048     62.5     71.0     48.2       59.0           500    8  1024 x 2048     16.5     12.7     14.8       22.9
+    //     8000  64  1408 x 2048     146      148      68.1       71.6           2000   8  1024 x 2048       .      28.6     15.9       30.4
+    //     98304 64  1408 x 2048       .     1170      465        340            32768  8  1024 x 2048       .      274      114        93.4
     const auto tiles = [&](float edge, float more) { return rows / edge + more * experts > experts ? rows / edge + more * experts : experts; };
     const auto rounds = [&](float n) { const float r = n / static_cast<float>(num_cus()); return static_cast<float>(static_cast<int>(r) + 1); };
-    const float k = static_cast<float>(p.K);
-    const int columns64 = (p.N + 63) / 64;
-    // 64 rows at a time, side by side; the LDS of the small-tile kernel holds the scales of that many rows up to K = 16000
-    float best = 1e30f;
-    int shape = 7;                  // of the small-tile kernel, or the tile edge.  (Two or three K-tiles for four wavefronts: 16809 rows, 128 experts of 1536 x 256 67 us, in 64 x 64 157)
-    const float passes = tiles(64.0f, 0.6f) * static_cast<float>(columns64) / static_cast<float>(num_cus());
-    if (ktiles >= 4 && ktiles <= 120) {
-        best = (passes > 0.8f ? passes + 0.5f : 1.0f) * (5.6f + k * 128.0f / 51e3f);
-        shape = 3;
-    }
-    if (ktiles >= kSlimStages && num_experts <= kMostExperts) {
-        const float r = rounds(tiles(kSlimEdge, 0.6f) * static_cast<float>((p.N + kSlimEdge - 1) / kSlimEdge));
-        const float t = (r > 1.0f ? r : 1.25f) * (static_cast<float>(ktiles) * 0.50f + 6.0f);
-        if (t < best) { best = t; shape = kSlimEdge; }
-    }
-    if (ktiles >= 3 && num_experts <= kMostExperts) {
-        const float t = rounds(tiles(BM, 0.5f) * static_cast<float>((p.N + BN - 1) / BN)) * (static_cast<float>(ktiles) * 1.3f + 11.7f);
-        if (t < best) { best = t; shape = BM; }
-    }
+    int shape = 3, beside = 1;      // of the small-tile kernel, or the tile edge; workgroups for the 64-row passes of an entry of 256 rows
     // Up to 24 rows an expert most have one pass of 32 x 64: their weights are read once, which is all of the time (4.6 TB/s).  Where that leaves CUs without
-    // one, fewer columns and up to 32 rows (8 experts of 1024 x 2048, 200 rows: 11.8 us and 13.8), and few rows besides (12 rows, 64 experts of
+    // one, fewer columns and up to 36 rows (8 experts of 1024 x 2048, 200 rows: 10.1 us and 11.9), and few rows besides (12 rows, 64 experts of
     // 256 x 6144: 16 x 16 12.9, 32 x 32 13, 32 x 64 16.3; 16 rows, 2 of 512 x 4096: 9.2, 10.7, 12).
     const bool fills = experts * static_cast<float>(columns64) >= static_cast<float>(num_cus());
-    if (rows <= (fills ? 24.0f : 32.0f) * static_cast<float>(num_experts)) shape = fills ? 7 : rows <= 10.0f * experts ? 0 : 1;
+    if (rows <= (fills ? 24.0f : 36.0f) * static_cast<float>(num_experts)) {
+        shape = fills ? 7 : rows <= 10.0f * experts ? 0 : 1;
+    } else if (ktiles >= 3) {
+        float best = 1e30f;
+        // the LDS of the small-tile kernel holds the scales of 64 rows up to K = 16000
+        if (ktiles >= 4 && ktiles <= 120) {
+            const float passes = tiles(64.0f, 0.6f) * static_cast<float>(columns64) / static_cast<float>(num_cus());
+            best = (passes > 0.8f ? passes + 0.5f : 1.0f) * (9.0f + static_cast<float>(ktiles) * 0.32f);
+            const long long each = (static_cast<long long>(total_rows) + 64LL * num_experts - 1) / (64LL * num_experts);
+            beside = each < 3 ? static_cast<int>(each) + 1 : 4;
+        }
+        if (ktiles >= kSlimStages && num_experts <= kMostExperts) {
+            const float r = rounds(tiles(kSlimEdge, 0.5f) * static_cast<float>((p.N + kSlimEdge - 1) / kSlimEdge));
+            const float t = (r > 1.0f ? r : 1.25f) * (static_cast<float>(ktiles) * 0.50f + 6.0f);
+            if (t < best) { best = t; shape = kSlimEdge; }
+        }
+        if (num_experts <= kMostExperts) {
+            const float t = rounds(tiles(BM, 0.5f) * static_cast<float>((p.N + BN - 1) / BN)) * (static_cast<float>(ktiles) * 1.1f + 11.7f);
+            if (t < best) shape = BM;
+        }
+        if (shape == 3 && ktiles > 120) shape = 7;          // more experts than the tile kernels' LDS counts, and a long K
+    }
     if (shape == BM) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, st);
     if (shape == kSlimEdge) return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, st);
     p.tiles_m = total_rows / BM + (num_experts < total_rows ? num_experts : total_rows);
-    if (shape == 3) {
-        const long long each = (static_cast<long long>(total_rows) + 64LL * num_experts - 1) / (64LL * num_experts);
-        p.tiles_m *= each < 3 ? static_cast<int>(each) + 1 : 4;           // workgroups for the passes of 256 rows
-    }
+    if (shape == 3) p.tiles_m *= beside;
     return grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, shape, st);
 }
 
