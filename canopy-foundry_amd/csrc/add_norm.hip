@@ -113,16 +113,21 @@ __device__ __forceinline__ void store8_bf16(uint16_t* p, size_t at, int n, const
         if (n & 1) q[n - 1] = static_cast<uint16_t>(n == 1 ? o[0] : n == 3 ? o[1] : n == 5 ? o[2] : o[3]);
     }
 }
-template <bool F32, bool TAIL>
+// An fp32 chunk goes in two halves, so that a line is written by two instructions.  PAST_L2 lets them leave at once (forward: 2000 rows of 7168 28.3 us, 33.8 without); the gradient's lines are gathered in the L2 (8192 x 4096 90.1 -> 87.9 us).
+template <bool F32, bool TAIL, bool PAST_L2>
 __device__ __forceinline__ void store8_stream(void* p, size_t at, int n, const float (&v)[8]) {
     if constexpr (!F32) {
         store8_bf16<TAIL>(static_cast<uint16_t*>(p), at, n, v);
     } else {
         f32x4_any* q = reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + at);
         const f32x4_any a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-        if (!TAIL || n >= 4) __builtin_nontemporal_store(a, q);
+        if (!TAIL || n >= 4) {
+            if constexpr (PAST_L2) __builtin_nontemporal_store(a, q);
+            else *q = a;
+        }
         if (!TAIL || n >= 8) {
-            __builtin_nontemporal_store(b, q + 1);
+            if constexpr (PAST_L2) __builtin_nontemporal_store(b, q + 1);
+            else q[1] = b;
         } else {
             float* r = static_cast<float*>(p) + at;
 #pragma unroll
@@ -283,7 +288,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNor
     float ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        if (p.sum && has(j)) store8_stream<F32, TAIL>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
+        if (p.sum && has(j)) store8_stream<F32, TAIL, true>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
         float part = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[j][i], h[j][i], part);
@@ -464,7 +469,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm_grad(const A
                     top = max(top, abs_bits(d[i]));
                 }
             }
-            if (has(j)) store8_stream<F32, TAIL>(p.dr, base + (t + j * T) * 8, left(j), d);
+            if (has(j)) store8_stream<F32, TAIL, false>(p.dr, base + (t + j * T) * 8, left(j), d);
             if constexpr (QUANT) {
                 const bool finite = __all(top < kInf) && s_finite;
 #pragma unroll

@@ -161,6 +161,47 @@ def main():
         lambda: cf.cf_rmsnorm_clip_quantize_rows(x, gamma, M, K, 1e-6, ceiling, 0, None, None, q, rs, rd, st))
     hbm("rmsnorm_clip_quantize_record (fused, per-tensor)", f"{M}x{K}", 5.0 * n,
         lambda: cf.cf_rmsnorm_clip_quantize_record(x, gamma, M, K, 1e-6, ceiling, 0, normed, None, q, sc, amax, st))
+    # the residual layer: addition + norm + quantize in one pass, its gradient, the clipping of what the weight gradients wrote
+    x2 = bf16(M, K); rms = torch.empty(M, device=dev); hsum = torch.empty_like(x)
+    gs = f32(M, K // 128); gd = f32(M, K // 128)
+    hbm("add_rmsnorm_quantize_rows", f"{M}x{K}", 7.0 * n + 8 * M,
+        lambda: cf.cf_add_rmsnorm_quantize_rows(x, x2, 0, gamma, M, K, 1e-6, 0, hsum, None, rms, q, rs, rd, st))
+    hbm("add_rmsnorm_quantize_block_1x128", f"{M}x{K}", 7.0 * n + n / 16,
+        lambda: cf.cf_add_rmsnorm_quantize_block_1x128(x, x2, 0, gamma, M, K, 1e-6, hsum, None, rms, q, gs, gd, st))
+
+    def recorded():
+        amax.zero_()
+        cf.cf_add_rmsnorm_quantize_record(x, x2, 0, gamma, M, K, 1e-6, 0, hsum, None, rms, q, sc, amax, st)
+    hbm("add_rmsnorm_quantize_record, amax cleared before", f"{M}x{K}", 7.0 * n, recorded)
+    x32 = x.float(); s32 = torch.empty_like(x32)
+    hbm("add_rmsnorm_quantize_rows, fp32 stream, keeps the bf16 row", f"{M}x{K}", 13.0 * n + 8 * M,
+        lambda: cf.cf_add_rmsnorm_quantize_rows(x32, x2, 1, gamma, M, K, 1e-6, 0, s32, normed, rms, q, rs, rd, st))
+    bsz = ctypes.c_size_t(0)
+    cf.raw_cf_add_rmsnorm_backward_workspace_bytes(M, K, ctypes.byref(bsz))
+    bws = u8(bsz.value); dgamma = torch.zeros(K, device=dev); dr = torch.empty_like(x)
+    hbm("add_rmsnorm_backward", f"{M}x{K}", 8.0 * n,
+        lambda: cf.cf_add_rmsnorm_backward(x2, hsum, 0, gamma, rms, x, M, K, dr, dgamma, 0, bws, bsz.value, st))
+    hbm("add_rmsnorm_backward_quant_e5m2", f"{M}x{K}", 9.0 * n,
+        lambda: cf.cf_add_rmsnorm_backward_quant_e5m2(x2, hsum, 0, gamma, rms, x, M, K, dr, dgamma, 0, q, sc, amax, bws, bsz.value, st))
+    del x32, s32, dr
+    if any(args.only in name for name in ("grad_norm", "grad_clip in place (given norm)")):
+        grads = [torch.randn(4 * K * K + 3 * K * N, device=dev, generator=g) * 1e-3, torch.randn(K, device=dev, generator=g)]
+        ptrs = torch.tensor([t.data_ptr() for t in grads], dtype=torch.int64)
+        counts_, types = torch.tensor([t.numel() for t in grads], dtype=torch.int64), torch.ones(2, dtype=torch.int32)
+        gsz = ctypes.c_size_t(0)
+        cf.cf_grad_list_bytes(counts_, 2, ctypes.byref(gsz))
+        table = torch.empty(gsz.value, dtype=torch.uint8)
+        cf.cf_grad_list_fill(ptrs, None, counts_, types, 2, table, gsz.value)
+        table = table.to(dev)
+        nsz = ctypes.c_size_t(0)
+        cf.cf_grad_norm_workspace_bytes(ctypes.byref(nsz))
+        nws = u8(nsz.value); norm = torch.zeros(1, device=dev); coef = torch.zeros(1, device=dev)
+        nbytes = 4.0 * sum(t.numel() for t in grads)
+        hbm("grad_norm", f"{nbytes / 1e6:.0f} MB fp32", nbytes, lambda: cf.cf_grad_norm(table, gsz.value, norm, nws, nsz.value, st))
+        one_norm = torch.ones(1, device=dev) * 2.0
+        hbm("grad_clip in place (given norm)", f"{nbytes / 1e6:.0f} MB fp32", 2 * nbytes,
+            lambda: cf.cf_grad_clip(table, gsz.value, 1.999, one_norm, coef, st))
+        del grads, table
     h = bf16(M, N)
     hq = u8(M, N)
     hbm("quantize_rows (per-token, one pass)", f"{M}x{N}", 3.0 * h.numel() + 8 * M,
@@ -312,6 +353,11 @@ def main():
     mfma("grouped down projection (config 5)", f"{total}x{H}x{Ie}", 2.0 * total * Ie * H,
          lambda: cf.cf_fp8_grouped_gemm_nt_bf16_ex(total, H, Ie, E, counts, offs, actq, total, Ie, None, ad, wd, wdd, 1, 0, None, None,
                                                    yy, H, ws, sz.value, st))
+    hbd = f32(T, H // 128); wgb = f32(E * Ie // 128, H // 128); acb = f32(total, Ie // 128); wdb = f32(E * H // 128, Ie // 128)
+    mfma("grouped block-scaled, gathered rows", f"{total}x{Ie}x{H}", 2.0 * total * Ie * H,
+         lambda: cf.cf_fp8_grouped_gemm_nt_bf16_ex(total, Ie, H, E, counts, offs, hq, T, H, cidx, hbd, wg, wgb, 2, 0, None, None, act, Ie, ws, sz.value, st))
+    mfma("grouped block-scaled, rows in expert order", f"{total}x{H}x{Ie}", 2.0 * total * Ie * H,
+         lambda: cf.cf_fp8_grouped_gemm_nt_bf16_ex(total, H, Ie, E, counts, offs, actq, total, Ie, None, acb, wd, wdb, 2, 0, None, None, yy, H, ws, sz.value, st))
     # the config 5 shapes as dense GEMMs (one expert's weights for all rows): what the short K costs without the
     # grouping, on the 256 x 256-tile kernel and on the two-workgroups-per-CU kernel
     mfma("dense at the config 5 shape: gate+up SiLU-gate", f"{total}x2x{Ie}x{H}", 4.0 * total * Ie * H,
