@@ -225,7 +225,7 @@ __device__ __forceinline__ void raise_first(float* amax, uint32_t m, unsigned ro
 }
 __device__ __forceinline__ void raise_last(float* amax, uint32_t m, unsigned row, int rows, float before) {
     if (raises_at_once(row, rows) || __uint_as_float(m) <= before) return;
-    __builtin_amdgcn_s_sleep(48);           // 3072 cycles
+    __builtin_amdgcn_s_sleep(48);           // 48 x 64 cycles
     if (__uint_as_float(m) > atomic_load_agent(amax)) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
 }
 
