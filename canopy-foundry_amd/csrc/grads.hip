@@ -189,7 +189,7 @@ int cf_grad_list_fill(void* const* d_tensors, void* const* d_out, const size_t* 
                       size_t list_bytes) {
     size_t need = 0;
     if (const int rc = cf_grad_list_bytes(counts, num_tensors, &need)) return rc;
-    if (list_bytes < need || (need && (!list || !d_tensors || !types))) return CF_ERR_INVALID_ARG;
+    if (list_bytes < need || (list_bytes && !list) || (need && (!d_tensors || !types))) return CF_ERR_INVALID_ARG;
     for (int i = 0; i < num_tensors; ++i) {
         if (counts[i] == 0) continue;
         const unsigned el = types[i] == CF_GRAD_F32 ? 4 : 2;
