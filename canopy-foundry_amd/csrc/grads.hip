@@ -153,9 +153,9 @@ __global__ __launch_bounds__(kThreads) void k_grad_clip(const Entry* __restrict_
 
 bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
-// the number of entries of a list, or an error below zero
+// the number of entries of a list, or an error below zero.  The kernels step beyond the last one in 32 bits.
 long long entries_of(const void* d_list, size_t list_bytes) {
-    if (list_bytes % sizeof(Entry) != 0 || list_bytes / sizeof(Entry) > 0xffffffffull) return CF_ERR_INVALID_ARG;
+    if (list_bytes % sizeof(Entry) != 0 || list_bytes / sizeof(Entry) > 0x7fffffffull) return CF_ERR_INVALID_ARG;
     if (list_bytes && (!d_list || misaligned(d_list, 16))) return CF_ERR_INVALID_ARG;
     return static_cast<long long>(list_bytes / sizeof(Entry));
 }

@@ -19,3 +19,11 @@ def test_bytes_to_clear_need_a_list(cf):
     image = torch.full((96,), 0xa5, dtype=torch.uint8)
     assert fill(cf, [0, 0], image.data_ptr(), 64) == 0
     assert bool((image[:64] == 0).all()) and bool((image[64:] == 0xa5).all())
+
+
+def test_lists_that_32_bits_do_not_walk(cf):
+    """A workgroup's walk steps over the entries in 32 bits, up to 2048 + 4096 beyond the last one: a list of that many less than 2^32 would never end."""
+    for entries in (2 ** 31, 2 ** 32 - 4096, 2 ** 32 - 1, 2 ** 32):
+        assert cf.raw_cf_grad_norm(P, entries * 32, P, P, 1 << 20, None) == -1
+        assert cf.raw_cf_grad_clip(P, entries * 32, 1.0, P, None, None) == -1
+        assert cf.raw_cf_grad_norm_clip(P, entries * 32, 1.0, P, None, P, 1 << 20, None) == -1
