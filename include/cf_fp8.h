@@ -243,7 +243,7 @@ int cf_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, 
  * y), h = d_sum and rms as the forward pass left them, dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
  *     xh = h / rms,  g = dy * scale,  d_grad_residual = T(dh + (g - xh * mean(g * xh)) / rms)
  * which is the gradient of r and, as bf16 or 8 bits, of x;   d_grad_scale [H] fp32 = (accumulate ? itself : 0) + sum over rows of dy * xh,
- * the rows added in an order that follows from rows and H alone.  d_grad_residual may be d_grad_sum.  rows = 0 leaves zeros in d_grad_scale
+ * the rows added in 64 bits, but for one rounding to fp32 for each workgroup's rows, in an order that follows from rows and H alone.  d_grad_residual may be d_grad_sum.  rows = 0 leaves zeros in d_grad_scale
  * unless it accumulates.  d_workspace: 16-byte aligned, cf_add_rmsnorm_backward_workspace_bytes() bytes; it belongs to the call. */
 int cf_add_rmsnorm_backward_workspace_bytes(int rows, int H, size_t* bytes);
 int cf_add_rmsnorm_backward(const uint16_t* d_grad_normed, const void* d_sum, int stream_is_f32, const uint16_t* d_scale, const float* d_rms,
