@@ -244,8 +244,8 @@ __device__ __forceinline__ void raise_last(float* amax, uint32_t m, unsigned row
 // anything needs the slow conversion, which keeps NaN codes.
 template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNormArgs p) {
-    __shared__ float sh_sum[16];
-    __shared__ uint32_t sh_max[2][16];
+    __shared__ float sh_sum[2][16];
+    __shared__ uint32_t sh_max[3][16];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     unsigned row = p.row0 + blockIdx.x;
     int t = threadIdx.x;
@@ -287,17 +287,43 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_add_norm(const AddNor
                 }
             }
     }
-    float ss = 0.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
+    for (int j = 0; j < V; ++j)
         if (p.sum && has(j)) store8_stream<F32, TAIL, true>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
-        float part = 0.0f;
+    auto mean_square = [&](float* sh) {
+        float ss = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[j][i], h[j][i], part);
-        ss += part;
+        for (int j = 0; j < V; ++j) {
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[j][i], h[j][i], part);
+            ss += part;
+        }
+        return row_sum<ONE_WAVE>(ss, sh) / static_cast<float>(H);
+    };
+    float mean = mean_square(sh_sum[0]) + p.eps;
+    // Squares that leave fp32 (|h| of 1e19 and more, or of 1e-15 and less under as small an eps): once more with the row and eps scaled by a power of two, which
+    // y does not see.  A row that holds infinities or NaNs stays as it is.
+    int e = 0;
+    if (!(mean >= 1e-30f && mean < __builtin_inff())) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, abs_bits(h[j][i]));
+        m = row_max<ONE_WAVE>(m, sh_max[2]);
+        const float most = fmaxf(__uint_as_float(m), sqrtf(p.eps));
+        if (m < kInf && most > 0.0f) {
+            e = __builtin_amdgcn_frexp_expf(most);
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[j][i] = ldexpf(h[j][i], -e);
+            mean = mean_square(sh_sum[1]) + ldexpf(p.eps, -2 * e);
+        }
     }
-    const float rms = sqrtf(row_sum<ONE_WAVE>(ss, sh_sum) / static_cast<float>(H) + p.eps);
-    if (t == 0 && p.rms) p.rms[row] = rms;
+    const float rms = sqrtf(mean);
+    if (t == 0 && p.rms) p.rms[row] = ldexpf(rms, e);
     const float inv = 1.0f / rms;
 
     const float F = p.e5m2 ? 57344.0f : 448.0f;

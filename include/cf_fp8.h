@@ -220,7 +220,7 @@ int cf_rmsnorm_clip_quantize_record(const uint16_t* d_x, const uint16_t* d_scale
  * d_sum [rows, H] receives h and may be d_residual; d_normed [rows, H] receives bf16(y) and may be d_x; d_rms [rows] is what the
  * backward pass takes.  All three may be null.  The 8-bit output is made from the fp32 y: y is rounded once on that way, where
  * cf_rmsnorm_clip_quantize_rows rounds it to bf16 first, as the reference's launches do.  A maximum leaves NaNs out; a NaN is NaN in
- * the output.  eps is above 0, or no row is all zeros.  H <= 16384, else CF_ERR_UNSUPPORTED; otherwise any H and any alignment
+ * the output.  Rows may be of any magnitude whose squares leave fp32.  eps is above 0, or no row is all zeros.  H <= 16384, else CF_ERR_UNSUPPORTED; otherwise any H and any alignment
  * that the elements have.  Rows are contiguous. */
 
 /* Per-row scales: scale = 448 (57344: is_e5m2) / max(max|y|, 1e-12), descale its inverse, as cf_fp8_quantize_rows
@@ -240,7 +240,7 @@ int cf_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, 
                                    float* d_amax, cf_stream_t stream);
 
 /* The gradient of the three (the quantize counts as the identity); no counterpart in the reference's fp8 path.  With dy = d_grad_normed [rows, H] bf16 (the gradient of
- * y), h = d_sum and rms as the forward pass left them, dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
+ * y), h = d_sum and rms as the forward pass left them (rms at least 2^-126, the least normal number), dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
  *     xh = h / rms,  g = dy * scale,  d_grad_residual = T(dh + (g - xh * mean(g * xh)) / rms)
  * which is the gradient of r and, as bf16 or 8 bits, of x;   d_grad_scale [H] fp32 = (accumulate ? itself : 0) + sum over rows of dy * xh,
  * the rows added in 64 bits, but for one rounding to fp32 for each workgroup's rows, in an order that follows from rows and H alone.  d_grad_residual may be d_grad_sum.  rows = 0 leaves zeros in d_grad_scale
