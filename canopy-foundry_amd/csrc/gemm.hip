@@ -2439,12 +2439,14 @@ int cf_fp8_grouped_gemm_nt_bf16_static(int total_rows, int N, int K, int num_exp
     size_t need = 0;
     const int rc = cf_fp8_grouped_gemm_workspace_bytes(total_rows, num_experts, &need);
     if (rc != CF_OK) return rc;
-    if (need > kStaticMapBytes) return CF_ERR_UNSUPPORTED;       // the table of this many row tiles does not fit the fixed array
     void* ptr = nullptr;
-    const int sc = static_scratch(&ptr);
-    if (sc != CF_OK) return sc;
-    // The table is rebuilt from the counts by every call (k_build_tile_map writes the entry count and every entry the
-    // GEMM reads), so nothing of the previous call's contents is used and nothing needs clearing.
+    if (scale_mode != SCALE_BLOCK) {                             // with block scales there is no table
+        if (need > kStaticMapBytes) return CF_ERR_UNSUPPORTED;   // the table of this many row tiles does not fit the fixed array
+        const int sc = static_scratch(&ptr);
+        if (sc != CF_OK) return sc;
+    }
+    // The table is rebuilt from the counts by every call that has one (k_build_tile_map writes the entry count and every entry
+    // the GEMM reads), so nothing of the previous call's contents is used and nothing needs clearing.
     return cf::grouped_gemm_nt_bf16(total_rows, N, K, num_experts, d_counts, d_offsets, A, a_rows, lda, d_a_row_index, a_descale, B,
                                     b_descale, scale_mode, epilogue, B_up, b_up_descale, C, ldc, ptr, kStaticMapBytes,
                                     true, 0, stream);
@@ -2491,7 +2493,7 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     if (total_rows < 0 || N < 0 || K < 0 || num_experts < 0 || a_rows < 0) return CF_ERR_INVALID_ARG;
     if (a_is_e5m2 && epilogue != EPI_NONE) return CF_ERR_UNSUPPORTED;
     if (total_rows == 0 || N == 0 || num_experts == 0) return CF_OK;
-    if (!d_counts || !d_offsets || !A || !B || !C || !a_descale || !b_descale || !d_workspace) return CF_ERR_INVALID_ARG;
+    if (!d_counts || !d_offsets || !A || !B || !C || !a_descale || !b_descale) return CF_ERR_INVALID_ARG;
     if (epilogue != EPI_NONE && epilogue != EPI_SILU_GATE) return CF_ERR_INVALID_ARG;
     if (epilogue == EPI_SILU_GATE && (!B_up || !b_up_descale)) return CF_ERR_INVALID_ARG;
     if (scale_mode != SCALE_TENSOR && scale_mode != SCALE_ROWCOL && scale_mode != SCALE_BLOCK) return CF_ERR_INVALID_ARG;
@@ -2499,9 +2501,11 @@ int cf::grouped_gemm_nt_bf16(int total_rows, int N, int K, int num_experts, cons
     // per-tensor descales would need one device scalar per expert for the weights: not built.  Rejected before
     // anything is launched, so a refused call leaves the workspace untouched.
     if (scale_mode == SCALE_TENSOR) return CF_ERR_UNSUPPORTED;
-    size_t need = 0;
-    cf_fp8_grouped_gemm_workspace_bytes(total_rows, num_experts, &need);
-    if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(d_workspace) & 3u)) return CF_ERR_INVALID_ARG;
+    if (scale_mode != SCALE_BLOCK) {            // with block scales the kernels count the row tiles themselves
+        size_t need = 0;
+        cf_fp8_grouped_gemm_workspace_bytes(total_rows, num_experts, &need);
+        if (!d_workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(d_workspace) & 3u)) return CF_ERR_INVALID_ARG;
+    }
     // what the ring kernel takes (the small-tile kernel would take more: a refusal must not depend on the number of rows)
     if (K % BK != 0 || K < 2 * BK || lda % 16 != 0 || !aligned16(A) || !aligned16(B) ||
         (epilogue == EPI_SILU_GATE && !aligned16(B_up)) || lda < K || ldc < N ||

@@ -470,7 +470,7 @@ int cf_fp8_grouped_gemm_workspace_bytes(int total_rows, int num_experts, size_t*
  * N a multiple of 8 (of 128 with the SiLU-gate epilogue), ldc % 8 == 0, 16-byte aligned operands,
  * descales and C, and a_rows * lda, N * K below 2^32.
  * scale_mode: CF_SCALE_ROW_COL, or CF_SCALE_BLOCK_128 with a_descale [a_rows, K/128] (the row index applies to its rows), b_descale
- * [num_experts, ceil(N/128), K/128], no fused epilogue and K <= 32768. */
+ * [num_experts, ceil(N/128), K/128], no fused epilogue and K <= 32768; that mode needs no workspace (d_workspace may be null). */
 int cf_fp8_grouped_gemm_nt_bf16_ex(int total_rows, int N, int K, int num_experts,
                                    const int* d_counts, const int* d_offsets, const void* d_A,
                                    int a_rows, int lda, const int* d_a_row_index, const float* d_a_descale,
@@ -488,6 +488,7 @@ int cf_fp8_grouped_gemm_nt_bf16_ex(int total_rows, int N, int K, int num_experts
  * 3276 row tiles, total_rows / 256 + num_experts) returns CF_ERR_UNSUPPORTED and launches nothing.  Every
  * call on a GPU shares that GPU's array: calls that may overlap in time on one GPU (different streams,
  * different host threads) race on it and must be serialised by the caller; calls on one stream are ordered.
+ * With CF_SCALE_BLOCK_128 there is no table: neither the limit nor the rule about overlapping calls applies.
  * cf_fp8_grouped_gemm_static_max_bytes is also the set-up call: it looks up the array's address on the
  * current device, so a caller that will record the entry point into a graph calls it once per device first
  * (without it the first call of the entry point on a device does the lookup). */
