@@ -413,7 +413,9 @@ int launch_plain(const GemmArgs& p, int epi, int scale_mode, int shape, hipStrea
             else return launch<FMT, false, BLOCK, GROUPED, 4, 2, 4, 2>(p, epi, scale_mode, st);
         case 3: return launch<FMT, false, BLOCK, GROUPED, 4, 4, 4, 2>(p, epi, scale_mode, st);
         default:
-            if constexpr (GROUPED) {
+            if constexpr (GROUPED && BLOCK) {          // 16 x 64 is not among the shapes that the rule for block scales takes
+                return shape == kWideShape + 1 ? launch<FMT, false, BLOCK, GROUPED, 2, 4, 4, 1>(p, epi, scale_mode, st) : CF_ERR_UNSUPPORTED;
+            } else if constexpr (GROUPED) {
                 return shape == kWideShape ? launch<FMT, false, BLOCK, GROUPED, 1, 4, 4, 2>(p, epi, scale_mode, st)
                                            : launch<FMT, false, BLOCK, GROUPED, 2, 4, 4, 1>(p, epi, scale_mode, st);
             } else if constexpr (BLOCK) return CF_ERR_UNSUPPORTED;
