@@ -15,6 +15,7 @@
 // registers, so the barrier stands there: behind it the next K-tile is visible and read under the last group, and the copies of the
 // K-tile after that go into the stage just left.
 #include "gemm_common.hpp"
+#include "grouped_block_plan.hpp"
 
 #include <mutex>
 
@@ -33,7 +34,6 @@ constexpr int kWideWaitVm0 = 0x0f70, kWideWaitVm16 = 0x4f70;      // s_waitcnt v
 // ---- the grouped form's row tiles ----
 // A workgroup counts the experts' row tiles into LDS before it begins (a kernel of its own for the table took 6 to 10 us and its launch): `first_tile` [experts + 1]
 // is the number of tiles before each expert's.
-constexpr int kMostExperts = 2048;
 constexpr int kTilesLds = (kMostExperts + 1 + 8) * 4;
 template <int TM>
 __device__ __forceinline__ int count_tiles(const GemmArgs& p, int* first_tile) {
@@ -423,9 +423,7 @@ void k_gemm_nt_block_wide(const GemmArgs p) {
 // What bounds it: the copies.  A K-tile is 512 cycles of MFMAs per SIMD and 32 KiB, of which a CU takes in about 37 bytes a cycle (0.4 us); LDS reads
 // (96 KiB) take 768 cycles.  So the stages are many rather than large, and operands are single: block by block the next K-tile's are read as this one's
 // fall free, with the other wavefront of the SIMD under way.
-constexpr int kSlimEdge = 128;
 constexpr int kSlimStage = 2 * kSlimEdge * BK;          // 32 KiB: activations, then weights
-constexpr int kSlimStages = 4;
 constexpr int kSlimSa = kSlimStages * kSlimStage;       // activation scales: a row of 128 floats per stage
 constexpr int kSlimSb = kSlimSa + kSlimStages * kSlimEdge * 4;      // weight-block scales: 2 tile parities x 256 floats
 constexpr int kSlimOut = kSlimSb + 2 * kWideMaxKb * 4;  // 2 KiB per wavefront in which the output is turned round
@@ -738,6 +736,7 @@ int gemm_nt_block_slim(GemmArgs p, hipStream_t st) {
 }
 
 namespace {
+static_assert(kPlanEdge == BM && kPlanEdge == BN && kPlanK == BK);
 static_assert(kWideLds + kTilesLds <= 160 * 1024 && kSlimLds + kTilesLds <= 160 * 1024);
 template <int TM, int TN, class Kernel>
 int launch_grouped(Kernel kernel, int lds, GemmArgs p, hipStream_t st) {
@@ -758,50 +757,12 @@ int grouped_gemm_nt_block(GemmArgs p, hipStream_t st) {
             err = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_gemm_nt_block_slim<true>), hipFuncAttributeMaxDynamicSharedMemorySize, kSlimLds + kTilesLds);
     });
     if (err != hipSuccess) return static_cast<int>(err);
-    const float rows = static_cast<float>(total_rows), experts = static_cast<float>(num_experts < total_rows ? num_experts : total_rows);
-    const int ktiles = p.K / BK, columns64 = (p.N + 63) / 64;
-    // Microseconds for rows that lie evenly: rounds of workgroups or tiles over the CUs.  An expert has half of a tile (0.6 of a small one) more than its rows
-    // fill, and one at least.  Fitted to 5200 sizes, of which 10 % run over 1.1 times the best kernel, 3 % over 1.25; some of them, us:
-    //     rows  experts N x K     32 x 64  64 x 64  128 x 128  256 x 256        rows  experts N x K     32 x 64  64 x 64  128 x 128  256 x 256
-    //     96    64  1408 x 2048     28.5     45       38         52             1000  16  1536 x 4096     46.3     38.8     25.9       38.5
-    //     1280  64  1408 x 2048     41.3     64.9     46.8       56.0           4000  16  2048 x 7168       .      241      134        114
-    //     2560  64  1408 x 2048     62.5     71.0     48.2       59.0           500    8  1024 x 2048     16.5     12.7     14.8       22.9
-    //     8000  64  1408 x 2048     146      148      68.1       71.6           2000   8  1024 x 2048       .      28.6     15.9       30.4
-    //     98304 64  1408 x 2048       .     1170      465        340            32768  8  1024 x 2048       .      274      114        93.4
-    const auto tiles = [&](float edge, float more) { return rows / edge + more * experts > experts ? rows / edge + more * experts : experts; };
-    const auto rounds = [&](float n) { const float r = n / static_cast<float>(num_cus()); return static_cast<float>(static_cast<int>(r) + 1); };
-    int shape = 3, beside = 1;      // of the small-tile kernel, or the tile edge; workgroups for the 64-row passes of an entry of 256 rows
-    // Up to 24 rows an expert most have one pass of 32 x 64: their weights are read once, which is all of the time (4.6 TB/s).  Where that leaves CUs without
-    // one, fewer columns and up to 36 rows (8 experts of 1024 x 2048, 200 rows: 10.1 us and 11.9), and few rows besides (12 rows, 64 experts of
-    // 256 x 6144: 16 x 16 12.9, 32 x 32 13, 32 x 64 16.3; 16 rows, 2 of 512 x 4096: 9.2, 10.7, 12).
-    const bool fills = experts * static_cast<float>(columns64) >= static_cast<float>(num_cus());
-    if (rows <= (fills ? 24.0f : 36.0f) * static_cast<float>(num_experts)) {
-        shape = fills ? 7 : rows <= 10.0f * experts ? 0 : 1;
-    } else if (ktiles >= 3) {
-        float best = 1e30f;
-        // the LDS of the small-tile kernel holds the scales of 64 rows up to K = 16000
-        if (ktiles >= 4 && ktiles <= 120) {
-            const float passes = tiles(64.0f, 0.6f) * static_cast<float>(columns64) / static_cast<float>(num_cus());
-            best = (passes > 0.8f ? passes + 0.5f : 1.0f) * (9.0f + static_cast<float>(ktiles) * 0.32f);
-            const long long each = (static_cast<long long>(total_rows) + 64LL * num_experts - 1) / (64LL * num_experts);
-            beside = each < 3 ? static_cast<int>(each) + 1 : 4;
-        }
-        if (ktiles >= kSlimStages && num_experts <= kMostExperts) {
-            const float r = rounds(tiles(kSlimEdge, 0.5f) * static_cast<float>((p.N + kSlimEdge - 1) / kSlimEdge));
-            const float t = (r > 1.0f ? r : 1.25f) * (static_cast<float>(ktiles) * 0.50f + 6.0f);
-            if (t < best) { best = t; shape = kSlimEdge; }
-        }
-        if (num_experts <= kMostExperts) {
-            const float t = rounds(tiles(BM, 0.5f) * static_cast<float>((p.N + BN - 1) / BN)) * (static_cast<float>(ktiles) * 1.1f + 11.7f);
-            if (t < best) shape = BM;
-        }
-        if (shape == 3 && ktiles > 120) shape = 7;          // more experts than the tile kernels' LDS counts, and a long K
-    }
-    if (shape == BM) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, st);
-    if (shape == kSlimEdge) return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, st);
+    const GroupedBlockPlan plan = grouped_block_plan(total_rows, num_experts, p.N, p.K, num_cus());
+    if (plan.shape == BM) return launch_grouped<BM, BN>(k_gemm_nt_block_wide<true>, kWideLds, p, st);
+    if (plan.shape == kSlimEdge) return launch_grouped<kSlimEdge, kSlimEdge>(k_gemm_nt_block_slim<true>, kSlimLds, p, st);
     p.tiles_m = total_rows / BM + (num_experts < total_rows ? num_experts : total_rows);
-    if (shape == 3) p.tiles_m *= beside;
-    return grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, shape, st);
+    p.tiles_m *= plan.beside;
+    return grouped_gemm_nt_direct(p, 0, EPI_NONE, SCALE_BLOCK, plan.shape, st);
 }
 
 }  // namespace cf
