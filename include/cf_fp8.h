@@ -220,8 +220,8 @@ int cf_rmsnorm_clip_quantize_record(const uint16_t* d_x, const uint16_t* d_scale
  * d_sum [rows, H] receives h and may be d_residual; d_normed [rows, H] receives bf16(y) and may be d_x; d_rms [rows] is what the
  * backward pass takes.  All three may be null.  The 8-bit output is made from the fp32 y: y is rounded once on that way, where
  * cf_rmsnorm_clip_quantize_rows rounds it to bf16 first, as the reference's launches do.  A maximum leaves NaNs out; a NaN is NaN in
- * the output.  Rows may be of any magnitude whose squares leave fp32.  eps is above 0, or no row is all zeros.  H <= 16384, else CF_ERR_UNSUPPORTED; otherwise any H and any alignment
- * that the elements have.  Rows are contiguous. */
+ * the output.  Rows may be of any magnitude, their squares may leave fp32.  eps is above 0, or no row is all zeros.  H <= 16384, else
+ * CF_ERR_UNSUPPORTED; otherwise any H and any alignment that the elements have.  Rows are contiguous. */
 
 /* Per-row scales: scale = 448 (57344: is_e5m2) / max(max|y|, 1e-12), descale its inverse, as cf_fp8_quantize_rows
  * (kernels/fp8.cu:37-39,49). */
@@ -239,12 +239,13 @@ int cf_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, 
                                    float eps, int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_rms, void* d_q, const float* d_qscale,
                                    float* d_amax, cf_stream_t stream);
 
-/* The gradient of the three (the quantize counts as the identity); no counterpart in the reference's fp8 path.  With dy = d_grad_normed [rows, H] bf16 (the gradient of
- * y), h = d_sum and rms as the forward pass left them (rms at least 2^-126, the least normal number), dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
+/* The gradient of the three (the quantize counts as the identity); no counterpart in the reference's fp8 path.  With dy = d_grad_normed
+ * [rows, H] bf16 (the gradient of y), h = d_sum and rms as the forward pass left them (rms at least 2^-126, the least normal number),
+ * dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
  *     xh = h / rms,  g = dy * scale,  d_grad_residual = T(dh + (g - xh * mean(g * xh)) / rms)
  * which is the gradient of r and, as bf16 or 8 bits, of x;   d_grad_scale [H] fp32 = (accumulate ? itself : 0) + sum over rows of dy * xh,
- * the rows added in 64 bits, but for one rounding to fp32 for each workgroup's rows, in an order that follows from rows and H alone.  d_grad_residual may be d_grad_sum.  rows = 0 leaves zeros in d_grad_scale
- * unless it accumulates.  d_workspace: 16-byte aligned, cf_add_rmsnorm_backward_workspace_bytes() bytes; it belongs to the call. */
+ * the rows added in 64 bits, but for one rounding to fp32 for each workgroup's rows, in an order that follows from rows and H alone.
+ * d_grad_residual may be d_grad_sum.  rows = 0 leaves zeros in d_grad_scale unless it accumulates.  d_workspace: 16-byte aligned, cf_add_rmsnorm_backward_workspace_bytes() bytes; it belongs to the call. */
 int cf_add_rmsnorm_backward_workspace_bytes(int rows, int H, size_t* bytes);
 int cf_add_rmsnorm_backward(const uint16_t* d_grad_normed, const void* d_sum, int stream_is_f32, const uint16_t* d_scale, const float* d_rms,
                             const void* d_grad_sum, int rows, int H, void* d_grad_residual, float* d_grad_scale, int accumulate,
@@ -263,7 +264,8 @@ int cf_add_rmsnorm_backward_quant_e5m2(const uint16_t* d_grad_normed, const void
  * The list is a table of the tensors' addresses and sizes, made once for buffers that stay where they are: cf_grad_list_bytes gives its
  * size, cf_grad_list_fill writes it to host memory (d_tensors, d_out, counts, types and list are host arrays), the caller copies it to
  * the device, 16-byte aligned, and passes that and its size to the calls below.  d_out: where the clipped gradients go, null = in place;
- * an output is its own input or overlaps no tensor.  Tensors need no more than their elements' alignment; a count of 0 takes no address. */
+ * an output is its own input or overlaps no tensor.  Tensors need no more than their elements' alignment; a count of 0 takes no address.
+ * A list has less than 2^31 runs; bytes behind those that it needs are cleared. */
 #define CF_GRAD_BF16 0
 #define CF_GRAD_F32  1
 int cf_grad_list_bytes(const size_t* counts, int num_tensors, size_t* bytes);
@@ -272,7 +274,8 @@ int cf_grad_list_fill(void* const* d_tensors, void* const* d_out, const size_t* 
 /* The norm alone (no counterpart, as above).  d_workspace: 16-byte aligned, this many bytes for any list; it belongs to the call. */
 int cf_grad_norm_workspace_bytes(size_t* bytes);
 int cf_grad_norm(const void* d_list, size_t list_bytes, float* d_norm, void* d_workspace, size_t workspace_bytes, cf_stream_t stream);
-/* Clips by a norm the caller has (no counterpart, as above; over several GPUs: the root of the sum of their squares).  max_norm >= 0, infinity = leave them;
+/* Clips by a norm the caller has (no counterpart, as above; over several GPUs: the root of the sum of their squares, squared and summed
+ * in 64 bits, since the square of a norm above 1.8e19 or below 1e-23 leaves fp32).  max_norm >= 0, infinity = leave them;
  * d_coef may be null and is not d_norm. */
 int cf_grad_clip(const void* d_list, size_t list_bytes, float max_norm, const float* d_norm, float* d_coef, cf_stream_t stream);
 /* Both (no counterpart, as above): the same norm and the same bits as the two calls. */
