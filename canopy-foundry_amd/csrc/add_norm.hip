@@ -232,7 +232,8 @@ __device__ __forceinline__ void raise_last(float* amax, uint32_t m, unsigned row
 // A row is held in registers, V chunks of eight elements a thread, chunk c by thread c % T: one read and one write of everything.  Sixteen
 // threads next to each other hold a scale group of 128.  TAIL: H is no multiple of 8, the last chunk is a part.
 // What bounds it: HBM, and for few rows the chain load - sum - maximum - store.  Both want a row on as many threads as it has chunks.  Threads a row x
-// chunks a thread, one row a workgroup (64: four rows), us:
+// chunks a thread, one row a workgroup (64: four rows), several sets of buffers in turn (one over and over, a part of which stays in the last-level cache:
+// 8192 x 4096 36 us), us:
 //     rows x H                        512 x 1   256 x 2   128 x 4    64 x 8   1024 x 1
 //     1 x 4096, bf16                    3.4       3.8       5.0       7.0       3.6
 //     512 x 4096                        4.6       4.8       6.2       8.7       5.4

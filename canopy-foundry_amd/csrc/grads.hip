@@ -1,7 +1,7 @@
 // The global norm of a list of gradients, and the gradients clipped by it:
 //     S = sum over all tensors of g^2,  norm = sqrt(S),  coef = norm > max_norm ? max_norm / norm : 1,  out = T(g * coef).
-// What bounds it: HBM; the gradients are read twice, but for 256 MB that stay in the last-level cache.  The sum of 3.9 GB in fp32 runs at 6.6 TB/s, both at 6.2 (a
-// copy of 4 GiB at 4.9).
+// What bounds it: HBM; the gradients are read twice, but for up to 256 MB that stay in the last-level cache.  The sum of 3.9 GB in fp32 runs at 6.5 to 6.6 TB/s, both
+// at 5.7 to 6.2, by the card (a copy of 4 GiB at 4.9).
 // S is summed in 64 bits: the square of a large or a small fp32 gradient does not fit fp32, and a billion terms lose their last bits there.
 // The sums' order follows from the list alone, so the same gradients give the same norm.
 #include "common.hpp"
@@ -13,7 +13,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr size_t kChunk = 16384;                // elements of one entry at most
-constexpr unsigned kCached = 4096;              // entries at the list's end that the sum leaves in the caches for the clipping, which begins there
+// entries at the list's end that the sum leaves in the caches for the clipping, which begins there: 256 MB of fp32, 128 MB of bf16
+constexpr unsigned kCached = 4096;
 constexpr int kMaxParts = 2048;                 // workgroups that leave a partial sum
 
 struct Entry {                                  // a run of one tensor's elements
@@ -159,7 +160,7 @@ long long entries_of(const void* d_list, size_t list_bytes) {
     if (list_bytes && (!d_list || misaligned(d_list, 16))) return CF_ERR_INVALID_ARG;
     return static_cast<long long>(list_bytes / sizeof(Entry));
 }
-// Workgroups: 2048 over a long list (3.9 GB: 1884 us, 1024 of them 1946), 1024 over a short one, whose partial sums are the longer part (3000 tensors
+// Workgroups: 2048 over a long list (3.9 GB: 1884 us, 1024 of them 1946 on the same card; 2064 on another), 1024 over a short one, whose partial sums are the longer part (3000 tensors
 // of 300: 15.0 us and 12.0).
 unsigned grid_of(long long entries) {
     const long long most = entries >= 8192 ? kMaxParts : kMaxParts / 2;
