@@ -240,7 +240,8 @@ int cf_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, 
                                    float* d_amax, cf_stream_t stream);
 
 /* The gradient of the three (the quantize counts as the identity); no counterpart in the reference's fp8 path.  With dy = d_grad_normed
- * [rows, H] bf16 (the gradient of y), h = d_sum and rms as the forward pass left them (rms at least 2^-126, the least normal number),
+ * [rows, H] bf16 (the gradient of y), h = d_sum and rms as the forward pass left them (rms from 2^-126 to 2^126: beyond, it or its
+ * inverse is subnormal and has fewer bits),
  * dh = d_grad_sum [rows, H] (what reaches h past the norm; null = nothing):
  *     xh = h / rms,  g = dy * scale,  d_grad_residual = T(dh + (g - xh * mean(g * xh)) / rms)
  * which is the gradient of r and, as bf16 or 8 bits, of x;   d_grad_scale [H] fp32 = (accumulate ? itself : 0) + sum over rows of dy * xh,

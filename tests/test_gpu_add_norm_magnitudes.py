@@ -58,3 +58,26 @@ def test_gradient_with_the_rms_of_the_forward_pass(cf, dev, monkeypatch, size, f
         dy = (1e-2 * size * torch.randn(rows, H, generator=g)).to(torch.bfloat16)         # so that dy / rms stays a normal number
         got = backward(cf, dev, fwd["sum"], w, fwd["rms"], dy, None, f32, quant, 1.0)
         check_backward(got, fwd["sum"], w, fwd["rms"], dy, None, quant, 1.0)
+
+
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("size", [3e-38, 1e-39, 1e-40, 3e38])
+def test_forward_of_rows_at_the_ends_of_the_type(cf, dev, monkeypatch, size, f32):
+    """Rows of subnormal numbers without eps, rows up to the largest number: y and the bytes are as for any other row; rms, where it is subnormal itself, is off by
+    half of a subnormal step, 2^-150, at most."""
+    monkeypatch.setattr(base, "EPS", 0.0)
+    for rows, H in SIZES:
+        case(f"add-norm rows={rows} H={H} up to {size} f32={f32}")
+        g = torch.Generator().manual_seed(H)
+        r, x = size * (2 * torch.rand(rows, H, generator=g, dtype=torch.float64) - 1), 0.0 * torch.rand(rows, H, generator=g, dtype=torch.float64)
+        x[:, ::3] = r[:, ::3] * -0.5
+        r, x, w = r.to(STREAM[f32]), x.to(torch.bfloat16), gamma_of(H, H + 2)
+        r[0, 0] = size
+        x[0, 0] = 0.0
+        got = forward(cf, dev, r, x, w, f32, "rows", 0)
+        h = (r.float() + x.float()).to(r.dtype)
+        assert torch.equal(got["sum"], h) and bool(torch.isfinite(h).all())
+        rms = h.double().square().mean(1).sqrt()
+        assert torch.all((got["rms"].double() - rms).abs() <= base.R * rms + 2.0 ** -150)
+        got["rms"] = torch.where(rms < 2.0 ** -126, rms, got["rms"].double())          # looked at above
+        check_forward(got, r, x, w, "rows", 0)
