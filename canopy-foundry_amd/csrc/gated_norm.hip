@@ -1,0 +1,756 @@
+// A block's output normed, gated and added to the scaled residual stream, then the next norm with its 8-bit output, in one pass; and its gradient.
+//
+// Forward, per row:  px = sqrt(mean(x^2) + eps),  xh = x / px,  h = T(res * r + gate * (xh * wp)),  p = sqrt(mean(h^2) + eps),  hh = h / p,
+// y = hh * w,  q = sat_rne(y * F / max|y| of the scale group).  T is the type the residual stream is kept in; the second norm reads h as it is stored.
+// Kept for the backward pass: px, p, and either the rows themselves or 8-bit checkpoints of the normalised rows, e4m3(xh * S) and e4m3(hh * S).  No element of
+// a normalised row is above sqrt(H), so S is the largest power of two with S * sqrt(H) <= 448, the same for every row: no maximum to look for, no scale to keep.
+//
+// Backward, per row:  g = dy * w,  D = dh + (g - hh * mean(g * hh)) / p,  dr = T(res * D),  e = D * gate * wp,  dx = (e - xh * mean(e * xh)) / px;
+// over the rows:  dw = sum(dy * hh);  over a gate's rows:  P = sum(D * xh),  dgate = wp * P;  over the gates:  dwp = sum(gate * P).
+#include "rows.hpp"
+
+#include <cmath>
+#include <type_traits>
+
+namespace cf {
+namespace {
+
+struct GatedNormArgs {
+    const void* residual;         // [rows, H] bf16 or fp32
+    const uint16_t* x;            // [rows, H] bf16
+    const uint16_t* gate;         // [ceil(rows / gate_rows), H] bf16 or null
+    const uint16_t* post_weight;  // [H] bf16
+    const uint16_t* weight;       // [H] bf16
+    void* sum;                    // [rows, H] like residual, or null
+    uint16_t* normed;             // [rows, H] bf16 or null
+    float *post_rms, *rms;        // [rows] or null
+    uint8_t *x8, *sum8;           // [rows, H] or null
+    uint8_t* q;                   // [rows, H]
+    float *scale, *descale;       // Q_ROWS: [rows]; Q_BLOCK: [rows, ceil(H / 128)]
+    const float* qscale;          // Q_RECORD
+    float* amax;
+    int rows, H, gate_rows;
+    unsigned row0;                // the launch's first row
+    float eps, res, kept;
+    int e5m2;
+};
+
+__device__ __forceinline__ float pair_at(const u32x4_any& v, int i) { return (i & 1) ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]); }
+
+// One row in registers, V chunks of eight elements a thread, as k_add_norm holds it: everything is read and written once.
+template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
+__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm(const GatedNormArgs p) {
+    __shared__ float sh_sum[4][16];
+    __shared__ uint32_t sh_max[4][16];
+    const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
+    unsigned row = p.row0 + blockIdx.x;
+    int t = threadIdx.x;
+    if constexpr (ONE_WAVE) {
+        row = __builtin_amdgcn_readfirstlane(p.row0 + blockIdx.x * 4 + (threadIdx.x >> 6));
+        t &= 63;
+        if (row >= static_cast<unsigned>(p.rows)) return;
+    }
+    const int chunks = TAIL ? (H + 7) / 8 : H / 8;
+    const size_t base = static_cast<size_t>(row) * H;
+    auto left = [&](int j) { return TAIL ? H - (t + j * T) * 8 : 8; };      // elements from chunk j of this thread on
+    auto has = [&](int j) { return t + j * T < chunks; };
+    const bool follows = static_cast<size_t>(p.rows - 1 - row) * H >= 7;         // elements behind this row, as many as a last chunk lacks
+
+    float h[V][8];
+    Raw8<F32> r[V];
+    u32x4_any w[V], wp[V], gate[V];
+    const uint16_t* gates = p.gate ? p.gate + static_cast<size_t>(row / static_cast<unsigned>(p.gate_rows)) * H : nullptr;
+    {
+        Raw8<false> x[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            clear8(r[j]);
+            clear8(x[j]);
+            w[j] = wp[j] = gate[j] = u32x4_any{0, 0, 0, 0};
+            if (has(j)) {
+                const int at = (t + j * T) * 8;
+                load8<false, TAIL>(p.x, base + at, left(j), follows, x[j]);
+                load8<F32, TAIL>(p.residual, base + at, left(j), follows, r[j]);
+                wp[j] = load_weight<TAIL>(p.post_weight, at, left(j), H);
+                if (gates) gate[j] = load_weight<TAIL>(gates, at, left(j), H);
+                w[j] = load_weight<TAIL>(p.weight, at, left(j), H);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[j][i] = value8<false, TAIL>(x[j], i, left(j));
+    }
+    // the checkpoint of a normalised row: its values are finite where its root mean square is, and not zero
+    auto keep = [&](uint8_t* to, int j, float inv, bool finite) {
+        if (!to || !has(j)) return;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = h[j][i] * inv * p.kept;
+        store8_fp8<TAIL>(to, base + (t + j * T) * 8, left(j), false, finite, v);
+    };
+    auto is_number = [](float rms) { return rms > 0.0f && rms < __builtin_inff(); };
+
+    int e;
+    const float post_rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum, sh_max[2], e);
+    if (t == 0 && p.post_rms) p.post_rms[row] = ldexpf(post_rms, e);
+    const float post_inv = 1.0f / post_rms;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        keep(p.x8, j, post_inv, is_number(post_rms));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float z = h[j][i] * post_inv * pair_at(wp[j], i);
+            if (gates) z *= pair_at(gate[j], i);
+            h[j][i] = __builtin_fmaf(p.res, value8<F32, TAIL>(r[j], i, left(j)), z);
+            if constexpr (!F32) h[j][i] = round_bf16_hw(h[j][i]);
+        }
+        if (p.sum && has(j)) store8_stream<F32, TAIL, true>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
+    }
+
+    const float rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum + 2, sh_max[3], e);
+    if (t == 0 && p.rms) p.rms[row] = ldexpf(rms, e);
+    const float inv = 1.0f / rms;
+    const float F = p.e5m2 ? 57344.0f : 448.0f;
+    uint32_t top[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        keep(p.sum8, j, inv, is_number(rms));
+        top[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            h[j][i] = h[j][i] * inv * pair_at(w[j], i);        // y from here on
+            top[j] = max(top[j], abs_bits(h[j][i]));
+        }
+        if (p.normed && has(j)) store8_bf16<TAIL>(p.normed, base + (t + j * T) * 8, left(j), h[j]);
+    }
+    // the largest |y| of a chunk without its NaNs
+    auto number = [&](int j) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(h[j][i]));
+        return __float_as_uint(m);
+    };
+    auto quantize = [&](int j, float s, bool finite) {
+        if (!has(j)) return;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = h[j][i] * s;
+        store8_fp8<TAIL>(p.q, base + (t + j * T) * 8, left(j), p.e5m2, finite, v);
+    };
+    if constexpr (QMODE == Q_BLOCK) {
+        const int groups = (H + 127) >> 7;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            uint32_t m = max16(top[j]);
+            const bool finite = __all(m < kInf);
+            if (!finite) m = max16(number(j));
+            const float a = fmaxf(__uint_as_float(m), 1e-12f), s = F / a;
+            const int c = t + j * T;
+            if ((c & 15) == 0 && has(j)) {
+                p.scale[static_cast<size_t>(row) * groups + (c >> 4)] = s;
+                p.descale[static_cast<size_t>(row) * groups + (c >> 4)] = a / F;
+            }
+            quantize(j, s, finite);
+        }
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = max(m, top[j]);
+        m = row_max<ONE_WAVE>(m, sh_max[0]);
+        bool finite = m < kInf;
+        if (!finite) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) n = max(n, number(j));
+            m = row_max<ONE_WAVE>(n, sh_max[1]);
+        }
+        float s, before = 0.0f;
+        if constexpr (QMODE == Q_ROWS) {
+            const float a = fmaxf(__uint_as_float(m), 1e-12f);
+            s = F / a;
+            if (t == 0) { p.scale[row] = s; p.descale[row] = a / F; }
+        } else {
+            s = *p.qscale;
+            if (t == 0) raise_first(p.amax, m, row, p.rows, before);
+            finite = finite && abs_bits(s) < kInf;         // 0 times infinity
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) quantize(j, s, finite);
+        if constexpr (QMODE == Q_RECORD) {
+            if (t == 0) raise_last(p.amax, m, row, p.rows, before);
+        }
+    }
+}
+
+struct GatedGradArgs {
+    const uint16_t* dy;           // [rows, H] bf16: the gradient of y
+    const void *sum, *x;          // [rows, H] h and x, or hh and xh in 8 bits
+    const uint16_t *gate, *post_weight, *weight;
+    const float *post_rms, *rms;  // [rows]
+    const void* dh;               // [rows, H] the residual stream's gradient, or null
+    void* dr;                     // [rows, H]
+    uint16_t* dx;                 // [rows, H] bf16 or null
+    uint8_t* q;                   // [rows, H] E5M2 of dx, or null
+    const float* qscale;
+    float* amax;
+    float* dgate;                 // GROUPS: [groups, H], written here for a group that one worker has whole
+    int accumulate_gate;
+    float* part_w;                // [parts, H] shares of dw
+    float* part_p;                // [parts, H] shares of P (GROUPS: of dwp)
+    float* part_amax;             // [parts]
+    float* segments;              // GROUPS: [workers, 2, H] shares of P of the groups that several workers have
+    int rows, H, gate_rows, groups, workers;
+    float res, kept_inv;
+};
+
+// Eight elements of a saved row: as it was, or the normalised row in 8 bits.
+template <bool F32, bool KEPT>
+struct Saved8 {
+    std::conditional_t<KEPT, u32x2_any, Raw8<F32>> v;
+    template <bool TAIL>
+    __device__ __forceinline__ void load(const void* p, size_t at, int n, bool whole) {
+        if constexpr (!KEPT) {
+            clear8(v);
+            if (n > 0) load8<F32, TAIL>(p, at, n, whole, v);
+        } else {
+            v = u32x2_any{0, 0};
+            if (n > 0) v = load8_bytes<TAIL>(static_cast<const uint8_t*>(p), at, n, whole);
+        }
+    }
+    // the normalised values; inv: 1 / rms, or of a checkpoint 1 / S
+    template <bool TAIL>
+    __device__ __forceinline__ void values(float (&o)[8], int n, float inv) const {
+        if constexpr (!KEPT) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = value8<F32, TAIL>(v, i, n) * inv;
+        } else {
+            unpack8_e4m3(v, inv, o);
+            if constexpr (TAIL) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = i < n ? o[i] : 0.0f;
+            }
+        }
+    }
+};
+
+// Which rows a worker has where groups of them share a gate: equal shares, or, where every worker has two groups or more, whole groups.
+__host__ __device__ inline bool whole_groups(int groups, int workers) { return groups >= 2 * static_cast<long long>(workers); }
+__host__ __device__ inline unsigned first_row(unsigned worker, int rows, int gate_rows, int groups, int workers) {
+    if (whole_groups(groups, workers)) {
+        const unsigned long long r = static_cast<unsigned long long>(worker) * groups / workers * gate_rows;
+        return static_cast<unsigned>(r < static_cast<unsigned>(rows) ? r : rows);
+    }
+    return static_cast<unsigned>(static_cast<unsigned long long>(worker) * rows / workers);
+}
+
+template <bool TAIL>
+__device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const float (&v)[8]) {
+    float* q = p + at;
+    if (!TAIL || n >= 8) {
+        reinterpret_cast<f32x4_any*>(q)[0] = f32x4_any{v[0], v[1], v[2], v[3]};
+        reinterpret_cast<f32x4_any*>(q)[1] = f32x4_any{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) q[i] = v[i];
+    }
+}
+
+// A worker (a workgroup; ONE_WAVE: a wavefront) holds a row as k_gated_norm does and loads the next row's operands before it works on one.  Its shares of
+// the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
+// workers take turns at the rows; GROUPS: each has rows next to each other, and leaves P at a group's end: dgate itself where it had the whole group.
+template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V>
+__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const GatedGradArgs p) {
+    __shared__ float sh[2][16];         // each is written again only behind the other one's barrier
+    __shared__ double sh_sum[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
+    const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
+    const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
+    const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
+    const unsigned rows = p.rows, step = GROUPS ? 1 : p.workers;
+    unsigned first = worker, end = rows;
+    if constexpr (GROUPS) {
+        first = end = rows;
+        if (worker < static_cast<unsigned>(p.workers)) {
+            first = first_row(worker, p.rows, p.gate_rows, p.groups, p.workers);
+            end = first_row(worker + 1, p.rows, p.gate_rows, p.groups, p.workers);
+        }
+    }
+    const int chunks = TAIL ? (H + 7) / 8 : H / 8;
+    auto left = [&](int j) { return TAIL ? H - (t + j * T) * 8 : 8; };
+    auto has = [&](int j) { return t + j * T < chunks; };
+
+    struct Row {
+        Raw8<false> dy[V];
+        Saved8<F32, KEPT> h[V];
+        Saved8<false, KEPT> x[V];
+        Raw8<F32> dh[V];
+        u32x4_any gate[GROUPS ? V : 1];
+        float rms, post_rms;
+    };
+    auto load = [&](Row& r, unsigned row) {
+        const size_t base = static_cast<size_t>(row) * H;
+        const bool follows = static_cast<size_t>(rows - 1 - row) * H >= 7;
+        const uint16_t* gates = GROUPS ? p.gate + static_cast<size_t>(row / static_cast<unsigned>(p.gate_rows)) * H : nullptr;
+        r.rms = p.rms[row];
+        r.post_rms = p.post_rms[row];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int at = (t + j * T) * 8, n = has(j) ? left(j) : 0;
+            clear8(r.dy[j]);
+            clear8(r.dh[j]);
+            r.h[j].template load<TAIL>(p.sum, base + at, n, follows);
+            r.x[j].template load<TAIL>(p.x, base + at, n, follows);
+            if constexpr (GROUPS) r.gate[j] = u32x4_any{0, 0, 0, 0};
+            if (n > 0) {
+                load8<false, TAIL>(p.dy, base + at, n, follows, r.dy[j]);
+                if (p.dh) load8<F32, TAIL>(p.dh, base + at, n, follows, r.dh[j]);
+                if constexpr (GROUPS) r.gate[j] = load_weight<TAIL>(gates, at, n, H);
+            }
+        }
+    };
+    u32x4_any w[V], wp[V], one_gate[V];
+    double dw[V][8], ps[V][8], dwp[GROUPS ? V : 1][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w[j] = wp[j] = u32x4_any{0, 0, 0, 0};
+        one_gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        if (has(j)) {
+            w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
+            wp[j] = load_weight<TAIL>(p.post_weight, (t + j * T) * 8, left(j), H);
+            if (!GROUPS && p.gate) one_gate[j] = load_weight<TAIL>(p.gate, (t + j * T) * 8, left(j), H);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            dw[j][i] = ps[j][i] = 0.0;
+            if constexpr (GROUPS) dwp[j][i] = 0.0;
+        }
+    }
+    const float s = p.q ? *p.qscale : 0.0f;
+    const bool s_finite = abs_bits(s) < kInf;
+    float amax = 0.0f;
+    unsigned group = 0, group_first = 0, group_end = 0;
+    if constexpr (GROUPS) {
+        group = first / static_cast<unsigned>(p.gate_rows);
+        group_first = group * p.gate_rows;
+    }
+    constexpr bool AHEAD = V == 1;          // 1024 threads have 128 registers each, too few for two rows of two chunks
+    Row r, next;
+    if (AHEAD && first < end) load(next, first);
+    for (unsigned row = first; row < end; row += step) {
+        if constexpr (AHEAD) {
+            r = next;
+            if (row + step < end) load(next, row + step);
+        } else {
+            load(r, row);
+        }
+        const size_t base = static_cast<size_t>(row) * H;
+        const float inv = 1.0f / r.rms, post_inv = 1.0f / r.post_rms;
+        float d[V][8], xh[V][8];
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            r.h[j].template values<TAIL>(d[j], left(j), KEPT ? p.kept_inv : inv);       // hh for now
+            r.x[j].template values<TAIL>(xh[j], left(j), KEPT ? p.kept_inv : post_inv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float dy = value8<false, TAIL>(r.dy[j], i, left(j));
+                dw[j][i] += static_cast<double>(dy * d[j][i]);
+                dot = __builtin_fmaf(dy * pair_at(w[j], i), d[j][i], dot);
+            }
+        }
+        const float c = row_sum<ONE_WAVE>(dot, sh[0]) / static_cast<float>(H);
+        dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const u32x4_any gate = GROUPS ? r.gate[GROUPS ? j : 0] : one_gate[j];
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float g = value8<false, TAIL>(r.dy[j], i, left(j)) * pair_at(w[j], i);
+                const float v = __builtin_fmaf(__builtin_fmaf(-d[j][i], c, g), inv, value8<F32, TAIL>(r.dh[j], i, left(j)));
+                o[i] = v * p.res;
+                ps[j][i] += static_cast<double>(v * xh[j][i]);
+                d[j][i] = v * (pair_at(gate, i) * pair_at(wp[j], i));                   // e from here on
+                dot = __builtin_fmaf(d[j][i], xh[j][i], dot);
+            }
+            if (has(j)) store8_stream<F32, TAIL, false>(p.dr, base + (t + j * T) * 8, left(j), o);
+        }
+        const float post_c = row_sum<ONE_WAVE>(dot, sh[1]) / static_cast<float>(H);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float o[8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                o[i] = __builtin_fmaf(-xh[j][i], post_c, d[j][i]) * post_inv;
+                amax = fmaxf(amax, fabsf(o[i]));
+                top = max(top, abs_bits(o[i]));
+            }
+            if (p.dx && has(j)) store8_bf16<TAIL>(p.dx, base + (t + j * T) * 8, left(j), o);
+            if (p.q) {
+                const bool finite = __all(top < kInf) && s_finite;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= s;
+                if (has(j)) store8_fp8<TAIL>(p.q, base + (t + j * T) * 8, left(j), true, finite, o);
+            }
+        }
+        if constexpr (GROUPS) {
+            group_end = group_first + p.gate_rows < rows ? group_first + p.gate_rows : rows;
+            if (row + 1 == group_end || row + 1 == end) {
+                const bool whole = group_first >= first && group_end <= end;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dwp[j][i] += ps[j][i] * static_cast<double>(pair_at(r.gate[j], i));
+                    if (has(j)) {
+                        const int at = (t + j * T) * 8;
+                        if (whole) {
+                            float* to = p.dgate + static_cast<size_t>(group) * H;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                double v = ps[j][i] * static_cast<double>(pair_at(wp[j], i));
+                                if (p.accumulate_gate && i < left(j)) v += static_cast<double>(to[at + i]);
+                                o[i] = static_cast<float>(v);
+                            }
+                            store8_f32<TAIL>(to, at, left(j), o);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) o[i] = static_cast<float>(ps[j][i]);
+                            store8_f32<TAIL>(p.segments + (static_cast<size_t>(worker) * 2 + (group_first >= first ? 1 : 0)) * H, at, left(j), o);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ps[j][i] = 0.0;
+                }
+                ++group;
+                group_first += p.gate_rows;
+            }
+        }
+    }
+    // the workgroup's shares
+    auto leave = [&](const double (&v)[V][8], float* to) {
+        float* part = to + static_cast<size_t>(blockIdx.x) * H;
+        if constexpr (ONE_WAVE) {
+            static_assert(V == 1);
+            const int wave = threadIdx.x >> 6;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sh_sum[wave][t * 8 + i] = v[0][i];
+            __syncthreads();
+            for (int i = threadIdx.x; i < H; i += 256) part[i] = static_cast<float>((sh_sum[0][i] + sh_sum[1][i]) + (sh_sum[2][i] + sh_sum[3][i]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (has(j)) {
+                    float o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = static_cast<float>(v[j][i]);
+                    store8_f32<TAIL>(part, (t + j * T) * 8, left(j), o);
+                }
+        }
+    };
+    leave(dw, p.part_w);
+    if constexpr (GROUPS) leave(dwp, p.part_p);
+    else leave(ps, p.part_p);
+    if (p.q) {
+        __syncthreads();
+        const uint32_t m = row_max<false>(__float_as_uint(amax), reinterpret_cast<uint32_t*>(sh[0]));
+        if (threadIdx.x == 0) p.part_amax[blockIdx.x] = __uint_as_float(m);
+    }
+}
+
+struct GatedSumArgs {
+    const float *part_w, *part_p, *part_amax;
+    const uint16_t *gate, *post_weight;
+    float *dw, *dwp, *dgate, *amax;
+    int H, parts, groups, accumulate, accumulate_gate;     // groups: 0 = no gate, 1 = one for all rows, which the shares of P do not hold yet
+};
+
+// The parts' shares added up in 64 bits, 32 columns a workgroup, 32 threads to a column that take every 32nd part: first dw's columns, then P's or dwp's; the
+// workgroup behind them raises *amax to the parts' maxima.
+constexpr int kSumColumns = 32, kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void k_gated_sum(const GatedSumArgs p) {
+    constexpr int kShares = kSumThreads / kSumColumns;
+    __shared__ double sh[kSumThreads];
+    const int t = threadIdx.x, blocks = (p.H + kSumColumns - 1) / kSumColumns;
+    if (static_cast<int>(blockIdx.x) >= 2 * blocks) {
+        uint32_t m = 0;
+        for (int b = t; b < p.parts; b += kSumThreads) m = max(m, __float_as_uint(p.part_amax[b]));
+        m = row_max<false>(m, reinterpret_cast<uint32_t*>(sh));
+        if (t == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
+        return;
+    }
+    const bool second = static_cast<int>(blockIdx.x) >= blocks;
+    const float* part = second ? p.part_p : p.part_w;
+    const int column = (blockIdx.x - (second ? blocks : 0)) * kSumColumns + t % kSumColumns, share = t / kSumColumns;
+    double v = 0.0;
+    if (column < p.H) {
+#pragma unroll 8
+        for (int b = share; b < p.parts; b += kShares) v += part[static_cast<size_t>(b) * p.H + column];
+    }
+    sh[t] = v;
+    __syncthreads();
+    if (share == 0 && column < p.H) {
+        v = 0.0;
+#pragma unroll
+        for (int g = 0; g < kShares; ++g) v += sh[g * kSumColumns + t];
+        if (second && p.groups == 1) {
+            const double d = v * static_cast<double>(bf16_to_f32(p.post_weight[column]));
+            p.dgate[column] = static_cast<float>(p.accumulate_gate ? static_cast<double>(p.dgate[column]) + d : d);
+            v *= static_cast<double>(bf16_to_f32(p.gate[column]));
+        }
+        float* to = second ? p.dwp : p.dw;
+        to[column] = static_cast<float>(p.accumulate ? static_cast<double>(to[column]) + v : v);
+    }
+}
+
+// dgate of the groups whose rows several workers had, from their segments in the order of the rows: 64 columns a workgroup, four threads to a column.
+__global__ __launch_bounds__(256) void k_gated_segments(const float* __restrict__ segments, const uint16_t* __restrict__ post_weight,
+                                                        float* __restrict__ dgate, int rows, int H, int gate_rows, int workers, int accumulate) {
+    __shared__ double sh[256];
+    const unsigned blocks = (H + 63) / 64, group = blockIdx.x / blocks;
+    const int column = (blockIdx.x % blocks) * 64 + (threadIdx.x & 63);
+    const unsigned start = group * gate_rows, end = start + gate_rows < static_cast<unsigned>(rows) ? start + gate_rows : rows;
+    // the worker that has a row: the last one that begins at or before it
+    const unsigned k0 = static_cast<unsigned>(((static_cast<unsigned long long>(start) + 1) * workers - 1) / rows);
+    const unsigned k1 = static_cast<unsigned>((static_cast<unsigned long long>(end) * workers - 1) / rows);
+    if (k0 == k1) return;
+    double v = 0.0;
+    if (column < H) {
+#pragma unroll 4
+        for (unsigned k = k0 + (threadIdx.x >> 6); k <= k1; k += 4) v += segments[(static_cast<size_t>(k) * 2 + (k == k0 ? 1 : 0)) * H + column];
+    }
+    sh[threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.x < 64 && column < H) {
+        v = ((sh[threadIdx.x] + sh[threadIdx.x + 64]) + (sh[threadIdx.x + 128] + sh[threadIdx.x + 192])) * static_cast<double>(bf16_to_f32(post_weight[column]));
+        float* to = dgate + static_cast<size_t>(group) * H + column;
+        *to = static_cast<float>(accumulate ? static_cast<double>(*to) + v : v);
+    }
+}
+
+float kept_scale(int H) {
+    int e = 0;
+    while (e < 8 && std::ldexp(1.0, 2 * (e + 1)) * H <= 448.0 * 448.0) ++e;
+    return std::ldexp(1.0f, e);
+}
+
+template <bool F32, int QMODE, bool TAIL>
+int launch_gated_norm(GatedNormArgs p, hipStream_t st) {
+    for (; p.row0 < static_cast<unsigned>(p.rows); p.row0 += kLaunchRows) {
+        const unsigned left = static_cast<unsigned>(p.rows) - p.row0, n = left < kLaunchRows ? left : kLaunchRows;
+        if (p.H <= kOneWaveH) k_gated_norm<F32, QMODE, TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
+        else if (p.H <= kOneChunkH) k_gated_norm<F32, QMODE, TAIL, false, 1><<<n, row_threads(p.H, 1), 0, st>>>(p);
+        else k_gated_norm<F32, QMODE, TAIL, false, 2><<<n, row_threads(p.H, 2), 0, st>>>(p);
+    }
+    return launch_status();
+}
+
+template <int QMODE>
+int gated_norm(const GatedNormArgs& p, bool f32, cf_stream_t stream) {
+    hipStream_t st = as_stream(stream);
+    if (p.H % 8 != 0) return f32 ? launch_gated_norm<true, QMODE, true>(p, st) : launch_gated_norm<false, QMODE, true>(p, st);
+    return f32 ? launch_gated_norm<true, QMODE, false>(p, st) : launch_gated_norm<false, QMODE, false>(p, st);
+}
+
+// what the three forward entry points ask of the arguments they share
+int check_forward(const GatedNormArgs& p, int stream_is_f32) {
+    if (!p.residual || !p.x || !p.post_weight || !p.weight || !p.q || (p.gate && p.gate_rows <= 0) || !std::isfinite(p.res)) return CF_ERR_INVALID_ARG;
+    const unsigned el = stream_is_f32 ? 4 : 2;
+    if (misaligned(p.residual, el) || misaligned(p.sum, el) || misaligned(p.x, 2) || misaligned(p.gate, 2) || misaligned(p.post_weight, 2) ||
+        misaligned(p.weight, 2) || misaligned(p.normed, 2) || misaligned(p.post_rms, 4) || misaligned(p.rms, 4))
+        return CF_ERR_INVALID_ARG;
+    return CF_OK;
+}
+
+GatedNormArgs forward_args(const void* d_residual, const uint16_t* d_x, float residual_scale, const uint16_t* d_gate, int rows_per_gate,
+                           const uint16_t* d_post_scale, const uint16_t* d_scale, int rows, int H, float eps, void* d_sum, uint16_t* d_normed,
+                           float* d_post_rms, float* d_rms, void* d_x8, void* d_sum8, void* d_q) {
+    GatedNormArgs p{};
+    p.residual = d_residual; p.x = d_x; p.res = residual_scale; p.gate = d_gate; p.gate_rows = rows_per_gate; p.post_weight = d_post_scale;
+    p.weight = d_scale; p.rows = rows; p.H = H; p.eps = eps; p.sum = d_sum; p.normed = d_normed; p.post_rms = d_post_rms; p.rms = d_rms;
+    p.x8 = static_cast<uint8_t*>(d_x8); p.sum8 = static_cast<uint8_t*>(d_sum8); p.q = static_cast<uint8_t*>(d_q);
+    p.kept = kept_scale(H);
+    return p;
+}
+
+// Workgroups of the backward pass, as many wavefronts as k_add_norm_grad runs and at least four rows each: see grad_parts() there.
+int gated_parts(int rows, int H) {
+    const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kOneChunkH ? 1 : 2) / kWave;
+    const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;
+    int parts = waves < 8 ? 2048 / waves : 256;
+    parts = parts < turns / 4 ? parts : turns / 4;
+    parts = parts > 256 ? parts : 256;
+    return parts < turns ? parts : turns;
+}
+struct GradPlan {
+    int parts, workers, groups;         // groups: 0 = no gate
+    bool several, segments;             // several groups; some of them in several workers' rows
+    size_t bytes;
+};
+GradPlan grad_plan(int rows, int H, int gate_rows) {
+    GradPlan g{};
+    if (rows == 0 || H == 0) return g;
+    g.parts = gated_parts(rows, H);
+    g.groups = gate_rows > 0 ? (rows - 1) / gate_rows + 1 : 0;
+    g.several = g.groups > 1;
+    g.workers = H <= kOneWaveH ? (4 * g.parts < rows ? 4 * g.parts : rows) : g.parts;
+    g.segments = g.several && !whole_groups(g.groups, g.workers);
+    const size_t shares = 2 * static_cast<size_t>(g.parts) + (g.segments ? 2 * static_cast<size_t>(g.workers) : 0);
+    g.bytes = (shares * H + g.parts) * sizeof(float);
+    return g;
+}
+
+template <bool F32, bool KEPT, bool GROUPS, bool TAIL>
+void launch_gated_grad(const GatedGradArgs& p, int parts, hipStream_t st) {
+    if (p.H <= kOneWaveH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, true, 1><<<parts, 4 * kWave, 0, st>>>(p);
+    else if (p.H <= kOneChunkH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1><<<parts, row_threads(p.H, 1), 0, st>>>(p);
+    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+}
+
+int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, float* d_grad_scale, int accumulate, void* d_workspace,
+               size_t workspace_bytes, cf_stream_t stream) {
+    const int chk = check_shape(p.rows, p.H);
+    if (chk < 0) return chk;
+    if ((p.gate && p.gate_rows <= 0) || !std::isfinite(p.res) || (accumulate & ~(CF_ACCUMULATE_SCALES | CF_ACCUMULATE_GATE))) return CF_ERR_INVALID_ARG;
+    if (p.H == 0) return CF_OK;
+    if (!d_grad_post_scale || !d_grad_scale || misaligned(d_grad_post_scale, 4) || misaligned(d_grad_scale, 4)) return CF_ERR_INVALID_ARG;
+    GatedSumArgs s{};
+    s.dw = d_grad_scale; s.dwp = d_grad_post_scale; s.H = p.H; s.accumulate = accumulate & CF_ACCUMULATE_SCALES;
+    const int blocks = 2 * ceil_div(p.H, kSumColumns);
+    if (p.rows == 0) {              // no rows: their sums are zero, and there is no gate
+        if (s.accumulate) return CF_OK;
+        k_gated_sum<<<blocks, kSumThreads, 0, as_stream(stream)>>>(s);
+        return launch_status();
+    }
+    if (!p.dy || !p.sum || !p.x || !p.post_weight || !p.weight || !p.post_rms || !p.rms || !p.dr || (!p.dx && !p.q) || !d_workspace ||
+        (p.q && (!p.qscale || !p.amax)) || (p.gate && !p.dgate))
+        return CF_ERR_INVALID_ARG;
+    const unsigned el = f32 ? 4 : 2;
+    if (misaligned(p.dy, 2) || (!kept && (misaligned(p.sum, el) || misaligned(p.x, 2))) || misaligned(p.gate, 2) || misaligned(p.post_weight, 2) ||
+        misaligned(p.weight, 2) || misaligned(p.post_rms, 4) || misaligned(p.rms, 4) || misaligned(p.dh, el) || misaligned(p.dr, el) ||
+        misaligned(p.dx, 2) || misaligned(p.dgate, 4) || misaligned(p.qscale, 4) || misaligned(p.amax, 4) || misaligned(d_workspace, 16))
+        return CF_ERR_INVALID_ARG;
+    const GradPlan plan = grad_plan(p.rows, p.H, p.gate ? p.gate_rows : 0);
+    if (workspace_bytes < plan.bytes) return CF_ERR_INVALID_ARG;
+    const size_t share = static_cast<size_t>(plan.parts) * p.H;
+    p.part_w = static_cast<float*>(d_workspace);
+    p.part_p = p.part_w + share;
+    p.segments = p.part_p + share;
+    p.part_amax = p.segments + (plan.segments ? 2 * static_cast<size_t>(plan.workers) * p.H : 0);
+    p.groups = plan.groups;
+    p.workers = plan.workers;
+    p.accumulate_gate = accumulate & CF_ACCUMULATE_GATE;
+    p.kept_inv = 1.0f / kept_scale(p.H);
+    hipStream_t st = as_stream(stream);
+    auto go = [&](auto stream_f32, auto in_8_bits, auto groups) {
+        constexpr bool F32 = decltype(stream_f32)::value, KEPT = decltype(in_8_bits)::value, GROUPS = decltype(groups)::value;
+        if (p.H % 8 != 0) launch_gated_grad<F32, KEPT, GROUPS, true>(p, plan.parts, st);
+        else launch_gated_grad<F32, KEPT, GROUPS, false>(p, plan.parts, st);
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    auto by_groups = [&](auto a, auto b) { plan.several ? go(a, b, yes) : go(a, b, no); };
+    if (f32) kept ? by_groups(yes, yes) : by_groups(yes, no);
+    else kept ? by_groups(no, yes) : by_groups(no, no);
+    s.part_w = p.part_w; s.part_p = p.part_p; s.part_amax = p.part_amax; s.gate = p.gate; s.post_weight = p.post_weight; s.dgate = p.dgate; s.amax = p.amax;
+    s.parts = plan.parts; s.groups = plan.several ? 0 : plan.groups; s.accumulate_gate = p.accumulate_gate;
+    k_gated_sum<<<blocks + (p.q ? 1 : 0), kSumThreads, 0, st>>>(s);
+    if (plan.segments)
+        k_gated_segments<<<static_cast<unsigned>(plan.groups) * ceil_div(p.H, 64), 256, 0, st>>>(p.segments, p.post_weight, p.dgate, p.rows, p.H, p.gate_rows,
+                                                                                              plan.workers, p.accumulate_gate);
+    return launch_status();
+}
+
+GatedGradArgs grad_args(const uint16_t* d_grad_normed, const void* d_sum, const void* d_x, float residual_scale, const uint16_t* d_gate,
+                        int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale, const float* d_post_rms, const float* d_rms,
+                        const void* d_grad_sum, int rows, int H, void* d_grad_residual, uint16_t* d_grad_x, void* d_grad8, const float* d_qscale,
+                        float* d_amax, float* d_grad_gate) {
+    GatedGradArgs p{};
+    p.dy = d_grad_normed; p.sum = d_sum; p.x = d_x; p.res = residual_scale; p.gate = d_gate; p.gate_rows = rows_per_gate; p.post_weight = d_post_scale;
+    p.weight = d_scale; p.post_rms = d_post_rms; p.rms = d_rms; p.dh = d_grad_sum; p.rows = rows; p.H = H; p.dr = d_grad_residual; p.dx = d_grad_x;
+    p.q = static_cast<uint8_t*>(d_grad8); p.qscale = d_qscale; p.amax = d_amax; p.dgate = d_grad_gate;
+    return p;
+}
+
+}  // namespace
+}  // namespace cf
+
+using namespace cf;
+
+extern "C" {
+
+int cf_gated_add_rmsnorm_quantize_rows(const void* d_residual, const uint16_t* d_x, int stream_is_f32, float residual_scale, const uint16_t* d_gate,
+                                       int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale, int rows, int H, float eps,
+                                       int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_post_rms, float* d_rms, void* d_x8, void* d_sum8,
+                                       void* d_q, float* d_row_scale, float* d_row_descale, cf_stream_t stream) {
+    const int chk = check_shape(rows, H);
+    if (chk != 0) return chk < 0 ? chk : CF_OK;
+    GatedNormArgs p = forward_args(d_residual, d_x, residual_scale, d_gate, rows_per_gate, d_post_scale, d_scale, rows, H, eps, d_sum, d_normed,
+                                   d_post_rms, d_rms, d_x8, d_sum8, d_q);
+    if (const int rc = check_forward(p, stream_is_f32)) return rc;
+    if (!d_row_scale || !d_row_descale || misaligned(d_row_scale, 4) || misaligned(d_row_descale, 4)) return CF_ERR_INVALID_ARG;
+    p.scale = d_row_scale; p.descale = d_row_descale; p.e5m2 = is_e5m2 != 0;
+    return gated_norm<Q_ROWS>(p, stream_is_f32 != 0, stream);
+}
+
+int cf_gated_add_rmsnorm_quantize_block_1x128(const void* d_residual, const uint16_t* d_x, int stream_is_f32, float residual_scale,
+                                              const uint16_t* d_gate, int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale,
+                                              int rows, int H, float eps, void* d_sum, uint16_t* d_normed, float* d_post_rms, float* d_rms,
+                                              void* d_x8, void* d_sum8, void* d_q, float* d_group_scale, float* d_group_descale, cf_stream_t stream) {
+    const int chk = check_shape(rows, H);
+    if (chk != 0) return chk < 0 ? chk : CF_OK;
+    GatedNormArgs p = forward_args(d_residual, d_x, residual_scale, d_gate, rows_per_gate, d_post_scale, d_scale, rows, H, eps, d_sum, d_normed,
+                                   d_post_rms, d_rms, d_x8, d_sum8, d_q);
+    if (const int rc = check_forward(p, stream_is_f32)) return rc;
+    if (!d_group_scale || !d_group_descale || misaligned(d_group_scale, 4) || misaligned(d_group_descale, 4)) return CF_ERR_INVALID_ARG;
+    p.scale = d_group_scale; p.descale = d_group_descale;
+    return gated_norm<Q_BLOCK>(p, stream_is_f32 != 0, stream);
+}
+
+int cf_gated_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, int stream_is_f32, float residual_scale, const uint16_t* d_gate,
+                                         int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale, int rows, int H, float eps,
+                                         int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_post_rms, float* d_rms, void* d_x8, void* d_sum8,
+                                         void* d_q, const float* d_qscale, float* d_amax, cf_stream_t stream) {
+    const int chk = check_shape(rows, H);
+    if (chk != 0) return chk < 0 ? chk : CF_OK;
+    GatedNormArgs p = forward_args(d_residual, d_x, residual_scale, d_gate, rows_per_gate, d_post_scale, d_scale, rows, H, eps, d_sum, d_normed,
+                                   d_post_rms, d_rms, d_x8, d_sum8, d_q);
+    if (const int rc = check_forward(p, stream_is_f32)) return rc;
+    if (!d_qscale || !d_amax || misaligned(d_qscale, 4) || misaligned(d_amax, 4)) return CF_ERR_INVALID_ARG;
+    p.qscale = d_qscale; p.amax = d_amax; p.e5m2 = is_e5m2 != 0;
+    return gated_norm<Q_RECORD>(p, stream_is_f32 != 0, stream);
+}
+
+int cf_gated_add_rmsnorm_backward_workspace_bytes(int rows, int H, int rows_per_gate, size_t* bytes) {
+    if (rows < 0 || H < 0 || rows_per_gate < 0 || !bytes) return CF_ERR_INVALID_ARG;
+    if (H > kMaxH) return CF_ERR_UNSUPPORTED;
+    *bytes = grad_plan(rows, H, rows_per_gate).bytes;
+    return CF_OK;
+}
+
+int cf_gated_add_rmsnorm_backward(const uint16_t* d_grad_normed, const void* d_sum, const uint16_t* d_x, int stream_is_f32, float residual_scale,
+                                  const uint16_t* d_gate, int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale,
+                                  const float* d_post_rms, const float* d_rms, const void* d_grad_sum, int rows, int H, void* d_grad_residual,
+                                  uint16_t* d_grad_x, void* d_grad8, const float* d_qscale, float* d_amax, float* d_grad_post_scale,
+                                  float* d_grad_scale, float* d_grad_gate, int accumulate, void* d_workspace, size_t workspace_bytes,
+                                  cf_stream_t stream) {
+    return gated_grad(grad_args(d_grad_normed, d_sum, d_x, residual_scale, d_gate, rows_per_gate, d_post_scale, d_scale, d_post_rms, d_rms, d_grad_sum,
+                                rows, H, d_grad_residual, d_grad_x, d_grad8, d_qscale, d_amax, d_grad_gate),
+                      false, stream_is_f32, d_grad_post_scale, d_grad_scale, accumulate, d_workspace, workspace_bytes, stream);
+}
+
+int cf_gated_add_rmsnorm_backward_ckpt8(const uint16_t* d_grad_normed, const void* d_sum8, const void* d_x8, int stream_is_f32, float residual_scale,
+                                        const uint16_t* d_gate, int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale,
+                                        const float* d_post_rms, const float* d_rms, const void* d_grad_sum, int rows, int H, void* d_grad_residual,
+                                        uint16_t* d_grad_x, void* d_grad8, const float* d_qscale, float* d_amax, float* d_grad_post_scale,
+                                        float* d_grad_scale, float* d_grad_gate, int accumulate, void* d_workspace, size_t workspace_bytes,
+                                        cf_stream_t stream) {
+    return gated_grad(grad_args(d_grad_normed, d_sum8, d_x8, residual_scale, d_gate, rows_per_gate, d_post_scale, d_scale, d_post_rms, d_rms, d_grad_sum,
+                                rows, H, d_grad_residual, d_grad_x, d_grad8, d_qscale, d_amax, d_grad_gate),
+                      true, stream_is_f32, d_grad_post_scale, d_grad_scale, accumulate, d_workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

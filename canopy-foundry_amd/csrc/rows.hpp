@@ -111,8 +111,8 @@ __device__ __forceinline__ void store8_stream(void* p, size_t at, int n, const f
         }
     }
 }
-template <bool TAIL>
-__device__ __forceinline__ void store8_fp8(uint8_t* p, size_t at, int n, bool e5m2, bool finite, const float (&v)[8]) {
+// Eight values as bytes; finite: there is no NaN among them.
+__device__ __forceinline__ u32x2_any pack8_fp8(bool e5m2, bool finite, const float (&v)[8]) {
     u32x2_any o;
     if (finite) {
         o.x = e5m2 ? cvt4_fp8_finite<true>(v[0], v[1], v[2], v[3]) : cvt4_fp8_finite<false>(v[0], v[1], v[2], v[3]);
@@ -121,6 +121,10 @@ __device__ __forceinline__ void store8_fp8(uint8_t* p, size_t at, int n, bool e5
         o.x = e5m2 ? cvt4_fp8<true>(v[0], v[1], v[2], v[3]) : cvt4_fp8<false>(v[0], v[1], v[2], v[3]);
         o.y = e5m2 ? cvt4_fp8<true>(v[4], v[5], v[6], v[7]) : cvt4_fp8<false>(v[4], v[5], v[6], v[7]);
     }
+    return o;
+}
+template <bool TAIL>
+__device__ __forceinline__ void store8_bytes(uint8_t* p, size_t at, int n, u32x2_any o) {
     if (!TAIL || n >= 8) {
         __builtin_nontemporal_store(o, reinterpret_cast<u32x2_any*>(p + at));
     } else {
@@ -140,6 +144,32 @@ __device__ __forceinline__ void store8_fp8(uint8_t* p, size_t at, int n, bool e5
         }
         if (n & 1) *q = static_cast<uint8_t>(rest);
     }
+}
+template <bool TAIL>
+__device__ __forceinline__ void store8_fp8(uint8_t* p, size_t at, int n, bool e5m2, bool finite, const float (&v)[8]) {
+    store8_bytes<TAIL>(p, at, n, pack8_fp8(e5m2, finite, v));
+}
+// Eight E4M3 bytes as the values they stand for times `scale`.
+__device__ __forceinline__ void unpack8_e4m3(const u32x2_any& v, float scale, float (&o)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(v[i]), false);
+        const f32x2_t b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(v[i]), true);
+        o[4 * i] = a.x * scale;
+        o[4 * i + 1] = a.y * scale;
+        o[4 * i + 2] = b.x * scale;
+        o[4 * i + 3] = b.y * scale;
+    }
+}
+// Eight bytes, n of them where neither that many follow nor the chunk is whole.
+template <bool TAIL>
+__device__ __forceinline__ u32x2_any load8_bytes(const uint8_t* p, size_t at, int n, bool whole) {
+    if (!TAIL || n >= 8 || whole) return *reinterpret_cast<const u32x2_any*>(p + at);
+    u32x2_any v = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) v[i >> 2] |= static_cast<uint32_t>(p[at + i]) << (8 * (i & 3));
+    return v;
 }
 
 // What a value is after the lanes of a group of 16 have exchanged it, by DPP: quad, half row, row.

@@ -258,6 +258,99 @@ int cf_add_rmsnorm_backward_quant_e5m2(const uint16_t* d_grad_normed, const void
                                        float* d_grad_scale, int accumulate, void* d_grad8, const float* d_qscale, float* d_amax,
                                        void* d_workspace, size_t workspace_bytes, cf_stream_t stream);
 
+/* ---- a layer with a norm on both sides of its block ------------------------------------------------------------------
+ * The block's output x is normed, goes through a gate and joins the residual stream, which is scaled; the next norm and its 8-bit output follow in
+ * the same pass.  No counterpart in the reference's kernel library, whose layers norm the block's input alone (src/trainer.cu:6281-6304).
+ *     px = sqrt(mean(x^2) + eps),  xh = x / px,   h = T(residual_scale * r + gate * (xh * post_scale))       T: the stream's type, bf16 or fp32
+ *     p = sqrt(mean(h^2) + eps),   hh = h / p,    y = hh * scale                                           of h as it is stored, y in fp32
+ * d_gate [ceil(rows / rows_per_gate), H] bf16: row i uses gate row i / rows_per_gate (one gate for all rows, one for each sequence, one for each token); null = no
+ * gate, rows_per_gate is not looked at then.  d_post_scale and d_scale are [H] bf16.  d_sum (h; may be d_residual), d_normed (bf16(y); may be d_x), d_post_rms (px)
+ * and d_rms (p) may be null.
+ * For the backward pass the caller keeps h and x, or in their place the normalised rows in 8 bits: d_x8 = e4m3(xh * S), d_sum8 = e4m3(hh * S) [rows, H], null = not
+ * wanted, with S the largest power of two with S * sqrt(H) <= 448, which no element of a normalised row can leave; S depends on H alone.  They round at
+ * 2^-4 of the element or at 2^-10 / S, whichever is more; a NaN is NaN.  d_x8 and d_sum8 overlap no other argument.
+ * q and its scales, alignments, magnitudes, NaNs, eps and H <= 16384: as cf_add_rmsnorm_quantize_*.  residual_scale is finite, else CF_ERR_INVALID_ARG. */
+
+/* Per-row scales (no counterpart, as above; the scale's formula is that of kernels/fp8.cu:37-39,49). */
+int cf_gated_add_rmsnorm_quantize_rows(const void* d_residual, const uint16_t* d_x, int stream_is_f32, float residual_scale, const uint16_t* d_gate,
+                                       int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale, int rows, int H, float eps,
+                                       int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_post_rms, float* d_rms, void* d_x8, void* d_sum8,
+                                       void* d_q, float* d_row_scale, float* d_row_descale, cf_stream_t stream);
+/* E4M3 with a scale for each 128 elements of a row, [rows, ceil(H/128)] (no counterpart, as above). */
+int cf_gated_add_rmsnorm_quantize_block_1x128(const void* d_residual, const uint16_t* d_x, int stream_is_f32, float residual_scale,
+                                              const uint16_t* d_gate, int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale,
+                                              int rows, int H, float eps, void* d_sum, uint16_t* d_normed, float* d_post_rms, float* d_rms,
+                                              void* d_x8, void* d_sum8, void* d_q, float* d_group_scale, float* d_group_descale, cf_stream_t stream);
+/* Delayed scaling: quantize with *d_qscale and raise *d_amax to max|y| (the caller zeroes it) (no counterpart, as above). */
+int cf_gated_add_rmsnorm_quantize_record(const void* d_residual, const uint16_t* d_x, int stream_is_f32, float residual_scale, const uint16_t* d_gate,
+                                         int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale, int rows, int H, float eps,
+                                         int is_e5m2, void* d_sum, uint16_t* d_normed, float* d_post_rms, float* d_rms, void* d_x8, void* d_sum8,
+                                         void* d_q, const float* d_qscale, float* d_amax, cf_stream_t stream);
+
+/* The gradient of the three (the quantize counts as the identity); no counterpart, as above.  With dy = d_grad_normed [rows, H] bf16 and dh = d_grad_sum
+ * [rows, H] (what reaches h past the norm; null = nothing):
+ *     g = dy * scale,  D = dh + (g - hh * mean(g * hh)) / p,  d_grad_residual = T(residual_scale * D)
+ *     e = D * gate * post_scale,  dx = (e - xh * mean(e * xh)) / px:  d_grad_x = bf16(dx), d_grad8 = e5m2(dx * *d_qscale) with *d_amax raised to max|dx| (the
+ *     caller zeroes it), either null where the other is wanted alone
+ *     d_grad_scale [H] = sum over rows of dy * hh,  P = sum over a gate's rows of D * xh,  d_grad_gate like d_gate but fp32 = post_scale * P (not looked at
+ *     without a gate),  d_grad_post_scale [H] = sum over the gates of gate * P
+ * The first form takes h and x as the forward pass left them, the second the checkpoints in 8 bits, from which hh = d_sum8 / S and xh = d_x8 / S; both the rms
+ * (from 2^-126 to 2^126).  accumulate: CF_ACCUMULATE_SCALES adds to d_grad_scale and d_grad_post_scale, CF_ACCUMULATE_GATE to d_grad_gate.  The sums over rows are taken
+ * in 64 bits, but for one rounding to fp32 for each share of the rows, in an order that follows from rows, H and rows_per_gate alone.  d_grad_residual may
+ * be d_grad_sum; no other output overlaps an argument.  rows = 0 leaves zeros in the two scales' gradients unless they accumulate.  d_workspace: 16-byte aligned,
+ * cf_gated_add_rmsnorm_backward_workspace_bytes() bytes (rows_per_gate = 0: no gate); it belongs to the call. */
+#define CF_ACCUMULATE_SCALES 1
+#define CF_ACCUMULATE_GATE   2
+int cf_gated_add_rmsnorm_backward_workspace_bytes(int rows, int H, int rows_per_gate, size_t* bytes);
+int cf_gated_add_rmsnorm_backward(const uint16_t* d_grad_normed, const void* d_sum, const uint16_t* d_x, int stream_is_f32, float residual_scale,
+                                  const uint16_t* d_gate, int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale,
+                                  const float* d_post_rms, const float* d_rms, const void* d_grad_sum, int rows, int H, void* d_grad_residual,
+                                  uint16_t* d_grad_x, void* d_grad8, const float* d_qscale, float* d_amax, float* d_grad_post_scale,
+                                  float* d_grad_scale, float* d_grad_gate, int accumulate, void* d_workspace, size_t workspace_bytes,
+                                  cf_stream_t stream);
+int cf_gated_add_rmsnorm_backward_ckpt8(const uint16_t* d_grad_normed, const void* d_sum8, const void* d_x8, int stream_is_f32, float residual_scale,
+                                        const uint16_t* d_gate, int rows_per_gate, const uint16_t* d_post_scale, const uint16_t* d_scale,
+                                        const float* d_post_rms, const float* d_rms, const void* d_grad_sum, int rows, int H, void* d_grad_residual,
+                                        uint16_t* d_grad_x, void* d_grad8, const float* d_qscale, float* d_amax, float* d_grad_post_scale,
+                                        float* d_grad_scale, float* d_grad_gate, int accumulate, void* d_workspace, size_t workspace_bytes,
+                                        cf_stream_t stream);
+
+/* ---- the gated activation, kept in 8 bits ------------------------------------------------------------------------------
+ * SwiGLU (kernels/activations.cu:26-40) with the 8-bit operand of the product behind it, in one pass that also leaves what the backward pass needs: gate and up as E4M3
+ * with a descale for each 128 elements of a row (448 / amax and its inverse, kernels/fp8.cu:37-39,49), 2 + 1/16 bytes an element in place of 4.  No counterpart
+ * in the reference, which keeps both in bf16.
+ *     a = gate * sigmoid(gate) * up in fp32,   q = f8(a * its scale)
+ * d_gate and d_up: bf16, rows ld elements apart (ld >= I: the halves of one product's output have ld = 2 I).  d_gate8, d_up8, d_q: [rows, I]; the descales
+ * [rows, ceil(I/128)].  A maximum leaves NaNs out; a NaN is NaN in the output; a group that holds an infinity decodes to NaN, and so does a row of the operand.
+ * Any alignment that the elements have.  Outputs overlap no argument.  I below 2^30. */
+
+/* Per-row scales; I <= 32768, else CF_ERR_UNSUPPORTED (no counterpart, as above). */
+int cf_swiglu_ckpt8_quantize_rows(const uint16_t* d_gate, const uint16_t* d_up, int ld, int rows, int I, int is_e5m2, void* d_gate8,
+                                  float* d_gate8_descale, void* d_up8, float* d_up8_descale, void* d_q, float* d_row_scale, float* d_row_descale,
+                                  cf_stream_t stream);
+/* E4M3 with a scale for each 128 elements of a row, [rows, ceil(I/128)] (no counterpart, as above). */
+int cf_swiglu_ckpt8_quantize_block_1x128(const uint16_t* d_gate, const uint16_t* d_up, int ld, int rows, int I, void* d_gate8,
+                                         float* d_gate8_descale, void* d_up8, float* d_up8_descale, void* d_q, float* d_group_scale,
+                                         float* d_group_descale, cf_stream_t stream);
+/* Delayed scaling: quantize with *d_qscale and raise *d_amax to max|a| (the caller zeroes it) (no counterpart, as above). */
+int cf_swiglu_ckpt8_quantize_record(const uint16_t* d_gate, const uint16_t* d_up, int ld, int rows, int I, int is_e5m2, void* d_gate8,
+                                    float* d_gate8_descale, void* d_up8, float* d_up8_descale, void* d_q, const float* d_qscale, float* d_amax,
+                                    cf_stream_t stream);
+
+/* Its gradient from those bytes (kernels/activations.cu:42-58 is the bf16 form); with dO = d_grad_out [rows, I] bf16, g and u what the bytes stand for, s = sigmoid(g):
+ *     d_grad_gate = dO * u * s * (1 + g * (1 - s)),   d_grad_up = dO * g * s,   d_act = g * s * u
+ * as bf16, the gradients ld elements a row (ld >= I), d_act [rows, I] or null (what the weight gradient of the product behind takes). */
+int cf_swiglu_ckpt8_backward(const uint16_t* d_grad_out, const void* d_gate8, const float* d_gate8_descale, const void* d_up8,
+                             const float* d_up8_descale, int rows, int I, uint16_t* d_grad_gate, uint16_t* d_grad_up, int ld, uint16_t* d_act,
+                             cf_stream_t stream);
+/* The same as the operands of the FP8 products that follow (no counterpart: the reference quantizes and transposes in launches of their own, kernels/fp8.cu:86-103,
+ * src/trainer.cu:1441-1448): d_grad8 [rows, 2 I] E5M2 = the gradients of gate and of up side by side * *d_qscale, *d_amax raised to their maximum (the caller
+ * zeroes it); d_grad8_t [2 I, rows] the same bytes transposed; d_act8_t [I, rows] E4M3 = the activation * *d_act_qscale, transposed: the operands of
+ * cf_fp8_gemm_nt_bf16_ex (E5M2 rows) and cf_fp8_gemm_tn_accum_f32.  The transposed ones may be null (weights that do not learn). */
+int cf_swiglu_ckpt8_backward_quant_e5m2(const uint16_t* d_grad_out, const void* d_gate8, const float* d_gate8_descale, const void* d_up8,
+                                        const float* d_up8_descale, int rows, int I, void* d_grad8, void* d_grad8_t, const float* d_qscale,
+                                        float* d_amax, void* d_act8_t, const float* d_act_qscale, cf_stream_t stream);
+
 /* ---- global norm of a list of gradients, and clipping by it: no counterpart in the reference's kernel library ------
  *     norm = sqrt(sum over all elements of all tensors of g^2),  coef = norm > max_norm ? max_norm / norm : 1,  out = T(g * coef)
  * The sum is taken in 64 bits, in an order that follows from the list alone.  A norm that is not finite (in fp32) is returned as it is and
