@@ -200,6 +200,7 @@ struct GatedGradArgs {
     float* part_p;                // [parts, H] shares of P (GROUPS: of dwp)
     float* part_amax;             // [parts]
     float* segments;              // GROUPS: [workers, 2, H] shares of P of the groups that several workers have
+    double* far_dwp;              // GROUPS, four chunks a thread: [parts, 32, threads], where neither registers nor LDS have room for it
     int rows, H, gate_rows, groups, workers;
     float res, kept_inv;
 };
@@ -208,6 +209,15 @@ struct GatedGradArgs {
 template <bool F32, bool KEPT>
 struct Saved8 {
     std::conditional_t<KEPT, u32x2_any, Raw8<F32>> v;
+    // what follows is made of the elements as they were loaded, not of values kept from before
+    __device__ __forceinline__ void hold() {
+        if constexpr (KEPT) {
+            asm volatile("" : "+v"(v));
+        } else {
+            asm volatile("" : "+v"(v.v[0]));
+            if constexpr (F32) asm volatile("" : "+v"(v.v[F32 ? 1 : 0]));
+        }
+    }
     template <bool TAIL>
     __device__ __forceinline__ void load(const void* p, size_t at, int n, bool whole) {
         if constexpr (!KEPT) {
@@ -257,13 +267,18 @@ __device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const flo
     }
 }
 
+constexpr int kGradThreads = 512;       // of a row at most: 256 registers each
 // A worker (a workgroup; ONE_WAVE: a wavefront) holds a row as k_gated_norm does and loads the next row's operands before it works on one.  Its shares of
 // the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
 // workers take turns at the rows; GROUPS: each has rows next to each other, and leaves P at a group's end: dgate itself where it had the whole group.
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const GatedGradArgs p) {
+__global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_grad(const GatedGradArgs p) {
+    constexpr bool IN_LDS = V == 4;     // dw: 128 KB
+    constexpr bool TIGHT = V > 1;
     __shared__ float sh[2][16];         // each is written again only behind the other one's barrier
     __shared__ double sh_sum[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
+    __shared__ double sh_dw[IN_LDS ? V * 8 * kGradThreads : 1];
+    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !IN_LDS ? V * 8 * kGradThreads : 1];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
     const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
@@ -309,21 +324,30 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const
             }
         }
     };
-    u32x4_any w[V], wp[V], one_gate[V];
-    double dw[V][8], ps[V][8], dwp[GROUPS ? V : 1][8];
+    u32x4_any w[V], wp[V], one_gate[GROUPS ? 1 : V];
+    double dw[IN_LDS ? 1 : V][8], ps[V][8], dwp[GROUPS && ONE_WAVE ? V : 1][8];
+    // dwp, which changes at a group's end only
+    auto dwp_at = [&](int j, int i) -> double& {
+        if constexpr (ONE_WAVE) return dwp[j][i];
+        else if constexpr (IN_LDS) return p.far_dwp[(static_cast<size_t>(blockIdx.x) * V * 8 + j * 8 + i) * T + t];
+        else return sh_dwp[(j * 8 + i) * T + t];
+    };
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         w[j] = wp[j] = u32x4_any{0, 0, 0, 0};
-        one_gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        if constexpr (!GROUPS) one_gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
         if (has(j)) {
             w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
             wp[j] = load_weight<TAIL>(p.post_weight, (t + j * T) * 8, left(j), H);
-            if (!GROUPS && p.gate) one_gate[j] = load_weight<TAIL>(p.gate, (t + j * T) * 8, left(j), H);
+            if constexpr (!GROUPS)
+                if (p.gate) one_gate[j] = load_weight<TAIL>(p.gate, (t + j * T) * 8, left(j), H);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            dw[j][i] = ps[j][i] = 0.0;
-            if constexpr (GROUPS) dwp[j][i] = 0.0;
+            ps[j][i] = 0.0;
+            if constexpr (IN_LDS) sh_dw[(j * 8 + i) * T + t] = 0.0;
+            else dw[j][i] = 0.0;
+            if constexpr (GROUPS) dwp_at(j, i) = 0.0;
         }
     }
     const float s = p.q ? *p.qscale : 0.0f;
@@ -346,44 +370,62 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const
         }
         const size_t base = static_cast<size_t>(row) * H;
         const float inv = 1.0f / r.rms, post_inv = 1.0f / r.post_rms;
-        float d[V][8], xh[V][8];
+        if constexpr (TIGHT) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) asm volatile("" : "+v"(w[j]), "+v"(wp[j]));        // kept as pairs, not as fp32 from row to row
+        }
+        const float hh_scale = KEPT ? p.kept_inv : inv, xh_scale = KEPT ? p.kept_inv : post_inv;
         float dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            r.h[j].template values<TAIL>(d[j], left(j), KEPT ? p.kept_inv : inv);       // hh for now
-            r.x[j].template values<TAIL>(xh[j], left(j), KEPT ? p.kept_inv : post_inv);
+            float hh[8];
+            r.h[j].template values<TAIL>(hh, left(j), hh_scale);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dy = value8<false, TAIL>(r.dy[j], i, left(j));
-                dw[j][i] += static_cast<double>(dy * d[j][i]);
-                dot = __builtin_fmaf(dy * pair_at(w[j], i), d[j][i], dot);
+                if constexpr (IN_LDS) sh_dw[(j * 8 + i) * T + t] += static_cast<double>(dy * hh[i]);
+                else dw[j][i] += static_cast<double>(dy * hh[i]);
+                if constexpr (TIGHT && !IN_LDS) asm volatile("" : "+v"(dw[j][i]));         // added here, not at the row's end, to which its terms would be kept
+                dot = __builtin_fmaf(dy * pair_at(w[j], i), hh[i], dot);
             }
         }
         const float c = row_sum<ONE_WAVE>(dot, sh[0]) / static_cast<float>(H);
         dot = 0.0f;
+        float e[V][8];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const u32x4_any gate = GROUPS ? r.gate[GROUPS ? j : 0] : one_gate[j];
-            float o[8];
+            if constexpr (TIGHT) {
+                r.h[j].hold();
+                r.x[j].hold();
+            }
+            u32x4_any gate;
+            if constexpr (GROUPS) gate = r.gate[j];
+            else gate = one_gate[j];
+            float hh[8], xh[8], o[8];
+            r.h[j].template values<TAIL>(hh, left(j), hh_scale);
+            r.x[j].template values<TAIL>(xh, left(j), xh_scale);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float g = value8<false, TAIL>(r.dy[j], i, left(j)) * pair_at(w[j], i);
-                const float v = __builtin_fmaf(__builtin_fmaf(-d[j][i], c, g), inv, value8<F32, TAIL>(r.dh[j], i, left(j)));
+                const float v = __builtin_fmaf(__builtin_fmaf(-hh[i], c, g), inv, value8<F32, TAIL>(r.dh[j], i, left(j)));
                 o[i] = v * p.res;
-                ps[j][i] += static_cast<double>(v * xh[j][i]);
-                d[j][i] = v * (pair_at(gate, i) * pair_at(wp[j], i));                   // e from here on
-                dot = __builtin_fmaf(d[j][i], xh[j][i], dot);
+                ps[j][i] += static_cast<double>(v * xh[i]);
+                if constexpr (TIGHT) asm volatile("" : "+v"(ps[j][i]));
+                e[j][i] = v * (pair_at(gate, i) * pair_at(wp[j], i));
+                dot = __builtin_fmaf(e[j][i], xh[i], dot);
             }
             if (has(j)) store8_stream<F32, TAIL, false>(p.dr, base + (t + j * T) * 8, left(j), o);
         }
         const float post_c = row_sum<ONE_WAVE>(dot, sh[1]) / static_cast<float>(H);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            float o[8];
+            if constexpr (TIGHT) r.x[j].hold();
+            float xh[8], o[8];
+            r.x[j].template values<TAIL>(xh, left(j), xh_scale);
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                o[i] = __builtin_fmaf(-xh[j][i], post_c, d[j][i]) * post_inv;
+                o[i] = __builtin_fmaf(-xh[i], post_c, e[j][i]) * post_inv;
                 amax = fmaxf(amax, fabsf(o[i]));
                 top = max(top, abs_bits(o[i]));
             }
@@ -403,7 +445,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const
                 for (int j = 0; j < V; ++j) {
                     float o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dwp[j][i] += ps[j][i] * static_cast<double>(pair_at(r.gate[j], i));
+                    for (int i = 0; i < 8; ++i) dwp_at(j, i) += ps[j][i] * static_cast<double>(pair_at(r.gate[j], i));
                     if (has(j)) {
                         const int at = (t + j * T) * 8;
                         if (whole) {
@@ -430,14 +472,14 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const
         }
     }
     // the workgroup's shares
-    auto leave = [&](const double (&v)[V][8], float* to) {
+    auto leave = [&](auto at, float* to) {
         float* part = to + static_cast<size_t>(blockIdx.x) * H;
         if constexpr (ONE_WAVE) {
             static_assert(V == 1);
             const int wave = threadIdx.x >> 6;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sh_sum[wave][t * 8 + i] = v[0][i];
+            for (int i = 0; i < 8; ++i) sh_sum[wave][t * 8 + i] = at(0, i);
             __syncthreads();
             for (int i = threadIdx.x; i < H; i += 256) part[i] = static_cast<float>((sh_sum[0][i] + sh_sum[1][i]) + (sh_sum[2][i] + sh_sum[3][i]));
         } else {
@@ -446,14 +488,19 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm_grad(const
                 if (has(j)) {
                     float o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = static_cast<float>(v[j][i]);
+                    for (int i = 0; i < 8; ++i) o[i] = static_cast<float>(at(j, i));
                     store8_f32<TAIL>(part, (t + j * T) * 8, left(j), o);
                 }
         }
     };
-    leave(dw, p.part_w);
-    if constexpr (GROUPS) leave(dwp, p.part_p);
-    else leave(ps, p.part_p);
+    leave([&](int j, int i) {
+        if constexpr (IN_LDS) return sh_dw[(j * 8 + i) * T + t];
+        else return dw[j][i];
+    }, p.part_w);
+    leave([&](int j, int i) {
+        if constexpr (GROUPS) return dwp_at(j, i);
+        else return ps[j][i];
+    }, p.part_p);
     if (p.q) {
         __syncthreads();
         const uint32_t m = row_max<false>(__float_as_uint(amax), reinterpret_cast<uint32_t*>(sh[0]));
@@ -576,9 +623,11 @@ GatedNormArgs forward_args(const void* d_residual, const uint16_t* d_x, float re
     return p;
 }
 
+// chunks of a row that a thread has in the backward pass
+constexpr int grad_chunks(int H) { return H <= 8 * kGradThreads ? 1 : H <= 16 * kGradThreads ? 2 : 4; }
 // Workgroups of the backward pass, as many wavefronts as k_add_norm_grad runs and at least four rows each: see grad_parts() there.
 int gated_parts(int rows, int H) {
-    const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kOneChunkH ? 1 : 2) / kWave;
+    const int waves = H <= kOneWaveH ? 4 : row_threads(H, grad_chunks(H)) / kWave;
     const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;
     int parts = waves < 8 ? 2048 / waves : 256;
     parts = parts < turns / 4 ? parts : turns / 4;
@@ -588,7 +637,7 @@ int gated_parts(int rows, int H) {
 struct GradPlan {
     int parts, workers, groups;         // groups: 0 = no gate
     bool several, segments;             // several groups; some of them in several workers' rows
-    size_t bytes;
+    size_t far, bytes;
 };
 GradPlan grad_plan(int rows, int H, int gate_rows) {
     GradPlan g{};
@@ -599,15 +648,17 @@ GradPlan grad_plan(int rows, int H, int gate_rows) {
     g.workers = H <= kOneWaveH ? (4 * g.parts < rows ? 4 * g.parts : rows) : g.parts;
     g.segments = g.several && !whole_groups(g.groups, g.workers);
     const size_t shares = 2 * static_cast<size_t>(g.parts) + (g.segments ? 2 * static_cast<size_t>(g.workers) : 0);
-    g.bytes = (shares * H + g.parts) * sizeof(float);
+    g.far = g.several && grad_chunks(H) == 4 ? static_cast<size_t>(g.parts) * 4 * 8 * row_threads(H, 4) * sizeof(double) : 0;
+    g.bytes = g.far + (shares * H + g.parts) * sizeof(float);
     return g;
 }
 
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL>
 void launch_gated_grad(const GatedGradArgs& p, int parts, hipStream_t st) {
     if (p.H <= kOneWaveH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, true, 1><<<parts, 4 * kWave, 0, st>>>(p);
-    else if (p.H <= kOneChunkH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1><<<parts, row_threads(p.H, 1), 0, st>>>(p);
-    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+    else if (grad_chunks(p.H) == 1) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1><<<parts, row_threads(p.H, 1), 0, st>>>(p);
+    else if (grad_chunks(p.H) == 2) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 4><<<parts, row_threads(p.H, 4), 0, st>>>(p);
 }
 
 int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, float* d_grad_scale, int accumulate, void* d_workspace,
@@ -636,7 +687,8 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     const GradPlan plan = grad_plan(p.rows, p.H, p.gate ? p.gate_rows : 0);
     if (workspace_bytes < plan.bytes) return CF_ERR_INVALID_ARG;
     const size_t share = static_cast<size_t>(plan.parts) * p.H;
-    p.part_w = static_cast<float*>(d_workspace);
+    p.far_dwp = static_cast<double*>(d_workspace);
+    p.part_w = reinterpret_cast<float*>(static_cast<char*>(d_workspace) + plan.far);
     p.part_p = p.part_w + share;
     p.segments = p.part_p + share;
     p.part_amax = p.segments + (plan.segments ? 2 * static_cast<size_t>(plan.workers) * p.H : 0);
