@@ -273,12 +273,13 @@ constexpr int kGradThreads = 512;       // of a row at most: 256 registers each
 // workers take turns at the rows; GROUPS: each has rows next to each other, and leaves P at a group's end: dgate itself where it had the whole group.
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_grad(const GatedGradArgs p) {
-    constexpr bool IN_LDS = V == 4;     // dw: 128 KB
+    constexpr bool IN_LDS = V > 1;      // dw: 64 or 128 KB
+    constexpr bool FAR = V == 4;
     constexpr bool TIGHT = V > 1;
     __shared__ float sh[2][16];         // each is written again only behind the other one's barrier
     __shared__ double sh_sum[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
     __shared__ double sh_dw[IN_LDS ? V * 8 * kGradThreads : 1];
-    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !IN_LDS ? V * 8 * kGradThreads : 1];
+    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !FAR ? V * 8 * kGradThreads : 1];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
     const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
@@ -300,13 +301,11 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         Saved8<F32, KEPT> h[V];
         Saved8<false, KEPT> x[V];
         Raw8<F32> dh[V];
-        u32x4_any gate[GROUPS ? V : 1];
         float rms, post_rms;
     };
     auto load = [&](Row& r, unsigned row) {
         const size_t base = static_cast<size_t>(row) * H;
         const bool follows = static_cast<size_t>(rows - 1 - row) * H >= 7;
-        const uint16_t* gates = GROUPS ? p.gate + static_cast<size_t>(row / static_cast<unsigned>(p.gate_rows)) * H : nullptr;
         r.rms = p.rms[row];
         r.post_rms = p.post_rms[row];
 #pragma unroll
@@ -316,31 +315,29 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
             clear8(r.dh[j]);
             r.h[j].template load<TAIL>(p.sum, base + at, n, follows);
             r.x[j].template load<TAIL>(p.x, base + at, n, follows);
-            if constexpr (GROUPS) r.gate[j] = u32x4_any{0, 0, 0, 0};
             if (n > 0) {
                 load8<false, TAIL>(p.dy, base + at, n, follows, r.dy[j]);
                 if (p.dh) load8<F32, TAIL>(p.dh, base + at, n, follows, r.dh[j]);
-                if constexpr (GROUPS) r.gate[j] = load_weight<TAIL>(gates, at, n, H);
             }
         }
     };
-    u32x4_any w[V], wp[V], one_gate[GROUPS ? 1 : V];
+    u32x4_any w[V], wp[V], gate[V];         // GROUPS: the gate is loaded where its rows begin
     double dw[IN_LDS ? 1 : V][8], ps[V][8], dwp[GROUPS && ONE_WAVE ? V : 1][8];
     // dwp, which changes at a group's end only
     auto dwp_at = [&](int j, int i) -> double& {
         if constexpr (ONE_WAVE) return dwp[j][i];
-        else if constexpr (IN_LDS) return p.far_dwp[(static_cast<size_t>(blockIdx.x) * V * 8 + j * 8 + i) * T + t];
+        else if constexpr (FAR) return p.far_dwp[(static_cast<size_t>(blockIdx.x) * V * 8 + j * 8 + i) * T + t];
         else return sh_dwp[(j * 8 + i) * T + t];
     };
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         w[j] = wp[j] = u32x4_any{0, 0, 0, 0};
-        if constexpr (!GROUPS) one_gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
         if (has(j)) {
             w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
             wp[j] = load_weight<TAIL>(p.post_weight, (t + j * T) * 8, left(j), H);
             if constexpr (!GROUPS)
-                if (p.gate) one_gate[j] = load_weight<TAIL>(p.gate, (t + j * T) * 8, left(j), H);
+                if (p.gate) gate[j] = load_weight<TAIL>(p.gate, (t + j * T) * 8, left(j), H);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -358,7 +355,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         group = first / static_cast<unsigned>(p.gate_rows);
         group_first = group * p.gate_rows;
     }
-    constexpr bool AHEAD = V == 1;          // 1024 threads have 128 registers each, too few for two rows of two chunks
+    constexpr bool AHEAD = V <= 2;          // four chunks leave no registers for a second row
     Row r, next;
     if (AHEAD && first < end) load(next, first);
     for (unsigned row = first; row < end; row += step) {
@@ -368,11 +365,18 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         } else {
             load(r, row);
         }
+        if constexpr (GROUPS) {
+            if (row == first || row == group_first) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (has(j)) gate[j] = load_weight<TAIL>(p.gate + static_cast<size_t>(group) * H, (t + j * T) * 8, left(j), H);
+            }
+        }
         const size_t base = static_cast<size_t>(row) * H;
         const float inv = 1.0f / r.rms, post_inv = 1.0f / r.post_rms;
         if constexpr (TIGHT) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) asm volatile("" : "+v"(w[j]), "+v"(wp[j]));        // kept as pairs, not as fp32 from row to row
+            for (int j = 0; j < V; ++j) asm volatile("" : "+v"(w[j]), "+v"(wp[j]), "+v"(gate[j]));        // kept as pairs, not as fp32 from row to row
         }
         const float hh_scale = KEPT ? p.kept_inv : inv, xh_scale = KEPT ? p.kept_inv : post_inv;
         float dot = 0.0f;
@@ -383,7 +387,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dy = value8<false, TAIL>(r.dy[j], i, left(j));
-                if constexpr (IN_LDS) sh_dw[(j * 8 + i) * T + t] += static_cast<double>(dy * hh[i]);
+                if constexpr (IN_LDS) unsafeAtomicAdd(&sh_dw[(j * 8 + i) * T + t], static_cast<double>(dy * hh[i]));
                 else dw[j][i] += static_cast<double>(dy * hh[i]);
                 if constexpr (TIGHT && !IN_LDS) asm volatile("" : "+v"(dw[j][i]));         // added here, not at the row's end, to which its terms would be kept
                 dot = __builtin_fmaf(dy * pair_at(w[j], i), hh[i], dot);
@@ -398,9 +402,6 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
                 r.h[j].hold();
                 r.x[j].hold();
             }
-            u32x4_any gate;
-            if constexpr (GROUPS) gate = r.gate[j];
-            else gate = one_gate[j];
             float hh[8], xh[8], o[8];
             r.h[j].template values<TAIL>(hh, left(j), hh_scale);
             r.x[j].template values<TAIL>(xh, left(j), xh_scale);
@@ -411,7 +412,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
                 o[i] = v * p.res;
                 ps[j][i] += static_cast<double>(v * xh[i]);
                 if constexpr (TIGHT) asm volatile("" : "+v"(ps[j][i]));
-                e[j][i] = v * (pair_at(gate, i) * pair_at(wp[j], i));
+                e[j][i] = v * (pair_at(gate[j], i) * pair_at(wp[j], i));
                 dot = __builtin_fmaf(e[j][i], xh[i], dot);
             }
             if (has(j)) store8_stream<F32, TAIL, false>(p.dr, base + (t + j * T) * 8, left(j), o);
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
                 for (int j = 0; j < V; ++j) {
                     float o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dwp_at(j, i) += ps[j][i] * static_cast<double>(pair_at(r.gate[j], i));
+                    for (int i = 0; i < 8; ++i) dwp_at(j, i) += ps[j][i] * static_cast<double>(pair_at(gate[j], i));
                     if (has(j)) {
                         const int at = (t + j * T) * 8;
                         if (whole) {
@@ -509,72 +510,77 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
 }
 
 struct GatedSumArgs {
-    const float *part_w, *part_p, *part_amax;
+    const float *part_w, *part_p, *part_amax, *segments;
     const uint16_t *gate, *post_weight;
     float *dw, *dwp, *dgate, *amax;
-    int H, parts, groups, accumulate, accumulate_gate;     // groups: 0 = no gate, 1 = one for all rows, which the shares of P do not hold yet
+    int rows, H, gate_rows, parts, workers, accumulate, accumulate_gate;
+    int groups;                     // 0 = no gate, 1 = one for all rows, which the shares of P do not hold yet
+    int sum_blocks;                 // workgroups for each of the two weights; behind them amax's, if there is one, then the segments'
+    int shares;                     // threads for a column of the segments
 };
 
 // The parts' shares added up in 64 bits, 32 columns a workgroup, 32 threads to a column that take every 32nd part: first dw's columns, then P's or dwp's; the
-// workgroup behind them raises *amax to the parts' maxima.
+// workgroup behind them raises *amax to the parts' maxima.  The rest make dgate of the groups whose rows several workers had, from their segments in the order of the rows.
 constexpr int kSumColumns = 32, kSumThreads = 1024;
 __global__ __launch_bounds__(kSumThreads) void k_gated_sum(const GatedSumArgs p) {
     constexpr int kShares = kSumThreads / kSumColumns;
     __shared__ double sh[kSumThreads];
-    const int t = threadIdx.x, blocks = (p.H + kSumColumns - 1) / kSumColumns;
-    if (static_cast<int>(blockIdx.x) >= 2 * blocks) {
+    const int t = threadIdx.x;
+    int block = blockIdx.x;
+    if (block < 2 * p.sum_blocks) {
+        const bool second = block >= p.sum_blocks;
+        const float* part = second ? p.part_p : p.part_w;
+        const int column = (block - (second ? p.sum_blocks : 0)) * kSumColumns + t % kSumColumns, share = t / kSumColumns;
+        double v = 0.0;
+        if (column < p.H) {
+#pragma unroll 8
+            for (int b = share; b < p.parts; b += kShares) v += part[static_cast<size_t>(b) * p.H + column];
+        }
+        sh[t] = v;
+        __syncthreads();
+        if (share == 0 && column < p.H) {
+            v = 0.0;
+#pragma unroll
+            for (int g = 0; g < kShares; ++g) v += sh[g * kSumColumns + t];
+            if (second && p.groups == 1) {
+                const double d = v * static_cast<double>(bf16_to_f32(p.post_weight[column]));
+                p.dgate[column] = static_cast<float>(p.accumulate_gate ? static_cast<double>(p.dgate[column]) + d : d);
+                v *= static_cast<double>(bf16_to_f32(p.gate[column]));
+            }
+            float* to = second ? p.dwp : p.dw;
+            to[column] = static_cast<float>(p.accumulate ? static_cast<double>(to[column]) + v : v);
+        }
+        return;
+    }
+    block -= 2 * p.sum_blocks;
+    if (p.amax && block-- == 0) {
         uint32_t m = 0;
         for (int b = t; b < p.parts; b += kSumThreads) m = max(m, __float_as_uint(p.part_amax[b]));
         m = row_max<false>(m, reinterpret_cast<uint32_t*>(sh));
         if (t == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
         return;
     }
-    const bool second = static_cast<int>(blockIdx.x) >= blocks;
-    const float* part = second ? p.part_p : p.part_w;
-    const int column = (blockIdx.x - (second ? blocks : 0)) * kSumColumns + t % kSumColumns, share = t / kSumColumns;
+    const int columns = kSumThreads / p.shares, across = (p.H + columns - 1) / columns;
+    const unsigned group = block / across, start = group * p.gate_rows, rows = p.rows;
+    const unsigned end = start + p.gate_rows < rows ? start + p.gate_rows : rows;
+    // the worker that has a row: the last one that begins at or before it
+    const unsigned k0 = static_cast<unsigned>(((static_cast<unsigned long long>(start) + 1) * p.workers - 1) / rows);
+    const unsigned k1 = static_cast<unsigned>((static_cast<unsigned long long>(end) * p.workers - 1) / rows);
+    if (k0 == k1) return;
+    const int at = t % columns, column = (block % across) * columns + at;
     double v = 0.0;
     if (column < p.H) {
-#pragma unroll 8
-        for (int b = share; b < p.parts; b += kShares) v += part[static_cast<size_t>(b) * p.H + column];
+#pragma unroll 4
+        for (unsigned k = k0 + t / columns; k <= k1; k += p.shares) v += p.segments[(static_cast<size_t>(k) * 2 + (k == k0 ? 1 : 0)) * p.H + column];
     }
     sh[t] = v;
     __syncthreads();
-    if (share == 0 && column < p.H) {
+    if (t < columns && column < p.H) {
         v = 0.0;
-#pragma unroll
-        for (int g = 0; g < kShares; ++g) v += sh[g * kSumColumns + t];
-        if (second && p.groups == 1) {
-            const double d = v * static_cast<double>(bf16_to_f32(p.post_weight[column]));
-            p.dgate[column] = static_cast<float>(p.accumulate_gate ? static_cast<double>(p.dgate[column]) + d : d);
-            v *= static_cast<double>(bf16_to_f32(p.gate[column]));
-        }
-        float* to = second ? p.dwp : p.dw;
-        to[column] = static_cast<float>(p.accumulate ? static_cast<double>(to[column]) + v : v);
-    }
-}
-
-// dgate of the groups whose rows several workers had, from their segments in the order of the rows: 64 columns a workgroup, four threads to a column.
-__global__ __launch_bounds__(256) void k_gated_segments(const float* __restrict__ segments, const uint16_t* __restrict__ post_weight,
-                                                        float* __restrict__ dgate, int rows, int H, int gate_rows, int workers, int accumulate) {
-    __shared__ double sh[256];
-    const unsigned blocks = (H + 63) / 64, group = blockIdx.x / blocks;
-    const int column = (blockIdx.x % blocks) * 64 + (threadIdx.x & 63);
-    const unsigned start = group * gate_rows, end = start + gate_rows < static_cast<unsigned>(rows) ? start + gate_rows : rows;
-    // the worker that has a row: the last one that begins at or before it
-    const unsigned k0 = static_cast<unsigned>(((static_cast<unsigned long long>(start) + 1) * workers - 1) / rows);
-    const unsigned k1 = static_cast<unsigned>((static_cast<unsigned long long>(end) * workers - 1) / rows);
-    if (k0 == k1) return;
-    double v = 0.0;
-    if (column < H) {
-#pragma unroll 4
-        for (unsigned k = k0 + (threadIdx.x >> 6); k <= k1; k += 4) v += segments[(static_cast<size_t>(k) * 2 + (k == k0 ? 1 : 0)) * H + column];
-    }
-    sh[threadIdx.x] = v;
-    __syncthreads();
-    if (threadIdx.x < 64 && column < H) {
-        v = ((sh[threadIdx.x] + sh[threadIdx.x + 64]) + (sh[threadIdx.x + 128] + sh[threadIdx.x + 192])) * static_cast<double>(bf16_to_f32(post_weight[column]));
-        float* to = dgate + static_cast<size_t>(group) * H + column;
-        *to = static_cast<float>(accumulate ? static_cast<double>(*to) + v : v);
+        for (int k = 0; k < p.shares; ++k) v += sh[k * columns + at];
+        v *= static_cast<double>(bf16_to_f32(p.post_weight[column]));
+        float* to = p.dgate + static_cast<size_t>(group) * p.H + column;
+        *to = static_cast<float>(p.accumulate_gate ? static_cast<double>(*to) + v : v);
     }
 }
 
@@ -629,7 +635,7 @@ constexpr int grad_chunks(int H) { return H <= 8 * kGradThreads ? 1 : H <= 16 * 
 int gated_parts(int rows, int H) {
     const int waves = H <= kOneWaveH ? 4 : row_threads(H, grad_chunks(H)) / kWave;
     const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;
-    int parts = waves < 8 ? 2048 / waves : 256;
+    int parts = 256 * (8 / waves);
     parts = parts < turns / 4 ? parts : turns / 4;
     parts = parts > 256 ? parts : 256;
     return parts < turns ? parts : turns;
@@ -670,10 +676,10 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     if (!d_grad_post_scale || !d_grad_scale || misaligned(d_grad_post_scale, 4) || misaligned(d_grad_scale, 4)) return CF_ERR_INVALID_ARG;
     GatedSumArgs s{};
     s.dw = d_grad_scale; s.dwp = d_grad_post_scale; s.H = p.H; s.accumulate = accumulate & CF_ACCUMULATE_SCALES;
-    const int blocks = 2 * ceil_div(p.H, kSumColumns);
+    s.sum_blocks = static_cast<int>(ceil_div(p.H, kSumColumns));
     if (p.rows == 0) {              // no rows: their sums are zero, and there is no gate
         if (s.accumulate) return CF_OK;
-        k_gated_sum<<<blocks, kSumThreads, 0, as_stream(stream)>>>(s);
+        k_gated_sum<<<2 * s.sum_blocks, kSumThreads, 0, as_stream(stream)>>>(s);
         return launch_status();
     }
     if (!p.dy || !p.sum || !p.x || !p.post_weight || !p.weight || !p.post_rms || !p.rms || !p.dr || (!p.dx && !p.q) || !d_workspace ||
@@ -707,12 +713,13 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     auto by_groups = [&](auto a, auto b) { plan.several ? go(a, b, yes) : go(a, b, no); };
     if (f32) kept ? by_groups(yes, yes) : by_groups(yes, no);
     else kept ? by_groups(no, yes) : by_groups(no, no);
-    s.part_w = p.part_w; s.part_p = p.part_p; s.part_amax = p.part_amax; s.gate = p.gate; s.post_weight = p.post_weight; s.dgate = p.dgate; s.amax = p.amax;
-    s.parts = plan.parts; s.groups = plan.several ? 0 : plan.groups; s.accumulate_gate = p.accumulate_gate;
-    k_gated_sum<<<blocks + (p.q ? 1 : 0), kSumThreads, 0, st>>>(s);
-    if (plan.segments)
-        k_gated_segments<<<static_cast<unsigned>(plan.groups) * ceil_div(p.H, 64), 256, 0, st>>>(p.segments, p.post_weight, p.dgate, p.rows, p.H, p.gate_rows,
-                                                                                              plan.workers, p.accumulate_gate);
+    s.part_w = p.part_w; s.part_p = p.part_p; s.part_amax = p.part_amax; s.segments = p.segments; s.gate = p.gate; s.post_weight = p.post_weight;
+    s.dgate = p.dgate; s.amax = p.q ? p.amax : nullptr; s.rows = p.rows; s.gate_rows = p.gate_rows; s.parts = plan.parts; s.workers = plan.workers;
+    s.groups = plan.several ? 0 : plan.groups; s.accumulate_gate = p.accumulate_gate;
+    // a group has some workers / groups segments
+    s.shares = plan.workers >= 16 * plan.groups ? 32 : plan.workers >= 4 * plan.groups ? 8 : 2;
+    const unsigned segment_blocks = plan.segments ? static_cast<unsigned>(plan.groups) * ceil_div(p.H, kSumThreads / s.shares) : 0;
+    k_gated_sum<<<2 * s.sum_blocks + (s.amax ? 1 : 0) + segment_blocks, kSumThreads, 0, st>>>(s);
     return launch_status();
 }
 
