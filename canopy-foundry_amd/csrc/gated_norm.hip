@@ -202,6 +202,7 @@ struct GatedGradArgs {
     float* segments;              // GROUPS: [workers, 2, H] shares of P of the groups that several workers have
     double* far_dwp;              // GROUPS, four chunks a thread: [parts, 32, threads], where neither registers nor LDS have room for it
     int rows, H, gate_rows, groups, workers;
+    unsigned share;
     float res, kept_inv;
 };
 
@@ -244,15 +245,55 @@ struct Saved8 {
     }
 };
 
-// Which rows a worker has where groups of them share a gate: equal shares, or, where every worker has two groups or more, whole groups.
-__host__ __device__ inline bool whole_groups(int groups, int workers) { return groups >= 2 * static_cast<long long>(workers); }
-__host__ __device__ inline unsigned first_row(unsigned worker, int rows, int gate_rows, int groups, int workers) {
-    if (whole_groups(groups, workers)) {
-        const unsigned long long r = static_cast<unsigned long long>(worker) * groups / workers * gate_rows;
-        return static_cast<unsigned>(r < static_cast<unsigned>(rows) ? r : rows);
+// Which rows a worker has where groups of them share a gate, and in which order.  With many groups a worker takes every workers-th one.  Otherwise the rows are cut
+// into equal shares, `share` rows each, without regard to the groups, so a group is a piece of one worker's share or of several that follow each other; the workers
+// of a group take turns at its rows (the shares' rows as they lie: 8192 x 4096 83.8 us, 76.0 in turns, so much do neighbouring rows help HBM).
+struct Walk {
+    unsigned worker, workers, rows, gate_rows, groups, share;
+    unsigned group, start, m, n, others, first_n, last_n, lead;
+    unsigned whole;                     // the group is this worker's alone
+
+    __host__ __device__ static bool by_groups(unsigned groups, unsigned workers) { return groups >= 8ull * workers; }
+    __device__ __forceinline__ bool begin() {
+        if (by_groups(groups, workers)) {
+            group = worker;
+        } else {
+            if (static_cast<unsigned long long>(worker) * share >= rows) return false;
+            group = worker * share / gate_rows;
+        }
+        return piece();
     }
-    return static_cast<unsigned>(static_cast<unsigned long long>(worker) * rows / workers);
-}
+    // the worker's piece of the group: n rows; of the group's other pieces the first has first_n rows, the last last_n, and the `others` between have `share`
+    __device__ __forceinline__ bool piece() {
+        if (group >= groups) return false;
+        start = group * gate_rows;
+        const unsigned end = gate_rows < rows - start ? start + gate_rows : rows;
+        m = lead = others = last_n = 0;
+        n = first_n = end - start;
+        whole = 1;
+        if (by_groups(groups, workers)) return true;
+        const unsigned k0 = start / share, k1 = (end - 1) / share, mine = worker * share;
+        if (start >= mine + share) return false;
+        if (k0 == k1) return true;
+        whole = 0;
+        first_n = (k0 + 1) * share - start;
+        last_n = end - k1 * share;
+        others = k1 - k0 - 1;
+        lead = worker - k0;
+        n = worker == k0 ? first_n : worker == k1 ? last_n : share;
+        return true;
+    }
+    __device__ __forceinline__ unsigned row() const {
+        const unsigned before = start + others * m + (m < first_n ? m : first_n) + (m < last_n ? m : last_n);
+        return lead == 0 ? before : before + lead - 1 + (m < first_n ? 1 : 0);
+    }
+    __device__ __forceinline__ bool last_of_piece() const { return m + 1 == n; }
+    __device__ __forceinline__ bool advance() {
+        if (++m < n) return true;
+        group += by_groups(groups, workers) ? workers : 1;
+        return piece();
+    }
+};
 
 template <bool TAIL>
 __device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const float (&v)[8]) {
@@ -283,15 +324,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
     const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
-    const unsigned rows = p.rows, step = GROUPS ? 1 : p.workers;
-    unsigned first = worker, end = rows;
-    if constexpr (GROUPS) {
-        first = end = rows;
-        if (worker < static_cast<unsigned>(p.workers)) {
-            first = first_row(worker, p.rows, p.gate_rows, p.groups, p.workers);
-            end = first_row(worker + 1, p.rows, p.gate_rows, p.groups, p.workers);
-        }
-    }
+    const unsigned rows = p.rows;
     const int chunks = TAIL ? (H + 7) / 8 : H / 8;
     auto left = [&](int j) { return TAIL ? H - (t + j * T) * 8 : 8; };
     auto has = [&](int j) { return t + j * T < chunks; };
@@ -322,6 +355,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         }
     };
     u32x4_any w[V], wp[V], gate[V];         // GROUPS: the gate is loaded where its rows begin
+    float gw[TIGHT ? 1 : V][8];                  // gate * wp
     double dw[IN_LDS ? 1 : V][8], ps[V][8], dwp[GROUPS && ONE_WAVE ? V : 1][8];
     // dwp, which changes at a group's end only
     auto dwp_at = [&](int j, int i) -> double& {
@@ -333,6 +367,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
     for (int j = 0; j < V; ++j) {
         w[j] = wp[j] = u32x4_any{0, 0, 0, 0};
         gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        if constexpr (GROUPS) gate[j] = u32x4_any{0, 0, 0, 0};
         if (has(j)) {
             w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
             wp[j] = load_weight<TAIL>(p.post_weight, (t + j * T) * 8, left(j), H);
@@ -342,6 +377,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             ps[j][i] = 0.0;
+            if constexpr (!TIGHT) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
             if constexpr (IN_LDS) sh_dw[(j * 8 + i) * T + t] = 0.0;
             else dw[j][i] = 0.0;
             if constexpr (GROUPS) dwp_at(j, i) = 0.0;
@@ -350,26 +386,41 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
     const float s = p.q ? *p.qscale : 0.0f;
     const bool s_finite = abs_bits(s) < kInf;
     float amax = 0.0f;
-    unsigned group = 0, group_first = 0, group_end = 0;
-    if constexpr (GROUPS) {
-        group = first / static_cast<unsigned>(p.gate_rows);
-        group_first = group * p.gate_rows;
-    }
     constexpr bool AHEAD = V <= 2;          // four chunks leave no registers for a second row
     Row r, next;
-    if (AHEAD && first < end) load(next, first);
-    for (unsigned row = first; row < end; row += step) {
+    Walk walk{worker, static_cast<unsigned>(p.workers), rows, static_cast<unsigned>(p.gate_rows), static_cast<unsigned>(p.groups), p.share}, then;
+    unsigned row = worker;
+    bool more = row < rows;
+    if constexpr (GROUPS) {
+        more = worker < static_cast<unsigned>(p.workers) && walk.begin();
+        if (more) row = walk.row();
+    }
+    if (AHEAD && more) load(next, row);
+    while (more) {
+        unsigned row_then = row + p.workers;
+        bool more_then = row_then < rows;
+        if constexpr (GROUPS) {
+            then = walk;
+            more_then = then.advance();
+            if (more_then) row_then = then.row();
+        }
         if constexpr (AHEAD) {
             r = next;
-            if (row + step < end) load(next, row + step);
+            if (more_then) load(next, row_then);
         } else {
             load(r, row);
         }
         if constexpr (GROUPS) {
-            if (row == first || row == group_first) {
+            if (walk.m == 0) {
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (has(j)) gate[j] = load_weight<TAIL>(p.gate + static_cast<size_t>(group) * H, (t + j * T) * 8, left(j), H);
+                    if (has(j)) {
+                        gate[j] = load_weight<TAIL>(p.gate + static_cast<size_t>(walk.group) * H, (t + j * T) * 8, left(j), H);
+                        if constexpr (!TIGHT) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
+                        }
+                    }
             }
         }
         const size_t base = static_cast<size_t>(row) * H;
@@ -412,7 +463,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
                 o[i] = v * p.res;
                 ps[j][i] += static_cast<double>(v * xh[i]);
                 if constexpr (TIGHT) asm volatile("" : "+v"(ps[j][i]));
-                e[j][i] = v * (pair_at(gate[j], i) * pair_at(wp[j], i));
+                e[j][i] = v * (TIGHT ? pair_at(gate[j], i) * pair_at(wp[j], i) : gw[TIGHT ? 0 : j][i]);
                 dot = __builtin_fmaf(e[j][i], xh[i], dot);
             }
             if (has(j)) store8_stream<F32, TAIL, false>(p.dr, base + (t + j * T) * 8, left(j), o);
@@ -439,9 +490,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
             }
         }
         if constexpr (GROUPS) {
-            group_end = group_first + p.gate_rows < rows ? group_first + p.gate_rows : rows;
-            if (row + 1 == group_end || row + 1 == end) {
-                const bool whole = group_first >= first && group_end <= end;
+            if (walk.last_of_piece()) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float o[8];
@@ -449,8 +498,8 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
                     for (int i = 0; i < 8; ++i) dwp_at(j, i) += ps[j][i] * static_cast<double>(pair_at(gate[j], i));
                     if (has(j)) {
                         const int at = (t + j * T) * 8;
-                        if (whole) {
-                            float* to = p.dgate + static_cast<size_t>(group) * H;
+                        if (walk.whole) {
+                            float* to = p.dgate + static_cast<size_t>(walk.group) * H;
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 double v = ps[j][i] * static_cast<double>(pair_at(wp[j], i));
@@ -461,16 +510,17 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
                         } else {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) o[i] = static_cast<float>(ps[j][i]);
-                            store8_f32<TAIL>(p.segments + (static_cast<size_t>(worker) * 2 + (group_first >= first ? 1 : 0)) * H, at, left(j), o);
+                            store8_f32<TAIL>(p.segments + (static_cast<size_t>(worker) * 2 + (walk.lead == 0 ? 1 : 0)) * H, at, left(j), o);
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) ps[j][i] = 0.0;
                 }
-                ++group;
-                group_first += p.gate_rows;
             }
+            walk = then;
         }
+        row = row_then;
+        more = more_then;
     }
     // the workgroup's shares
     auto leave = [&](auto at, float* to) {
@@ -513,7 +563,8 @@ struct GatedSumArgs {
     const float *part_w, *part_p, *part_amax, *segments;
     const uint16_t *gate, *post_weight;
     float *dw, *dwp, *dgate, *amax;
-    int rows, H, gate_rows, parts, workers, accumulate, accumulate_gate;
+    int rows, H, gate_rows, parts, accumulate, accumulate_gate;
+    unsigned share;                 // rows a worker
     int groups;                     // 0 = no gate, 1 = one for all rows, which the shares of P do not hold yet
     int sum_blocks;                 // workgroups for each of the two weights; behind them amax's, if there is one, then the segments'
     int shares;                     // threads for a column of the segments
@@ -563,9 +614,7 @@ __global__ __launch_bounds__(kSumThreads) void k_gated_sum(const GatedSumArgs p)
     const int columns = kSumThreads / p.shares, across = (p.H + columns - 1) / columns;
     const unsigned group = block / across, start = group * p.gate_rows, rows = p.rows;
     const unsigned end = start + p.gate_rows < rows ? start + p.gate_rows : rows;
-    // the worker that has a row: the last one that begins at or before it
-    const unsigned k0 = static_cast<unsigned>(((static_cast<unsigned long long>(start) + 1) * p.workers - 1) / rows);
-    const unsigned k1 = static_cast<unsigned>((static_cast<unsigned long long>(end) * p.workers - 1) / rows);
+    const unsigned k0 = start / p.share, k1 = (end - 1) / p.share;
     if (k0 == k1) return;
     const int at = t % columns, column = (block % across) * columns + at;
     double v = 0.0;
@@ -643,6 +692,7 @@ int gated_parts(int rows, int H) {
 struct GradPlan {
     int parts, workers, groups;         // groups: 0 = no gate
     bool several, segments;             // several groups; some of them in several workers' rows
+    unsigned share;                     // rows of a worker
     size_t far, bytes;
 };
 GradPlan grad_plan(int rows, int H, int gate_rows) {
@@ -652,7 +702,8 @@ GradPlan grad_plan(int rows, int H, int gate_rows) {
     g.groups = gate_rows > 0 ? (rows - 1) / gate_rows + 1 : 0;
     g.several = g.groups > 1;
     g.workers = H <= kOneWaveH ? (4 * g.parts < rows ? 4 * g.parts : rows) : g.parts;
-    g.segments = g.several && !whole_groups(g.groups, g.workers);
+    g.share = static_cast<unsigned>((rows - 1) / g.workers + 1);
+    g.segments = g.several && !Walk::by_groups(g.groups, g.workers);
     const size_t shares = 2 * static_cast<size_t>(g.parts) + (g.segments ? 2 * static_cast<size_t>(g.workers) : 0);
     g.far = g.several && grad_chunks(H) == 4 ? static_cast<size_t>(g.parts) * 4 * 8 * row_threads(H, 4) * sizeof(double) : 0;
     g.bytes = g.far + (shares * H + g.parts) * sizeof(float);
@@ -700,6 +751,7 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     p.part_amax = p.segments + (plan.segments ? 2 * static_cast<size_t>(plan.workers) * p.H : 0);
     p.groups = plan.groups;
     p.workers = plan.workers;
+    p.share = plan.share;
     p.accumulate_gate = accumulate & CF_ACCUMULATE_GATE;
     p.kept_inv = 1.0f / kept_scale(p.H);
     hipStream_t st = as_stream(stream);
@@ -714,7 +766,7 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     if (f32) kept ? by_groups(yes, yes) : by_groups(yes, no);
     else kept ? by_groups(no, yes) : by_groups(no, no);
     s.part_w = p.part_w; s.part_p = p.part_p; s.part_amax = p.part_amax; s.segments = p.segments; s.gate = p.gate; s.post_weight = p.post_weight;
-    s.dgate = p.dgate; s.amax = p.q ? p.amax : nullptr; s.rows = p.rows; s.gate_rows = p.gate_rows; s.parts = plan.parts; s.workers = plan.workers;
+    s.dgate = p.dgate; s.amax = p.q ? p.amax : nullptr; s.rows = p.rows; s.gate_rows = p.gate_rows; s.parts = plan.parts; s.share = plan.share;
     s.groups = plan.several ? 0 : plan.groups; s.accumulate_gate = p.accumulate_gate;
     // a group has some workers / groups segments
     s.shares = plan.workers >= 16 * plan.groups ? 32 : plan.workers >= 4 * plan.groups ? 8 : 2;
