@@ -39,7 +39,7 @@ __device__ __forceinline__ float pair_at(const u32x4_any& v, int i) { return (i 
 
 // One row in registers, V chunks of eight elements a thread, as k_add_norm holds it: everything is read and written once.
 template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_gated_norm(const GatedNormArgs p) {
+__global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_norm(const GatedNormArgs p) {
     __shared__ float sh_sum[4][16];
     __shared__ uint32_t sh_max[4][16];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
@@ -572,34 +572,35 @@ struct GatedSumArgs {
 
 // The parts' shares added up in 64 bits, 32 columns a workgroup, 32 threads to a column that take every 32nd part: first dw's columns, then P's or dwp's; the
 // workgroup behind them raises *amax to the parts' maxima.  The rest make dgate of the groups whose rows several workers had, from their segments in the order of the rows.
-constexpr int kSumColumns = 32, kSumThreads = 1024;
+constexpr int kSumThreads = 1024, kSumColumns = 32, kSumShares = kSumThreads / kSumColumns;
+struct Sum4 { double v[4]; };
 __global__ __launch_bounds__(kSumThreads) void k_gated_sum(const GatedSumArgs p) {
-    constexpr int kShares = kSumThreads / kSumColumns;
-    __shared__ double sh[kSumThreads];
+    __shared__ Sum4 sh[kSumThreads];
     const int t = threadIdx.x;
     int block = blockIdx.x;
     if (block < 2 * p.sum_blocks) {
         const bool second = block >= p.sum_blocks;
         const float* part = second ? p.part_p : p.part_w;
-        const int column = (block - (second ? p.sum_blocks : 0)) * kSumColumns + t % kSumColumns, share = t / kSumColumns;
-        double v = 0.0;
-        if (column < p.H) {
+        const int c = (block - (second ? p.sum_blocks : 0)) * kSumColumns + t % kSumColumns;
+        double* one = &sh[0].v[0];
+        double sum = 0.0;
+        if (c < p.H) {
 #pragma unroll 8
-            for (int b = share; b < p.parts; b += kShares) v += part[static_cast<size_t>(b) * p.H + column];
+            for (int b = t / kSumColumns; b < p.parts; b += kSumShares) sum += part[static_cast<size_t>(b) * p.H + c];
         }
-        sh[t] = v;
+        one[t] = sum;
         __syncthreads();
-        if (share == 0 && column < p.H) {
-            v = 0.0;
+        if (t < kSumColumns && c < p.H) {
+            sum = 0.0;
 #pragma unroll
-            for (int g = 0; g < kShares; ++g) v += sh[g * kSumColumns + t];
+            for (int g = 0; g < kSumShares; ++g) sum += one[g * kSumColumns + t];
             if (second && p.groups == 1) {
-                const double d = v * static_cast<double>(bf16_to_f32(p.post_weight[column]));
-                p.dgate[column] = static_cast<float>(p.accumulate_gate ? static_cast<double>(p.dgate[column]) + d : d);
-                v *= static_cast<double>(bf16_to_f32(p.gate[column]));
+                const double d = sum * static_cast<double>(bf16_to_f32(p.post_weight[c]));
+                p.dgate[c] = static_cast<float>(p.accumulate_gate ? static_cast<double>(p.dgate[c]) + d : d);
+                sum *= static_cast<double>(bf16_to_f32(p.gate[c]));
             }
             float* to = second ? p.dwp : p.dw;
-            to[column] = static_cast<float>(p.accumulate ? static_cast<double>(to[column]) + v : v);
+            to[c] = static_cast<float>(p.accumulate ? static_cast<double>(to[c]) + sum : sum);
         }
         return;
     }
@@ -611,25 +612,39 @@ __global__ __launch_bounds__(kSumThreads) void k_gated_sum(const GatedSumArgs p)
         if (t == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
         return;
     }
-    const int columns = kSumThreads / p.shares, across = (p.H + columns - 1) / columns;
+    const int quads = kSumThreads / p.shares, across = (p.H + 4 * quads - 1) / (4 * quads);
     const unsigned group = block / across, start = group * p.gate_rows, rows = p.rows;
-    const unsigned end = start + p.gate_rows < rows ? start + p.gate_rows : rows;
+    const unsigned end = p.gate_rows < static_cast<int>(rows - start) ? start + p.gate_rows : rows;
     const unsigned k0 = start / p.share, k1 = (end - 1) / p.share;
     if (k0 == k1) return;
-    const int at = t % columns, column = (block % across) * columns + at;
-    double v = 0.0;
+    const int first = (block % across) * quads * 4, column = first + t % quads * 4;
+    Sum4 v{};
     if (column < p.H) {
-#pragma unroll 4
-        for (unsigned k = k0 + t / columns; k <= k1; k += p.shares) v += p.segments[(static_cast<size_t>(k) * 2 + (k == k0 ? 1 : 0)) * p.H + column];
+        const int n = p.H - column;
+        for (unsigned k = k0 + t / quads; k <= k1; k += 4 * p.shares) {         // four loads on their way
+            f32x4_any part[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const unsigned from = k + u * p.shares <= k1 ? k + u * p.shares : k;
+                const float* at = p.segments + (static_cast<size_t>(from) * 2 + (from == k0 ? 1 : 0)) * p.H + column;
+                if (n >= 4) part[u] = *reinterpret_cast<const f32x4_any*>(at);
+                else part[u] = f32x4_any{at[0], n > 1 ? at[1] : 0.0f, n > 2 ? at[2] : 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (k + u * p.shares <= k1) v.v[i] += static_cast<double>(part[u][i]);
+        }
     }
     sh[t] = v;
     __syncthreads();
-    if (t < columns && column < p.H) {
-        v = 0.0;
-        for (int k = 0; k < p.shares; ++k) v += sh[k * columns + at];
-        v *= static_cast<double>(bf16_to_f32(p.post_weight[column]));
-        float* to = p.dgate + static_cast<size_t>(group) * p.H + column;
-        *to = static_cast<float>(p.accumulate_gate ? static_cast<double>(*to) + v : v);
+    for (int c = t; c < quads * 4 && first + c < p.H; c += kSumThreads) {
+        double sum = 0.0;
+        for (int k = 0; k < p.shares; ++k) sum += sh[k * quads + c / 4].v[c % 4];
+        sum *= static_cast<double>(bf16_to_f32(p.post_weight[first + c]));
+        float* to = p.dgate + static_cast<size_t>(group) * p.H + first + c;
+        *to = static_cast<float>(p.accumulate_gate ? static_cast<double>(*to) + sum : sum);
     }
 }
 
@@ -639,13 +654,29 @@ float kept_scale(int H) {
     return std::ldexp(1.0f, e);
 }
 
+// Chunks of a row that a thread has.  Two reductions follow each other here, which many rows hide best with some four workgroups a CU, whole rows behind each other's;
+// a row alone wants as many threads as it can have.  1, 2, 4 chunks, us, rows of both checkpoints, 33.6 M elements (the first line: kernel alone):
+//     1 row of 4096, bf16       3.7   4.4   5.8             H = 1024, f32     82.5  82.6  85.0
+//     H = 1024, bf16           60.3  57.3  68.8             H = 4096, f32     82.9  83.9  89.3
+//     H = 4096, bf16           61.4  58.5  61.0             H = 5120, f32     93.5  86.2  88.8
+//     H = 5120, bf16           76.6  62.8  62.2             H = 7168, f32     93.1  87.3  89.3
+//     H = 6144, bf16           73.8  65.1  60.6             H = 12288, f32      -   91.1 100.0
+//     H = 7168, bf16           78.5  65.2  61.4             H = 16384, f32      -   91.5  94.0
+//     H = 12288, bf16            -   63.7  74.2             H = 16384, bf16     -   70.9  63.3
+int forward_chunks(int rows, int H, bool f32) {
+    if (rows <= 256 && H <= kOneChunkH) return 1;
+    return !f32 && ((H >= 5120 && H <= kOneChunkH) || H > 14336) ? 4 : 2;
+}
+
 template <bool F32, int QMODE, bool TAIL>
 int launch_gated_norm(GatedNormArgs p, hipStream_t st) {
     for (; p.row0 < static_cast<unsigned>(p.rows); p.row0 += kLaunchRows) {
         const unsigned left = static_cast<unsigned>(p.rows) - p.row0, n = left < kLaunchRows ? left : kLaunchRows;
+        const int V = forward_chunks(p.rows, p.H, F32);
         if (p.H <= kOneWaveH) k_gated_norm<F32, QMODE, TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
-        else if (p.H <= kOneChunkH) k_gated_norm<F32, QMODE, TAIL, false, 1><<<n, row_threads(p.H, 1), 0, st>>>(p);
-        else k_gated_norm<F32, QMODE, TAIL, false, 2><<<n, row_threads(p.H, 2), 0, st>>>(p);
+        else if (V == 1) k_gated_norm<F32, QMODE, TAIL, false, 1><<<n, row_threads(p.H, 1), 0, st>>>(p);
+        else if (V == 2) k_gated_norm<F32, QMODE, TAIL, false, 2><<<n, row_threads(p.H, 2), 0, st>>>(p);
+        else k_gated_norm<F32, QMODE, TAIL, false, 4><<<n, row_threads(p.H, 4), 0, st>>>(p);
     }
     return launch_status();
 }
@@ -770,7 +801,7 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     s.groups = plan.several ? 0 : plan.groups; s.accumulate_gate = p.accumulate_gate;
     // a group has some workers / groups segments
     s.shares = plan.workers >= 16 * plan.groups ? 32 : plan.workers >= 4 * plan.groups ? 8 : 2;
-    const unsigned segment_blocks = plan.segments ? static_cast<unsigned>(plan.groups) * ceil_div(p.H, kSumThreads / s.shares) : 0;
+    const unsigned segment_blocks = plan.segments ? static_cast<unsigned>(plan.groups) * ceil_div(p.H, 4 * kSumThreads / s.shares) : 0;
     k_gated_sum<<<2 * s.sum_blocks + (s.amax ? 1 : 0) + segment_blocks, kSumThreads, 0, st>>>(s);
     return launch_status();
 }
