@@ -111,6 +111,30 @@ __device__ __forceinline__ void store8_stream(void* p, size_t at, int n, const f
         }
     }
 }
+// Eight values as bytes by the conversion alone: what is not above the format's largest value by more than roundings, or, after saturate_fp8(), anything
+// finite.  A NaN is a NaN; an infinity is one in E4M3 and an infinity in E5M2.
+template <bool E5M2>
+__device__ __forceinline__ u32x2_any convert8_fp8(const float (&v)[8]) {
+    u32x2_any o;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        int r = 0;
+        if constexpr (E5M2) {
+            r = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * i], v[4 * i + 1], r, false);
+            r = __builtin_amdgcn_cvt_pk_bf8_f32(v[4 * i + 2], v[4 * i + 3], r, true);
+        } else {
+            r = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], r, false);
+            r = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], r, true);
+        }
+        o[i] = static_cast<uint32_t>(r);
+    }
+    return o;
+}
+// From here on the wavefront's conversions to 8 bits give the largest finite value for finite ones beyond it (MODE.FP16_OVFL, which holds for fp16 and bf16 as well), so
+// that no clamp is needed.  What is converted has to be a product with `factor`, by which the compiler cannot move it up past the change.
+__device__ __forceinline__ void saturate_fp8(float& factor) {
+    asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 23, 1), 1\n\ts_nop 1" : "+v"(factor));
+}
 // Eight values as bytes; finite: there is no NaN among them.
 __device__ __forceinline__ u32x2_any pack8_fp8(bool e5m2, bool finite, const float (&v)[8]) {
     u32x2_any o;

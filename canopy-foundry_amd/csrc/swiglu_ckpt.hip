@@ -7,17 +7,16 @@
 namespace cf {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kKeepThreads = 512;
+#ifndef KEEPV
+#define KEEPV 1
+#endif
 constexpr int kMaxRow = 32768;              // of the form that holds a whole row
 
-// sigmoid(g).  The exponent g * log2(e) is carried in two terms, so that the result keeps its relative error of a few 2^-24 where g is far below zero (one term:
-// |g| * 2^-24).  Below -87, where it is under 2^-125, it is taken as 0.
+// sigmoid(g), by the two units' instructions (1 ulp each).  The rounding of the exponent's argument costs e^-g a relative 1.2 |g| 2^-24, so the result is off by
+// (6 + 1.2 |g| (1 - s)) 2^-24 at most; carrying the argument in two terms took four more of eleven instructions.  0 where e^-g leaves fp32.
 __device__ __forceinline__ float sigmoid(float g) {
-    const float x = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f), t = x * -1.44269502f;        // log2(e) to 24 bits, and what that leaves
-    const float rest = __builtin_fmaf(x, -1.92596299e-8f, __builtin_fmaf(x, -1.44269502f, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, rest * 0.693147181f, e));
-    return g < -87.0f ? 0.0f : s;
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
 }
 
 struct SwigluKeepArgs {
@@ -29,7 +28,8 @@ struct SwigluKeepArgs {
     const float* qscale;            // Q_RECORD
     float* amax;
     int rows, I;
-    unsigned row0, row_end;         // the launch's rows
+    unsigned row0;                  // the launch's first row
+    unsigned parts;                 // workgroups of a row
     int e5m2;
 };
 
@@ -41,158 +41,140 @@ __device__ __forceinline__ void cut(Raw8<false>& r, int n) {
         for (int k = 0; k < 4; ++k) r.v[0][k] &= 2 * k + 1 < n ? 0xffffffffu : 2 * k < n ? 0xffffu : 0u;
     }
 }
-
-// The maximum of |v| over the 16 lanes of a group, as bits and without NaNs; finite: there is neither an infinity nor a NaN.
-__device__ __forceinline__ uint32_t group_max(const Raw8<false>& r, bool& finite) {
+// The largest |v| of a group's 16 lanes, without its NaNs: as the bits of bf16 pairs while there are none, which costs half.
+__device__ __forceinline__ float group_max(const Raw8<false>& r) {
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) m = pk_absmax(m, r.v[0][k]);
-    m = max16(max(m << 16, m & 0xffff0000u));
-    finite = __all(m < kInf);
-    if (!finite) {
+    m = max(m << 16, m & 0xffff0000u);
+    if (__any(m > kInf)) {
         float f = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) f = fmaxf(f, fabsf(r.at(i)));
-        m = max16(__float_as_uint(f));
+        m = __float_as_uint(f);
     }
-    return m;
+    return __uint_as_float(max16(m));
 }
-// A chunk of a checkpoint, and by its group's first lane the descale.
-template <bool TAIL>
-__device__ __forceinline__ void keep(const Raw8<false>& r, uint8_t* to, size_t at, int n, float* descale) {
-    bool finite;
-    const float a = fmaxf(__uint_as_float(group_max(r, finite)), 1e-12f), s = 448.0f / a;
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = r.at(i) * s;
-    if (n > 0) {
-        store8_fp8<TAIL>(to, at, n, false, finite, v);
-        if ((threadIdx.x & 15) == 0) *descale = a / 448.0f;
-    }
-}
-__device__ __forceinline__ void activate(const Raw8<false>& g, const Raw8<false>& u, float (&a)[8], uint32_t& top) {
-    top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = g.at(i);
-        a[i] = v * sigmoid(v) * u.at(i);
-        top = max(top, abs_bits(a[i]));
-    }
-}
-__device__ __forceinline__ uint32_t number(const float (&a)[8]) {
+// a lane's value for the 16 around it
+template <int LANE>
+__device__ __forceinline__ float from_lane(float v) { return __uint_as_float(dpp<0x150 + LANE>(__float_as_uint(v))); }
+__device__ __forceinline__ float largest(const float (&a)[8]) {
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(a[i]));
-    return __float_as_uint(m);
-}
-template <bool TAIL>
-__device__ __forceinline__ void load_pair(const SwigluKeepArgs& p, unsigned row, int at, int n, Raw8<false>& g, Raw8<false>& u) {
-    clear8(g);
-    clear8(u);
-    if (n > 0) {
-        const size_t from = row * p.ld + at;
-        const bool whole = static_cast<size_t>(static_cast<unsigned>(p.rows) - 1 - row) * p.ld + n >= 8;       // eight elements from here on in the tensor
-        load8<false, TAIL>(p.gate, from, n, whole, g);
-        load8<false, TAIL>(p.up, from, n, whole, u);
-        cut<TAIL>(g, n);
-        cut<TAIL>(u, n);
-    }
+    return m;
 }
 
-// 16 lanes a group of 128 elements, workgroups that walk over all groups.
-template <int QMODE, bool TAIL>
-__global__ __launch_bounds__(kThreads) void k_swiglu_keep(const SwigluKeepArgs p) {
+// A thread has V chunks of eight elements of a row, chunk c by thread c % T of the row's workgroup or, where the scale is not the whole row's, of one of its `parts`.  Sixteen
+// lanes are a group of 128 elements.  Of the two (Q_BLOCK: three) scales of a group each quarter of its lanes makes one, in the same instructions: a division takes a dozen.
+// What has been divided by its own maximum needs no clamp.
+template <int QMODE, bool TAIL, bool ONE_WAVE, int V>
+__global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThreads) void k_swiglu_keep(const SwigluKeepArgs p) {
     __shared__ uint32_t sh[16];
-    const unsigned groups = (static_cast<unsigned>(p.I) + 127) / 128, total = (p.row_end - p.row0) * groups;
-    const int lane = threadIdx.x & 15;
-    const float F = QMODE == Q_RECORD && p.e5m2 ? 57344.0f : 448.0f;
-    const float qs = QMODE == Q_RECORD ? *p.qscale : 0.0f;
-    uint32_t most = 0;
-    for (unsigned i = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4); i < total; i += gridDim.x * (kThreads / 16)) {
-        const unsigned row = p.row0 + i / groups, group = i % groups;
-        const int at = group * 128 + lane * 8, n = p.I - at;
-        const size_t to = static_cast<size_t>(row) * p.I + at, slot = static_cast<size_t>(row) * groups + group;
-        Raw8<false> g, u;
-        load_pair<TAIL>(p, row, at, n, g, u);
-        keep<TAIL>(g, p.gate8, to, n, p.gate_descale + slot);
-        keep<TAIL>(u, p.up8, to, n, p.up_descale + slot);
-        float a[8];
-        uint32_t m;
-        activate(g, u, a, m);
-        float s = qs;
-        bool finite;
-        if constexpr (QMODE == Q_BLOCK) {
-            m = max16(m);
-            finite = __all(m < kInf);
-            if (!finite) m = max16(number(a));
-            const float top = fmaxf(__uint_as_float(m), 1e-12f);
-            s = F / top;
-            if (lane == 0) {
-                p.scale[slot] = s;
-                p.descale[slot] = top / F;
-            }
-        } else {
-            finite = __all(m < kInf) && abs_bits(s) < kInf;
-            most = max(most, m < kInf ? m : number(a));
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) a[k] *= s;
-        if (n > 0) store8_fp8<TAIL>(p.q, to, n, QMODE == Q_RECORD && p.e5m2, finite, a);
-    }
-    if constexpr (QMODE == Q_RECORD) {
-        most = row_max<false>(most, sh);
-        if (threadIdx.x == 0) atomic_max_nonneg(p.amax, __uint_as_float(most));
-    }
-}
-
-// A row in the registers of its threads, V chunks of eight elements each, for a scale that is the whole row's.
-template <bool TAIL, bool ONE_WAVE, int V>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : 1024) void k_swiglu_keep_rows(const SwigluKeepArgs p) {
-    __shared__ uint32_t sh[2][16];
     const int T = ONE_WAVE ? kWave : blockDim.x;
-    unsigned row = p.row0 + blockIdx.x;
+    unsigned row, part = 0;
     int t = threadIdx.x;
     if constexpr (ONE_WAVE) {
         row = __builtin_amdgcn_readfirstlane(p.row0 + blockIdx.x * 4 + (threadIdx.x >> 6));
         t &= 63;
-        if (row >= p.row_end) return;
+        if (row >= static_cast<unsigned>(p.rows)) return;
+    } else if constexpr (QMODE == Q_ROWS) {
+        row = p.row0 + blockIdx.x;
+    } else {
+        row = p.row0 + blockIdx.x / p.parts;
+        part = blockIdx.x % p.parts;
     }
     const unsigned groups = (static_cast<unsigned>(p.I) + 127) / 128;
-    const size_t base = static_cast<size_t>(row) * p.I;
+    const size_t base = static_cast<size_t>(row) * p.I, slots = static_cast<size_t>(row) * groups;
+    const int lane = threadIdx.x & 15, first = part * T * V + t;
+    auto at = [&](int j) { return (first + j * T) * 8; };
+    auto left = [&](int j) { return p.I - at(j); };
+
     Raw8<false> g[V], u[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) load_pair<TAIL>(p, row, (t + j * T) * 8, p.I - (t + j * T) * 8, g[j], u[j]);
-    float a[V][8];
-    uint32_t m = 0;
+    for (int j = 0; j < V; ++j) {
+        clear8(g[j]);
+        clear8(u[j]);
+        if (left(j) > 0) {
+            const size_t from = row * p.ld + at(j);
+            const bool whole = static_cast<size_t>(static_cast<unsigned>(p.rows) - 1 - row) * p.ld + left(j) >= 8;       // eight elements from here on in the tensor
+            load8<false, TAIL>(p.gate, from, left(j), whole, g[j]);
+            load8<false, TAIL>(p.up, from, left(j), whole, u[j]);
+            cut<TAIL>(g[j], left(j));
+            cut<TAIL>(u[j], left(j));
+        }
+    }
+    const bool e5m2 = QMODE != Q_BLOCK && p.e5m2;
+    const float F = e5m2 ? 57344.0f : 448.0f;
+    float qs = 0.0f;
+    if constexpr (QMODE == Q_RECORD) {
+        qs = *p.qscale;
+        saturate_fp8(qs);
+    }
+    float a[QMODE == Q_ROWS ? V : 1][8], most = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = t + j * T, n = p.I - c * 8;
-        const size_t slot = static_cast<size_t>(row) * groups + (c >> 4);
-        keep<TAIL>(g[j], p.gate8, base + c * 8, n, p.gate_descale + slot);
-        keep<TAIL>(u[j], p.up8, base + c * 8, n, p.up_descale + slot);
-        uint32_t top;
-        activate(g[j], u[j], a[j], top);
-        m = max(m, top);
-    }
-    m = row_max<ONE_WAVE>(m, sh[0]);
-    const bool finite = m < kInf;
-    if (!finite) {
-        uint32_t top = 0;
+        float (&o)[8] = a[QMODE == Q_ROWS ? j : 0];
 #pragma unroll
-        for (int j = 0; j < V; ++j) top = max(top, number(a[j]));
-        m = row_max<ONE_WAVE>(top, sh[1]);
-    }
-    const float F = p.e5m2 ? 57344.0f : 448.0f, most = fmaxf(__uint_as_float(m), 1e-12f), s = F / most;
-    if (t == 0) {
-        p.scale[row] = s;
-        p.descale[row] = most / F;
-    }
+        for (int i = 0; i < 8; ++i) {
+            const float v = g[j].at(i);
+            o[i] = v * sigmoid(v) * u[j].at(i);
+        }
+        float m = largest(o);
+        const float mg = group_max(g[j]), mu = group_max(u[j]);
+        float one = lane < 4 ? mg : mu;
+        if constexpr (QMODE == Q_BLOCK) {
+            m = __uint_as_float(max16(__float_as_uint(m)));
+            one = lane < 8 ? one : m;
+        }
+        one = fmaxf(one, 1e-12f);
+        const float s = 448.0f / one, d = one / 448.0f;
+        const size_t slot = slots + (static_cast<unsigned>(at(j)) >> 7);
+        if ((lane & 3) == 0 && lane < (QMODE == Q_BLOCK ? 12 : 8) && left(j) > -8 * lane) {
+            (lane == 0 ? p.gate_descale : lane == 4 ? p.up_descale : p.descale)[slot] = d;
+            if (QMODE == Q_BLOCK && lane == 8) p.scale[slot] = s;
+        }
+        const float sg = from_lane<0>(s), su = from_lane<4>(s);
+        float v[8];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int n = p.I - (t + j * T) * 8;
+        for (int i = 0; i < 8; ++i) v[i] = g[j].at(i) * sg;
+        if (left(j) > 0) store8_bytes<TAIL>(p.gate8, base + at(j), left(j), convert8_fp8<false>(v));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[j][i] *= s;
-        if (n > 0) store8_fp8<TAIL>(p.q, base + (t + j * T) * 8, n, p.e5m2, finite, a[j]);
+        for (int i = 0; i < 8; ++i) v[i] = u[j].at(i) * su;
+        if (left(j) > 0) store8_bytes<TAIL>(p.up8, base + at(j), left(j), convert8_fp8<false>(v));
+        most = fmaxf(most, m);
+        if constexpr (QMODE != Q_ROWS) {
+            const float sa = QMODE == Q_BLOCK ? from_lane<8>(s) : qs;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = o[i] * sa;
+            u32x2_any b;
+            if (QMODE == Q_RECORD && (__any(m == __builtin_inff()) || abs_bits(qs) >= kInf)) b = pack8_fp8(e5m2, false, v);
+            else b = e5m2 ? convert8_fp8<true>(v) : convert8_fp8<false>(v);
+            if (left(j) > 0) store8_bytes<TAIL>(p.q, base + at(j), left(j), b);
+        }
+    }
+    if constexpr (QMODE == Q_ROWS) {
+        most = __uint_as_float(row_max<ONE_WAVE>(__float_as_uint(most), sh));
+        most = fmaxf(most, 1e-12f);
+        const float s = F / most;
+        if (t == 0) {
+            p.scale[row] = s;
+            p.descale[row] = most / F;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[j][i] *= s;
+            if (left(j) > 0) store8_bytes<TAIL>(p.q, base + at(j), left(j), e5m2 ? convert8_fp8<true>(a[j]) : convert8_fp8<false>(a[j]));
+        }
+    }
+    if constexpr (QMODE == Q_RECORD) {
+        const uint32_t m = row_max<false>(__float_as_uint(most), sh);
+        if (threadIdx.x == 0) {
+            float before;
+            raise_first(p.amax, m, blockIdx.x, gridDim.x, before);
+            raise_last(p.amax, m, blockIdx.x, gridDim.x, before);
+        }
     }
 }
 
@@ -208,7 +190,7 @@ struct SwigluGradArgs {
     const float *qscale, *act_qscale;
     float* amax;
     int rows, I;
-    unsigned row0, row_end;
+    unsigned row0, parts;
 };
 
 // what eight elements give: dg, du and the activation
@@ -229,26 +211,23 @@ __device__ __forceinline__ void grads8(const Raw8<false>& d, const u32x2_any& g8
     }
 }
 
-// bf16 outputs: 16 lanes a group of 128 elements, as k_swiglu_keep.
+// bf16 outputs, a chunk a thread; workgroups as k_swiglu_keep's.
 template <bool TAIL>
-__global__ __launch_bounds__(kThreads) void k_swiglu_grad(const SwigluGradArgs p) {
-    const unsigned groups = (static_cast<unsigned>(p.I) + 127) / 128, total = (p.row_end - p.row0) * groups;
-    for (unsigned i = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4); i < total; i += gridDim.x * (kThreads / 16)) {
-        const unsigned row = p.row0 + i / groups, group = i % groups;
-        const int at = group * 128 + (threadIdx.x & 15) * 8, n = p.I - at;
-        if (n <= 0) continue;
-        const size_t from = static_cast<size_t>(row) * p.I + at, slot = static_cast<size_t>(row) * groups + group;
-        const bool whole = static_cast<size_t>(static_cast<unsigned>(p.rows) - 1 - row) * p.I + n >= 8;
-        Raw8<false> d;
-        clear8(d);
-        load8<false, TAIL>(p.grad, from, n, whole, d);
-        const u32x2_any g8 = load8_bytes<TAIL>(p.gate8, from, n, whole), u8 = load8_bytes<TAIL>(p.up8, from, n, whole);
-        Grads8 o;
-        grads8<TAIL>(d, g8, u8, p.gate_descale[slot], p.up_descale[slot], n, o);
-        store8_bf16<TAIL>(p.grad_gate, row * p.ld + at, n, o.dg);
-        store8_bf16<TAIL>(p.grad_up, row * p.ld + at, n, o.du);
-        if (p.act) store8_bf16<TAIL>(p.act, from, n, o.a);
-    }
+__global__ __launch_bounds__(kKeepThreads) void k_swiglu_grad(const SwigluGradArgs p) {
+    const unsigned row = p.row0 + blockIdx.x / p.parts, groups = (static_cast<unsigned>(p.I) + 127) / 128;
+    const int at = ((blockIdx.x % p.parts) * blockDim.x + threadIdx.x) * 8, n = p.I - at;
+    if (n <= 0) return;
+    const size_t from = static_cast<size_t>(row) * p.I + at, slot = static_cast<size_t>(row) * groups + (static_cast<unsigned>(at) >> 7);
+    const bool whole = static_cast<size_t>(static_cast<unsigned>(p.rows) - 1 - row) * p.I + n >= 8;
+    Raw8<false> d;
+    clear8(d);
+    load8<false, TAIL>(p.grad, from, n, whole, d);
+    const u32x2_any g8 = load8_bytes<TAIL>(p.gate8, from, n, whole), u8 = load8_bytes<TAIL>(p.up8, from, n, whole);
+    Grads8 o;
+    grads8<TAIL>(d, g8, u8, p.gate_descale[slot], p.up_descale[slot], n, o);
+    store8_bf16<TAIL>(p.grad_gate, row * p.ld + at, n, o.dg);
+    store8_bf16<TAIL>(p.grad_up, row * p.ld + at, n, o.du);
+    if (p.act) store8_bf16<TAIL>(p.act, from, n, o.a);
 }
 
 // rows r0..r3 hold bytes n0..n3; returns columns: c[j] = {r0.bj, r1.bj, r2.bj, r3.bj}
@@ -265,77 +244,95 @@ __device__ __forceinline__ void transpose4x4(uint32_t r0, uint32_t r1, uint32_t 
 
 typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
 
-// 8-bit outputs: a workgroup has 128 x 128 elements, a thread 8 x 8 of them, whose bytes it writes along the rows and, through LDS, along the columns.
-constexpr int kTile = 128;
+// 8-bit outputs: a workgroup has 128 x 128 elements, a thread four rows of eight of them, whose bytes it writes along the rows and, through LDS, along the columns.
+// LDS holds [column][128 bytes of rows] for each of the three outputs.  A wavefront's store instruction writes four bytes for each of 16 column blocks and four row blocks:
+// the 16-byte pieces of a column are xor-swizzled by the column block, and the upper eight blocks store their columns in swapped pairs, so that 64 lanes hit 64 banks.
+constexpr int kTile = 128, kTileThreads = 512;
 template <bool TAIL>
-__global__ __launch_bounds__(kThreads) void k_swiglu_grad8(const SwigluGradArgs p) {
-    __shared__ __attribute__((aligned(16))) uint8_t tile[kTile * kTile];      // [column][row]
+__global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradArgs p) {
+    __shared__ __attribute__((aligned(16))) uint8_t tile[3][kTile * kTile];
     __shared__ uint32_t sh[16];
-    const unsigned across = (static_cast<unsigned>(p.I) + kTile - 1) / kTile;
-    const unsigned r0 = blockIdx.x / across * kTile;
-    const int c0 = static_cast<int>(blockIdx.x % across) * kTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const unsigned across = (static_cast<unsigned>(p.I) + kTile - 1) / kTile, rows = p.rows;
+    const unsigned r0 = blockIdx.x / across * kTile, group = blockIdx.x % across;
+    const int c0 = static_cast<int>(group) * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int at = c0 + tx * 8, n = p.I - at;
-    const unsigned rows = p.rows;
-    const float s = *p.qscale, as = p.act8_t ? *p.act_qscale : 0.0f;
-    const bool s_finite = abs_bits(s) < kInf, as_finite = abs_bits(as) < kInf;
-    u32x2_any bytes[3][8];
+    float s = *p.qscale, as = p.act8_t ? *p.act_qscale : 0.0f;
+    const bool plain = abs_bits(s) < kInf && abs_bits(as) < kInf;
+    saturate_fp8(s);
+    saturate_fp8(as);
+    Raw8<false> d[4];
+    u32x2_any g8[4], u8[4], bytes[3][4];
+    float gs[4], us[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned row = r0 + ty * 4 + i;
+        clear8(d[i]);
+        g8[i] = u8[i] = u32x2_any{0, 0};
+        gs[i] = us[i] = 0.0f;
+        if (row < rows && n > 0) {
+            const size_t from = static_cast<size_t>(row) * p.I + at, slot = static_cast<size_t>(row) * across + group;
+            const bool whole = static_cast<size_t>(rows - 1 - row) * p.I + n >= 8;
+            load8<false, TAIL>(p.grad, from, n, whole, d[i]);
+            g8[i] = load8_bytes<TAIL>(p.gate8, from, n, whole);
+            u8[i] = load8_bytes<TAIL>(p.up8, from, n, whole);
+            gs[i] = p.gate_descale[slot];
+            us[i] = p.up_descale[slot];
+        }
+    }
     float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const unsigned row = r0 + ty * 8 + i;
-        bytes[0][i] = bytes[1][i] = bytes[2][i] = u32x2_any{0, 0};
-        if (row >= rows || n <= 0) continue;
-        const size_t from = static_cast<size_t>(row) * p.I + at, slot = static_cast<size_t>(row) * across + blockIdx.x % across;
-        const bool whole = static_cast<size_t>(rows - 1 - row) * p.I + n >= 8;
-        Raw8<false> d;
-        clear8(d);
-        load8<false, TAIL>(p.grad, from, n, whole, d);
-        const u32x2_any g8 = load8_bytes<TAIL>(p.gate8, from, n, whole), u8 = load8_bytes<TAIL>(p.up8, from, n, whole);
+    for (int i = 0; i < 4; ++i) {
+        const unsigned row = r0 + ty * 4 + i;
         Grads8 o;
-        grads8<TAIL>(d, g8, u8, p.gate_descale[slot], p.up_descale[slot], n, o);
-        uint32_t top = 0, act_top = 0;
+        grads8<TAIL>(d[i], g8[i], u8[i], gs[i], us[i], n, o);
+        float m = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (!TAIL || k < n) most = fmaxf(most, fmaxf(fabsf(o.dg[k]), fabsf(o.du[k])));
-            top = max(top, max(abs_bits(o.dg[k]), abs_bits(o.du[k])));
-            act_top = max(act_top, abs_bits(o.a[k]));
-        }
-        const bool finite = __all(top < kInf) && s_finite, act_finite = __all(act_top < kInf) && as_finite;
+        for (int k = 0; k < 8; ++k)
+            if (!TAIL || k < n) m = fmaxf(fmaxf(m, fabsf(o.dg[k])), fabsf(o.du[k]));
+        most = fmaxf(most, m);
+        const bool usual = plain && !__any(fmaxf(m, largest(o.a)) == __builtin_inff());
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             o.dg[k] *= s;
             o.du[k] *= s;
             o.a[k] *= as;
         }
-        bytes[0][i] = pack8_fp8(true, finite, o.dg);
-        bytes[1][i] = pack8_fp8(true, finite, o.du);
-        bytes[2][i] = pack8_fp8(false, act_finite, o.a);
-        store8_bytes<TAIL>(p.grad8, static_cast<size_t>(row) * 2 * p.I + at, n, bytes[0][i]);
-        store8_bytes<TAIL>(p.grad8, static_cast<size_t>(row) * 2 * p.I + p.I + at, n, bytes[1][i]);
+        bytes[0][i] = usual ? convert8_fp8<true>(o.dg) : pack8_fp8(true, false, o.dg);
+        bytes[1][i] = usual ? convert8_fp8<true>(o.du) : pack8_fp8(true, false, o.du);
+        bytes[2][i] = usual ? convert8_fp8<false>(o.a) : pack8_fp8(false, false, o.a);
+        if (row < rows && n > 0) {
+            const size_t to = static_cast<size_t>(row) * 2 * p.I + at;
+            store8_bytes<TAIL>(p.grad8, to, n, bytes[0][i]);
+            store8_bytes<TAIL>(p.grad8, to + p.I, n, bytes[1][i]);
+        }
     }
+    auto out_of = [&](int part) { return part == 2 ? p.act8_t : p.grad8_t ? p.grad8_t + (part == 1 ? static_cast<size_t>(p.I) * rows : 0) : nullptr; };
+    const bool swap = tx & 8;
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
-        uint8_t* out = part == 2 ? p.act8_t : p.grad8_t ? p.grad8_t + (part == 1 ? static_cast<size_t>(p.I) * rows : 0) : nullptr;
-        if (!out) continue;             // the same in every thread
-        __syncthreads();
+        if (!out_of(part)) continue;            // the same in every thread
+        uint8_t* wr = tile[part] + tx * 8 * kTile + (((ty >> 2) ^ (tx & 7)) << 4) + (ty & 3) * 4;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            uint32_t lo[4], hi[4];
-            transpose4x4(bytes[part][0][half], bytes[part][1][half], bytes[part][2][half], bytes[part][3][half], lo);
-            transpose4x4(bytes[part][4][half], bytes[part][5][half], bytes[part][6][half], bytes[part][7][half], hi);
+            uint32_t c[4];
+            transpose4x4(bytes[part][0][half], bytes[part][1][half], bytes[part][2][half], bytes[part][3][half], c);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<uint2*>(&tile[(tx * 8 + half * 4 + k) * kTile + ty * 8]) = make_uint2(lo[k], hi[k]);
+            for (int k = 0; k < 4; ++k)          // instruction k stores column k ^ swap
+                *reinterpret_cast<uint32_t*>(wr + (half * 4 + (k ^ (swap ? 1 : 0))) * kTile) = swap ? c[k ^ 1] : c[k];
         }
-        __syncthreads();
-        const int chunk = threadIdx.x & 7, rr = threadIdx.x >> 3;       // 8 lanes cover one 128-byte output row
+    }
+    __syncthreads();
+    const int chunk = threadIdx.x & 7, rr = threadIdx.x >> 3;       // 8 lanes cover one 128-byte output row
+    const unsigned row = r0 + chunk * 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = i * 32 + rr;
-            const unsigned row = r0 + chunk * 16;
+    for (int part = 0; part < 3; ++part) {
+        uint8_t* out = out_of(part);
+        if (!out) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = i * 64 + rr;
             if (c0 + c >= p.I || row >= rows) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(&tile[c * kTile + chunk * 16]);
+            const uint4 v = *reinterpret_cast<const uint4*>(&tile[part][c * kTile + ((chunk ^ ((c >> 3) & 7)) << 4)]);
             uint8_t* to = out + static_cast<size_t>(c0 + c) * rows + row;
             if (!TAIL || row + 16 <= rows) {
                 __builtin_nontemporal_store(u32x4_byte{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_byte*>(to));
@@ -347,33 +344,39 @@ __global__ __launch_bounds__(kThreads) void k_swiglu_grad8(const SwigluGradArgs 
             }
         }
     }
-    __syncthreads();
     const uint32_t m = row_max<false>(__float_as_uint(most), sh);
-    if (threadIdx.x == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
+    if (threadIdx.x == 0) {
+        float before;
+        raise_first(p.amax, m, blockIdx.x, gridDim.x, before);
+        raise_last(p.amax, m, blockIdx.x, gridDim.x, before);
+    }
 }
 
-// the groups of a launch and, at 16 a workgroup, its workgroups: a few for each CU, which walk over the rest
-constexpr unsigned kWalkers = 2048;
-unsigned rows_of_launch(int I) { return (1u << 30) / (static_cast<unsigned>(I + 127) / 128); }
-unsigned walkers(unsigned rows, int I) {
-    const size_t groups = static_cast<size_t>(rows) * ((I + 127) / 128);
-    const unsigned blocks = ceil_div(groups, kThreads / 16);
-    return blocks < kWalkers ? blocks : kWalkers;
+// Workgroups of a row with V chunks a thread, and their threads.
+struct Parts { unsigned parts, threads; };
+Parts row_parts(int I, int V) {
+    const unsigned chunks = (static_cast<unsigned>(I) + 7) / 8, most = kKeepThreads * V, parts = (chunks + most - 1) / most;
+    const unsigned each = (chunks + parts * V - 1) / (parts * V);
+    return {parts, (each + kWave - 1) / kWave * kWave};
 }
+// rows of a launch: fewer than 2^32 threads
+unsigned launch_rows(unsigned parts) { return parts < (kLaunchRows >> 1) ? (kLaunchRows << 1) / parts : 1; }
 
 template <int QMODE, bool TAIL>
 int launch_keep(SwigluKeepArgs p, hipStream_t st) {
-    const unsigned rows = p.rows, most = QMODE == Q_ROWS ? kLaunchRows : rows_of_launch(p.I);
+    const int V = QMODE == Q_ROWS ? 1 : KEEPV;
+    const Parts cut = QMODE == Q_ROWS ? Parts{1, 0} : row_parts(p.I, V);
+    p.parts = cut.parts;
+    const unsigned rows = p.rows, most = QMODE == Q_ROWS ? kLaunchRows : launch_rows(cut.parts);
     for (p.row0 = 0; p.row0 < rows; p.row0 += most) {
         const unsigned n = rows - p.row0 < most ? rows - p.row0 : most;
-        p.row_end = p.row0 + n;
         if constexpr (QMODE == Q_ROWS) {
-            if (p.I <= kOneWaveH) k_swiglu_keep_rows<TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
-            else if (p.I <= kOneChunkH) k_swiglu_keep_rows<TAIL, false, 1><<<n, row_threads(p.I, 1), 0, st>>>(p);
-            else if (p.I <= 2 * kOneChunkH) k_swiglu_keep_rows<TAIL, false, 2><<<n, row_threads(p.I, 2), 0, st>>>(p);
-            else k_swiglu_keep_rows<TAIL, false, 4><<<n, row_threads(p.I, 4), 0, st>>>(p);
+            if (p.I <= kOneWaveH) k_swiglu_keep<QMODE, TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
+            else if (p.I <= kOneChunkH) k_swiglu_keep<QMODE, TAIL, false, 1><<<n, row_threads(p.I, 1), 0, st>>>(p);
+            else if (p.I <= 2 * kOneChunkH) k_swiglu_keep<QMODE, TAIL, false, 2><<<n, row_threads(p.I, 2), 0, st>>>(p);
+            else k_swiglu_keep<QMODE, TAIL, false, 4><<<n, row_threads(p.I, 4), 0, st>>>(p);
         } else {
-            k_swiglu_keep<QMODE, TAIL><<<walkers(n, p.I), kThreads, 0, st>>>(p);
+            k_swiglu_keep<QMODE, TAIL, false, KEEPV><<<n * cut.parts, cut.threads, 0, st>>>(p);
         }
     }
     return launch_status();
@@ -457,12 +460,13 @@ int cf_swiglu_ckpt8_backward(const uint16_t* d_grad_out, const void* d_gate8, co
     if (!d_grad_gate || !d_grad_up || misaligned(d_grad_gate, 2) || misaligned(d_grad_up, 2) || misaligned(d_act, 2)) return CF_ERR_INVALID_ARG;
     p.grad_gate = d_grad_gate; p.grad_up = d_grad_up; p.ld = static_cast<size_t>(ld); p.act = d_act;
     hipStream_t st = as_stream(stream);
-    const unsigned most = rows_of_launch(I), all = rows;
+    const Parts cut = row_parts(I, 1);
+    p.parts = cut.parts;
+    const unsigned most = launch_rows(cut.parts), all = rows;
     for (p.row0 = 0; p.row0 < all; p.row0 += most) {
         const unsigned n = all - p.row0 < most ? all - p.row0 : most;
-        p.row_end = p.row0 + n;
-        if (I % 8 != 0) k_swiglu_grad<true><<<walkers(n, I), kThreads, 0, st>>>(p);
-        else k_swiglu_grad<false><<<walkers(n, I), kThreads, 0, st>>>(p);
+        if (I % 8 != 0) k_swiglu_grad<true><<<n * cut.parts, cut.threads, 0, st>>>(p);
+        else k_swiglu_grad<false><<<n * cut.parts, cut.threads, 0, st>>>(p);
     }
     return launch_status();
 }
@@ -479,9 +483,9 @@ int cf_swiglu_ckpt8_backward_quant_e5m2(const uint16_t* d_grad_out, const void* 
     p.grad8 = static_cast<uint8_t*>(d_grad8); p.grad8_t = static_cast<uint8_t*>(d_grad8_t); p.act8_t = static_cast<uint8_t*>(d_act8_t);
     p.qscale = d_qscale; p.amax = d_amax; p.act_qscale = d_act_qscale;
     const size_t tiles = static_cast<size_t>(ceil_div(rows, kTile)) * ceil_div(I, kTile);
-    if (tiles * kThreads >= (static_cast<size_t>(1) << 32)) return CF_ERR_UNSUPPORTED;         // a terabyte of gradients
-    if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true><<<static_cast<unsigned>(tiles), kThreads, 0, as_stream(stream)>>>(p);
-    else k_swiglu_grad8<false><<<static_cast<unsigned>(tiles), kThreads, 0, as_stream(stream)>>>(p);
+    if (tiles * kTileThreads >= (static_cast<size_t>(1) << 32)) return CF_ERR_UNSUPPORTED;         // a terabyte of gradients
+    if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true><<<static_cast<unsigned>(tiles), kTileThreads, 0, as_stream(stream)>>>(p);
+    else k_swiglu_grad8<false><<<static_cast<unsigned>(tiles), kTileThreads, 0, as_stream(stream)>>>(p);
     return launch_status();
 }
 

@@ -1,19 +1,48 @@
 """GPU: the gated activation with its 8-bit operand and its 8-bit checkpoints, and the gradient from those, against the formulas in 64 bits.
 
 Tolerances.  u = 2^-24.  The checkpoints are compared bit for bit: a group's maximum is a bf16 value, 448 / amax, amax / 448 and the product with the scale are one fp32 rounding each.
-The sigmoid: exponent argument, exponential (1 ulp), addition and reciprocal (1 ulp) stay below 10 u where |g| <= 87; the activation adds two products: 12 u.  Below -87 it is
-taken as zero, which is off by 87 e^-87 |u| < 2e-36 |u|.  On top comes the rounding to the output's type: bf16 2^-8, E4M3 2^-4 or half of its smallest step, E5M2 2^-3 or half of its."""
+The sigmoid s of g is 1 / (1 + e), e = 2^t, t = -g log2(e).  t is rounded once and its constant is off by 0.22 u: 1.22 u |t|, which moves e by ln 2 times
+that, 1.22 u |g|; the exponential adds 2 u.  In s these count (1 - s) times, the addition 1 u, the reciprocal 2 u: s is off by (5 + 1.22 |g| (1 - s)) u at most, here
+(6 + 2 |g| (1 - s)) u =: sig.  The activation adds two products.  Where e leaves fp32 (g < -87) s is zero, off by 87 e^-87 |u| < 2e-36 |u| in the activation.  On top comes the rounding to the
+output's type: bf16 2^-8, E4M3 2^-4 or half of its smallest step, E5M2 2^-3 or half of its."""
 import pytest
 import torch
 
 from gpu_util import case, stream
-from test_gpu_add_norm import U, Out, rows_of, shifted
-from test_gpu_gated_norm import check_quantized
+from test_gpu_add_norm import F8, U, Out, rows_of, shifted
 
 pytestmark = pytest.mark.gpu
 
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
-A = 12 * U
+
+
+def activation(g, u):
+    """(a, how far it may be off) in 64 bits."""
+    g, u = g.double(), u.double()
+    s = torch.sigmoid(g)
+    a = s * g * u
+    return a, a.abs() * U * (9 + 2 * g.abs() * (1 - s)) + 2e-36 * u.abs() * (g < -86)
+
+
+def check_quantized(got, a, off, form, e5m2, qscale):
+    dtype, top, half, least = F8[e5m2]
+    if form == "record":
+        m = max(0.125, float(a.abs().max()))
+        assert abs(got["amax"] - m) <= float(off.max()) + U * m
+        scale, rel = torch.full_like(a[:, :1], qscale), torch.zeros_like(a[:, :1])
+    else:
+        width = 128 if form == "block" else a.shape[1]
+        parts = lambda t: torch.stack([p.abs().amax(1) for p in t.split(width, 1)], 1)  # noqa: E731
+        m = parts(a).clamp_min(1e-12)
+        rel = parts(off) / m + 3 * U            # a maximum is off by the largest of its elements' errors; then a division
+        assert torch.all((got["scale"].double().view(m.shape) * m / top - 1).abs() <= 1.01 * rel)
+        assert torch.all((got["descale"].double().view(m.shape) * top / m - 1).abs() <= 1.01 * rel)
+        spread = lambda t: t.repeat_interleave(width, 1)[:, :a.shape[1]]  # noqa: E731
+        scale, rel = spread(top / m), spread(rel)
+    v = (a * scale).clamp(-top, top)
+    q = got["q"].view(dtype).double()
+    assert torch.all((q - v).abs() <= torch.maximum(half * v.abs(), torch.tensor(least, dtype=torch.float64)) + 1.1 * (off * scale + (rel + 2 * U) * v.abs()))
+
 
 
 def groups_of(t):
@@ -69,8 +98,7 @@ def check_forward(got, g, u, form, e5m2, qscale=3.0):
         q, d = checkpoint(t)
         assert torch.equal(got[name + "_descale"], d), name
         assert torch.equal(got[name], q.view(torch.uint8)), name
-    a = torch.sigmoid(g.double()) * g.double() * u.double()
-    check_quantized(got, a, form, e5m2, qscale, A)
+    check_quantized(got, *activation(g, u), form, e5m2, qscale)
 
 
 FORMS = [("rows", 0), ("rows", 1), ("block", 0), ("record", 0), ("record", 1)]
@@ -111,8 +139,7 @@ def test_forward_far_gates(cf, dev, form):
     u = torch.full((2, 512), 0.5).to(torch.bfloat16)
     u[1] = 1e-3
     got = forward(cf, dev, g, u, form)
-    a = torch.sigmoid(g.double()) * g.double() * u.double()
-    check_quantized(got, a, form, 0, 3.0, A)
+    check_quantized(got, *activation(g, u), form, 0, 3.0)
     far = torch.tensor([[-3.38e38, -1e30, -1000.0, -88.0, 1000.0, 88.0, 1e30, 0.0]]).to(torch.bfloat16)
     got = forward(cf, dev, far, torch.full((1, 8), 1e-6).to(torch.bfloat16), "record", qscale=1.0)
     assert not torch.isnan(got["q"].view(E4M3).float()).any() and torch.all(got["q"].view(E4M3).float()[0, :4] == 0)
@@ -157,12 +184,14 @@ class Grad:
         g, u, d = restored(self.g8, self.gd), restored(self.u8, self.ud), self.do.double()
         s = torch.sigmoid(g)
         slope = s * (1 + g * (1 - s))
-        # 1 - s is off by 11 u s + u, the factors by 10 u and a few u; the decoded values by one rounding each, under which silu and its slope move by 2 u (|g| + 1)
-        slope_off = 14 * U * slope.abs() + s * g.abs() * (11 * U * s + U) + 4 * U * s * (1 + g.abs() * (1 - s)) + 2 * U * g.abs()
+        # 1 - s is off by s sig + u (1 - s), g times that and an fma's rounding by |g| so much more; the decoded values by one rounding each, under which silu and its slope
+        # move by 2 u (|g| + 1)
+        sig = U * (6 + 2 * g.abs() * (1 - s))
+        slope_off = (sig + 2 * U) * slope.abs() + s * (g.abs() * (sig * s + U * (1 - s)) + 2 * U * (1 + g * (1 - s)).abs()) + 2 * U * g.abs()
         dg, du, a = d * u * slope, d * g * s, g * s * u
         drift, far = 2 * U * (1 + g.abs()), 2e-36 * (g < -86)
-        return ((dg, (d * u).abs() * (slope_off + far) + 4 * U * dg.abs()), (du, (14 * U + drift) * du.abs() + far * d.abs()),
-                (a, (14 * U + drift) * a.abs() + far * u.abs()))
+        return ((dg, (d * u).abs() * (slope_off + far) + 4 * U * dg.abs()), (du, (sig + 4 * U + drift) * du.abs() + far * d.abs()),
+                (a, (sig + 4 * U + drift) * a.abs() + far * u.abs()))
 
 
 def backward(cf, dev, x, shift=0, pad=0, fused=False, with_act=True):
