@@ -105,7 +105,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_
             h[j][i] = __builtin_fmaf(p.res, value8<F32, TAIL>(r[j], i, left(j)), z);
             if constexpr (!F32) h[j][i] = round_bf16_hw(h[j][i]);
         }
-        if (p.sum && has(j)) store8_stream<F32, TAIL, true>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
+        if (p.sum && has(j)) store8_stream<F32, TAIL, !TAIL>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
     }
 
     const float rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum + 2, sh_max[3], e);

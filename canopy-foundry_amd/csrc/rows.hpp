@@ -147,10 +147,11 @@ __device__ __forceinline__ u32x2_any pack8_fp8(bool e5m2, bool finite, const flo
     }
     return o;
 }
-template <bool TAIL>
+template <bool TAIL, bool PAST_L2 = true>
 __device__ __forceinline__ void store8_bytes(uint8_t* p, size_t at, int n, u32x2_any o) {
     if (!TAIL || n >= 8) {
-        __builtin_nontemporal_store(o, reinterpret_cast<u32x2_any*>(p + at));
+        if constexpr (PAST_L2) __builtin_nontemporal_store(o, reinterpret_cast<u32x2_any*>(p + at));
+        else *reinterpret_cast<u32x2_any*>(p + at) = o;
     } else {
         typedef uint32_t u32_byte __attribute__((aligned(1)));
         typedef uint16_t u16_byte __attribute__((aligned(1)));

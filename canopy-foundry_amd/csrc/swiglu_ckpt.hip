@@ -4,6 +4,8 @@
 // Backward, with g and u from their bytes:  dg = dO * u * s * (1 + g * (1 - s)),  du = dO * g * s.
 #include "rows.hpp"
 
+#include <type_traits>
+
 namespace cf {
 namespace {
 
@@ -245,15 +247,22 @@ __device__ __forceinline__ void transpose4x4(uint32_t r0, uint32_t r1, uint32_t 
 typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
 
 // 8-bit outputs: a workgroup has 128 x 128 elements, a thread four rows of eight of them, whose bytes it writes along the rows and, through LDS, along the columns.
+// Pieces that are whole 128-byte lines leave past the L2 (8192 x 14336: 213 us, 223 through it); where they are not (WHOLE_ROWS: of the straight outputs, WHOLE_LINES: of the transposed), the
+// L2 puts a line together from neighbouring tiles, which is why one XCD has them: 8191 x 8192 240 us past it, 153 through it, 162 with the tiles in row-major order over all XCDs.
 // LDS holds [column][128 bytes of rows] for each of the three outputs.  A wavefront's store instruction writes four bytes for each of 16 column blocks and four row blocks:
 // the 16-byte pieces of a column are xor-swizzled by the column block, and the upper eight blocks store their columns in swapped pairs, so that 64 lanes hit 64 banks.
 constexpr int kTile = 128, kTileThreads = 512;
-template <bool TAIL>
+template <bool TAIL, bool WHOLE_ROWS, bool WHOLE_LINES>
 __global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t tile[3][kTile * kTile];
     __shared__ uint32_t sh[16];
-    const unsigned across = (static_cast<unsigned>(p.I) + kTile - 1) / kTile, rows = p.rows;
-    const unsigned r0 = blockIdx.x / across * kTile, group = blockIdx.x % across;
+    // the eight XCDs, which take workgroups in turn, each have an eighth of the tiles, in strips of a few column tiles and down the rows within one
+    const unsigned across = (static_cast<unsigned>(p.I) + kTile - 1) / kTile, rows = p.rows, down = (rows + kTile - 1) / kTile;
+    const unsigned total = across * down, each = (total + 7) / 8, index = blockIdx.x % 8 * each + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= each || index >= total) return;
+    constexpr unsigned kStrip = WHOLE_LINES ? 8 : 4;
+    const unsigned strip = index / (kStrip * down) * kStrip, rest = index % (kStrip * down), wide = across - strip < kStrip ? across - strip : kStrip;
+    const unsigned r0 = rest / wide * kTile, group = strip + rest % wide;
     const int c0 = static_cast<int>(group) * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int at = c0 + tx * 8, n = p.I - at;
     float s = *p.qscale, as = p.act8_t ? *p.act_qscale : 0.0f;
@@ -302,8 +311,8 @@ __global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradA
         bytes[2][i] = usual ? convert8_fp8<false>(o.a) : pack8_fp8(false, false, o.a);
         if (row < rows && n > 0) {
             const size_t to = static_cast<size_t>(row) * 2 * p.I + at;
-            store8_bytes<TAIL>(p.grad8, to, n, bytes[0][i]);
-            store8_bytes<TAIL>(p.grad8, to + p.I, n, bytes[1][i]);
+            store8_bytes<TAIL, WHOLE_ROWS>(p.grad8, to, n, bytes[0][i]);
+            store8_bytes<TAIL, WHOLE_ROWS>(p.grad8, to + p.I, n, bytes[1][i]);
         }
     }
     auto out_of = [&](int part) { return part == 2 ? p.act8_t : p.grad8_t ? p.grad8_t + (part == 1 ? static_cast<size_t>(p.I) * rows : 0) : nullptr; };
@@ -335,7 +344,8 @@ __global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradA
             const uint4 v = *reinterpret_cast<const uint4*>(&tile[part][c * kTile + ((chunk ^ ((c >> 3) & 7)) << 4)]);
             uint8_t* to = out + static_cast<size_t>(c0 + c) * rows + row;
             if (!TAIL || row + 16 <= rows) {
-                __builtin_nontemporal_store(u32x4_byte{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_byte*>(to));
+                if constexpr (WHOLE_LINES) __builtin_nontemporal_store(u32x4_byte{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_byte*>(to));
+                else *reinterpret_cast<u32x4_byte*>(to) = u32x4_byte{v.x, v.y, v.z, v.w};
             } else {
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -484,8 +494,17 @@ int cf_swiglu_ckpt8_backward_quant_e5m2(const uint16_t* d_grad_out, const void* 
     p.qscale = d_qscale; p.amax = d_amax; p.act_qscale = d_act_qscale;
     const size_t tiles = static_cast<size_t>(ceil_div(rows, kTile)) * ceil_div(I, kTile);
     if (tiles * kTileThreads >= (static_cast<size_t>(1) << 32)) return CF_ERR_UNSUPPORTED;         // a terabyte of gradients
-    if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true><<<static_cast<unsigned>(tiles), kTileThreads, 0, as_stream(stream)>>>(p);
-    else k_swiglu_grad8<false><<<static_cast<unsigned>(tiles), kTileThreads, 0, as_stream(stream)>>>(p);
+    const unsigned grid = (static_cast<unsigned>(tiles) + 7) / 8 * 8;
+    hipStream_t st = as_stream(stream);
+    auto go = [&](auto rows_whole, auto lines_whole) {
+        constexpr bool ROWS = decltype(rows_whole)::value, LINES = decltype(lines_whole)::value;
+        if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+        else k_swiglu_grad8<false, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    if (I % kTile == 0) rows % kTile == 0 ? go(yes, yes) : go(yes, no);
+    else rows % kTile == 0 ? go(no, yes) : go(no, no);
     return launch_status();
 }
 
