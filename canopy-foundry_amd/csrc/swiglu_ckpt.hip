@@ -10,9 +10,6 @@ namespace cf {
 namespace {
 
 constexpr int kKeepThreads = 512;
-#ifndef KEEPV
-#define KEEPV 1
-#endif
 constexpr int kMaxRow = 32768;              // of the form that holds a whole row
 
 // sigmoid(g), by the two units' instructions (1 ulp each).  The rounding of the exponent's argument costs e^-g a relative 1.2 |g| 2^-24, so the result is off by
@@ -31,7 +28,7 @@ struct SwigluKeepArgs {
     float* amax;
     int rows, I;
     unsigned row0;                  // the launch's first row
-    unsigned parts;                 // workgroups of a row
+    unsigned parts, turns, total;   // pieces of a row, pieces that a workgroup takes, pieces of all the launch's rows
     int e5m2;
 };
 
@@ -72,7 +69,7 @@ __device__ __forceinline__ float largest(const float (&a)[8]) {
 // What has been divided by its own maximum needs no clamp.
 template <int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThreads) void k_swiglu_keep(const SwigluKeepArgs p) {
-    __shared__ uint32_t sh[16];
+    __shared__ uint32_t sh[2][16];
     const int T = ONE_WAVE ? kWave : blockDim.x;
     unsigned row, part = 0;
     int t = threadIdx.x;
@@ -83,29 +80,30 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
     } else if constexpr (QMODE == Q_ROWS) {
         row = p.row0 + blockIdx.x;
     } else {
-        row = p.row0 + blockIdx.x / p.parts;
-        part = blockIdx.x % p.parts;
+        const unsigned index = blockIdx.x * (QMODE == Q_RECORD ? p.turns : 1);
+        row = p.row0 + index / p.parts;
+        part = index % p.parts;
     }
     const unsigned groups = (static_cast<unsigned>(p.I) + 127) / 128;
-    const size_t base = static_cast<size_t>(row) * p.I, slots = static_cast<size_t>(row) * groups;
-    const int lane = threadIdx.x & 15, first = part * T * V + t;
-    auto at = [&](int j) { return (first + j * T) * 8; };
-    auto left = [&](int j) { return p.I - at(j); };
+    const int lane = threadIdx.x & 15;
+    auto at = [&](unsigned piece, int j) { return (static_cast<int>(piece) * T * V + t + j * T) * 8; };
 
     Raw8<false> g[V], u[V];
+    auto load = [&] {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        clear8(g[j]);
-        clear8(u[j]);
-        if (left(j) > 0) {
-            const size_t from = row * p.ld + at(j);
-            const bool whole = static_cast<size_t>(static_cast<unsigned>(p.rows) - 1 - row) * p.ld + left(j) >= 8;       // eight elements from here on in the tensor
-            load8<false, TAIL>(p.gate, from, left(j), whole, g[j]);
-            load8<false, TAIL>(p.up, from, left(j), whole, u[j]);
-            cut<TAIL>(g[j], left(j));
-            cut<TAIL>(u[j], left(j));
+        for (int j = 0; j < V; ++j) {
+            const int n = p.I - at(part, j);
+            clear8(g[j]);
+            clear8(u[j]);
+            if (n > 0) {
+                const size_t from = row * p.ld + at(part, j);
+                const bool whole = static_cast<size_t>(static_cast<unsigned>(p.rows) - 1 - row) * p.ld + n >= 8;       // eight elements from here on in the tensor
+                load8<false, TAIL>(p.gate, from, n, whole, g[j]);
+                load8<false, TAIL>(p.up, from, n, whole, u[j]);
+            }
         }
-    }
+    };
+    load();
     const bool e5m2 = QMODE != Q_BLOCK && p.e5m2;
     const float F = e5m2 ? 57344.0f : 448.0f;
     float qs = 0.0f;
@@ -114,16 +112,22 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
         saturate_fp8(qs);
     }
     float a[QMODE == Q_ROWS ? V : 1][8], most = 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        float (&o)[8] = a[QMODE == Q_ROWS ? j : 0];
+    // the descale that this lane writes; the pointers in registers, or the compiler loads the one that is chosen, and waits for it
+    float *descale = p.gate_descale, *second = p.up_descale, *third = p.descale;
+    asm volatile("" : "+s"(descale), "+s"(second), "+s"(third));
+    descale = lane == 0 ? descale : lane == 4 ? second : third;
+    auto chunk = [&](Raw8<false> gate, Raw8<false> up, float (&o)[8], unsigned in_row, unsigned piece, int j) {
+        const int from = at(piece, j), n = p.I - from;
+        const size_t to = static_cast<size_t>(in_row) * p.I + from, slot = static_cast<size_t>(in_row) * groups + (static_cast<unsigned>(from) >> 7);
+        cut<TAIL>(gate, n);
+        cut<TAIL>(up, n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float v = g[j].at(i);
-            o[i] = v * sigmoid(v) * u[j].at(i);
+            const float v = gate.at(i);
+            o[i] = v * sigmoid(v) * up.at(i);
         }
         float m = largest(o);
-        const float mg = group_max(g[j]), mu = group_max(u[j]);
+        const float mg = group_max(gate), mu = group_max(up);
         float one = lane < 4 ? mg : mu;
         if constexpr (QMODE == Q_BLOCK) {
             m = __uint_as_float(max16(__float_as_uint(m)));
@@ -131,19 +135,18 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
         }
         one = fmaxf(one, 1e-12f);
         const float s = 448.0f / one, d = one / 448.0f;
-        const size_t slot = slots + (static_cast<unsigned>(at(j)) >> 7);
-        if ((lane & 3) == 0 && lane < (QMODE == Q_BLOCK ? 12 : 8) && left(j) > -8 * lane) {
-            (lane == 0 ? p.gate_descale : lane == 4 ? p.up_descale : p.descale)[slot] = d;
+        if ((lane & 3) == 0 && lane < (QMODE == Q_BLOCK ? 12 : 8) && n > -8 * lane) {         // the group's first element is there
+            descale[slot] = d;
             if (QMODE == Q_BLOCK && lane == 8) p.scale[slot] = s;
         }
         const float sg = from_lane<0>(s), su = from_lane<4>(s);
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = g[j].at(i) * sg;
-        if (left(j) > 0) store8_bytes<TAIL>(p.gate8, base + at(j), left(j), convert8_fp8<false>(v));
+        for (int i = 0; i < 8; ++i) v[i] = gate.at(i) * sg;
+        if (n > 0) store8_bytes<TAIL>(p.gate8, to, n, convert8_fp8<false>(v));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = u[j].at(i) * su;
-        if (left(j) > 0) store8_bytes<TAIL>(p.up8, base + at(j), left(j), convert8_fp8<false>(v));
+        for (int i = 0; i < 8; ++i) v[i] = up.at(i) * su;
+        if (n > 0) store8_bytes<TAIL>(p.up8, to, n, convert8_fp8<false>(v));
         most = fmaxf(most, m);
         if constexpr (QMODE != Q_ROWS) {
             const float sa = QMODE == Q_BLOCK ? from_lane<8>(s) : qs;
@@ -152,11 +155,42 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
             u32x2_any b;
             if (QMODE == Q_RECORD && (__any(m == __builtin_inff()) || abs_bits(qs) >= kInf)) b = pack8_fp8(e5m2, false, v);
             else b = e5m2 ? convert8_fp8<true>(v) : convert8_fp8<false>(v);
-            if (left(j) > 0) store8_bytes<TAIL>(p.q, base + at(j), left(j), b);
+            if (n > 0) store8_bytes<TAIL>(p.q, to, n, b);
         }
+    };
+    if constexpr (QMODE == Q_RECORD) {
+        const unsigned turns = p.total - blockIdx.x * p.turns < p.turns ? p.total - blockIdx.x * p.turns : p.turns;
+        for (unsigned turn = 0; turn < turns; ++turn) {
+            const Raw8<false> now_g = g[0], now_u = u[0];
+            const unsigned now_row = row, now_part = part;
+            if (turn + 1 < turns) {
+                const unsigned index = blockIdx.x * p.turns + turn + 1;
+                row = p.row0 + index / p.parts;
+                part = index % p.parts;
+                load();
+            }
+            chunk(now_g, now_u, a[0], now_row, now_part, 0);
+            if (turn == 0 && turns > 1 && blockIdx.x % 64 == 0) {
+                const uint32_t m = row_max<false>(__float_as_uint(most), sh[0]);
+                if (threadIdx.x == 0) atomic_max_nonneg(p.amax, __uint_as_float(m));
+            }
+        }
+        const uint32_t m = row_max<false>(__float_as_uint(most), sh[1]);
+        if (threadIdx.x == 0) {
+            if (turns > 1) {
+                atomic_max_nonneg(p.amax, __uint_as_float(m));
+            } else {
+                float before;
+                raise_first(p.amax, m, blockIdx.x, gridDim.x, before);
+                raise_last(p.amax, m, blockIdx.x, gridDim.x, before);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) chunk(g[j], u[j], a[QMODE == Q_ROWS ? j : 0], row, part, j);
     }
     if constexpr (QMODE == Q_ROWS) {
-        most = __uint_as_float(row_max<ONE_WAVE>(__float_as_uint(most), sh));
+        most = __uint_as_float(row_max<ONE_WAVE>(__float_as_uint(most), sh[0]));
         most = fmaxf(most, 1e-12f);
         const float s = F / most;
         if (t == 0) {
@@ -165,17 +199,10 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
+            const int n = p.I - at(0, j);
 #pragma unroll
             for (int i = 0; i < 8; ++i) a[j][i] *= s;
-            if (left(j) > 0) store8_bytes<TAIL>(p.q, base + at(j), left(j), e5m2 ? convert8_fp8<true>(a[j]) : convert8_fp8<false>(a[j]));
-        }
-    }
-    if constexpr (QMODE == Q_RECORD) {
-        const uint32_t m = row_max<false>(__float_as_uint(most), sh);
-        if (threadIdx.x == 0) {
-            float before;
-            raise_first(p.amax, m, blockIdx.x, gridDim.x, before);
-            raise_last(p.amax, m, blockIdx.x, gridDim.x, before);
+            if (n > 0) store8_bytes<TAIL>(p.q, static_cast<size_t>(row) * p.I + at(0, j), n, e5m2 ? convert8_fp8<true>(a[j]) : convert8_fp8<false>(a[j]));
         }
     }
 }
@@ -372,10 +399,13 @@ Parts row_parts(int I, int V) {
 // rows of a launch: fewer than 2^32 threads
 unsigned launch_rows(unsigned parts) { return parts < (kLaunchRows >> 1) ? (kLaunchRows << 1) / parts : 1; }
 
+// Recording a maximum: a workgroup that takes two pieces in turn has one maximum to report where it had two, and one in 64 raises it after the first piece, before any
+// other looks.  8192 x 14336: one piece 154 to 159 us, two 145, three 149, four 154; as many workgroups as run at once 167; without a maximum 148.
+constexpr unsigned kTurnPieces = 4096;
+
 template <int QMODE, bool TAIL>
 int launch_keep(SwigluKeepArgs p, hipStream_t st) {
-    const int V = QMODE == Q_ROWS ? 1 : KEEPV;
-    const Parts cut = QMODE == Q_ROWS ? Parts{1, 0} : row_parts(p.I, V);
+    const Parts cut = QMODE == Q_ROWS ? Parts{1, 0} : row_parts(p.I, 1);
     p.parts = cut.parts;
     const unsigned rows = p.rows, most = QMODE == Q_ROWS ? kLaunchRows : launch_rows(cut.parts);
     for (p.row0 = 0; p.row0 < rows; p.row0 += most) {
@@ -386,7 +416,9 @@ int launch_keep(SwigluKeepArgs p, hipStream_t st) {
             else if (p.I <= 2 * kOneChunkH) k_swiglu_keep<QMODE, TAIL, false, 2><<<n, row_threads(p.I, 2), 0, st>>>(p);
             else k_swiglu_keep<QMODE, TAIL, false, 4><<<n, row_threads(p.I, 4), 0, st>>>(p);
         } else {
-            k_swiglu_keep<QMODE, TAIL, false, KEEPV><<<n * cut.parts, cut.threads, 0, st>>>(p);
+            p.total = n * cut.parts;
+            p.turns = QMODE == Q_RECORD && p.total >= kTurnPieces ? 2 : 1;
+            k_swiglu_keep<QMODE, TAIL, false, 1><<<(p.total - 1) / p.turns + 1, cut.threads, 0, st>>>(p);
         }
     }
     return launch_status();
