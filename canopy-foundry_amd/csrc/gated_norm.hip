@@ -40,7 +40,8 @@ __device__ __forceinline__ float pair_at(const u32x4_any& v, int i) { return (i 
 // One row in registers, V chunks of eight elements a thread, as k_add_norm holds it: everything is read and written once.
 template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_norm(const GatedNormArgs p) {
-    __shared__ float sh_sum[4][16];
+    __shared__ double sh_post[2][16];
+    __shared__ float sh_sum[2][16];
     __shared__ uint32_t sh_max[4][16];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     unsigned row = p.row0 + blockIdx.x;
@@ -81,41 +82,48 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[j][i] = value8<false, TAIL>(x[j], i, left(j));
     }
-    // the checkpoint of a normalised row: its values are finite where its root mean square is, and not zero
-    auto keep = [&](uint8_t* to, int j, float inv, bool finite) {
+    // the checkpoint of eight normalised values, none of which is above sqrt(H) but by roundings
+    auto keep = [&](uint8_t* to, int j, float scale) {
         if (!to || !has(j)) return;
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = h[j][i] * inv * p.kept;
-        store8_fp8<TAIL>(to, base + (t + j * T) * 8, left(j), false, finite, v);
+        for (int i = 0; i < 8; ++i) v[i] = h[j][i] * scale;
+        store8_bytes<TAIL>(to, base + (t + j * T) * 8, left(j), convert8_fp8<false>(v));
     };
-    auto is_number = [](float rms) { return rms > 0.0f && rms < __builtin_inff(); };
 
+    // Each operation up to h is rounded to fp32 as it is written, and the root mean square comes from the threads' sums added in 64 bits, so that h has the bits that the formula
+    // has in fp32: a bf16 stream takes the next value where h lies next to the border of two, and through the maximum of a group one such value can be all of a scale's
+    // difference (some 160 of 7 million values lie there).  x / px is x times the inverse and a correction by what that leaves.
     int e;
-    const float post_rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum, sh_max[2], e);
+    const float post_rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_post, sh_max[2], e);
     if (t == 0 && p.post_rms) p.post_rms[row] = ldexpf(post_rms, e);
-    const float post_inv = 1.0f / post_rms;
+    const float post_inv = 1.0f / post_rms, divisor = post_rms < __builtin_inff() ? post_rms : 0.0f;         // infinite: 0 or NaN
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        keep(p.x8, j, post_inv, is_number(post_rms));
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float z = h[j][i] * post_inv * pair_at(wp[j], i);
+            const float q = h[j][i] * post_inv;
+            h[j][i] = __builtin_fmaf(__builtin_fmaf(-q, divisor, h[j][i]), post_inv, q);
+        }
+        keep(p.x8, j, p.kept);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float z = h[j][i] * pair_at(wp[j], i);
             if (gates) z *= pair_at(gate[j], i);
-            h[j][i] = __builtin_fmaf(p.res, value8<F32, TAIL>(r[j], i, left(j)), z);
+            h[j][i] = p.res * value8<F32, TAIL>(r[j], i, left(j)) + z;
             if constexpr (!F32) h[j][i] = round_bf16_hw(h[j][i]);
         }
         if (p.sum && has(j)) store8_stream<F32, TAIL, !TAIL>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
     }
 
-    const float rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum + 2, sh_max[3], e);
+    const float rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum, sh_max[3], e);
     if (t == 0 && p.rms) p.rms[row] = ldexpf(rms, e);
     const float inv = 1.0f / rms;
     const float F = p.e5m2 ? 57344.0f : 448.0f;
     uint32_t top[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        keep(p.sum8, j, inv, is_number(rms));
+        keep(p.sum8, j, inv * p.kept);
         top[j] = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

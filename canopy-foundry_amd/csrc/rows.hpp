@@ -244,12 +244,39 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* sh) {
 constexpr uint32_t kInf = 0x7f800000u;
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// Over a row's threads in 64 bits, as row_sum().
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint64_t lo = dpp<CTRL>(static_cast<uint32_t>(b)), hi = dpp<CTRL>(static_cast<uint32_t>(b >> 32));
+    return __builtin_bit_cast(double, hi << 32 | lo);
+}
+__device__ __forceinline__ double add16(double v) {
+    v += dpp64<0xb1>(v);
+    v += dpp64<0x4e>(v);
+    v += dpp64<0x141>(v);
+    return v + dpp64<0x140>(v);
+}
+template <bool ONE_WAVE>
+__device__ __forceinline__ double row_sum(double v, double* sh) {
+    v = add16(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    if constexpr (!ONE_WAVE) {
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int w = threadIdx.x & 15;
+        v = add16(w < static_cast<int>(blockDim.x >> 6) ? sh[w] : 0.0);
+    }
+    return v;
+}
+
 // The root mean square of a row that its threads hold in chunks of eight, V each: sqrt(mean(h^2) + eps) = 2^e times what is returned, with the row scaled by
 // 2^-e, which h / rms does not see.  e is 0 but where squares leave fp32 (|h| of 1e19 and more, or of 1e-15 and less under as small an eps): then the sum is taken once
-// more of the scaled row.  A row that holds infinities or NaNs stays as it is.  `sh`: two sums, `sh_max`: one maximum, as row_sum() and row_max() ask.
-template <bool ONE_WAVE, int V>
-__device__ __forceinline__ float row_rms(float (&h)[V][8], int H, float eps, float (*sh)[16], uint32_t* sh_max, int& e) {
-    auto mean_square = [&](float* s) {
+// more of the scaled row.  A row that holds infinities or NaNs stays as it is.  SUM: the type in which the threads' sums are added up.  `sh`: two sums, `sh_max`: one maximum, as row_sum() and row_max() ask.
+template <bool ONE_WAVE, int V, typename SUM>
+__device__ __forceinline__ float row_rms(float (&h)[V][8], int H, float eps, SUM (*sh)[16], uint32_t* sh_max, int& e) {
+    auto mean_square = [&](SUM* s) {
         float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -258,11 +285,11 @@ __device__ __forceinline__ float row_rms(float (&h)[V][8], int H, float eps, flo
             for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[j][i], h[j][i], part);
             ss += part;
         }
-        return row_sum<ONE_WAVE>(ss, s) / static_cast<float>(H);
+        return row_sum<ONE_WAVE>(static_cast<SUM>(ss), s) / static_cast<SUM>(H);
     };
-    float mean = mean_square(sh[0]) + eps;
+    SUM mean = mean_square(sh[0]) + eps;
     e = 0;
-    if (!(mean >= 1e-30f && mean < __builtin_inff())) {
+    if (!(mean >= static_cast<SUM>(1e-30f) && mean < static_cast<SUM>(__builtin_inff()))) {
         uint32_t m = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -279,7 +306,8 @@ __device__ __forceinline__ float row_rms(float (&h)[V][8], int H, float eps, flo
             mean = mean_square(sh[1]) + ldexpf(eps, -2 * e);
         }
     }
-    return sqrtf(mean);
+    if constexpr (sizeof(SUM) == 8) return static_cast<float>(sqrt(mean));
+    else return sqrtf(mean);
 }
 
 // Raising one maximum from every row.  Atomics on one address take turns, and the rows that run first all find the value they start from: with an

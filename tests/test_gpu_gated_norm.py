@@ -132,6 +132,22 @@ def test_forward(cf, dev, rows, H, gate_rows, f32, form, e5m2):
     check_forward(forward(cf, dev, a, form, e5m2), a, form, e5m2)
 
 
+@pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("rows,H,gate_rows", [(300, 2048, 0), (200, 4096, 64), (64, 7168, 1), (40, 12288, 40), (500, 200, 3), (33, 1001, 10)])
+def test_forward_stream_has_the_bits_of_the_formula(cf, dev, rows, H, gate_rows, f32):
+    """Up to h every operation is one fp32 rounding, in the order in which the formula is written: a bf16 stream next to the border of two values depends on it."""
+    case(f"gated norm bits rows={rows} H={H} gate_rows={gate_rows} f32={f32}")
+    a = Layer(rows, H, f32, gate_rows, 1.25, rows + H)
+    got = forward(cf, dev, a)
+    z = a.x.float() / got["post_rms"][:, None] * a.wp.float()
+    if a.gate is not None:
+        z = a.gate.float().repeat_interleave(gate_rows, 0)[:rows] * z
+    assert torch.equal(got["sum"], (1.25 * a.r.float() + z).to(a.r.dtype))
+    # a thread's own sum has at most four chains of eight fmas, added up: 12 roundings of u, halved by the root; the rest is in 64 bits, and the result rounded once
+    px = (a.x.double().square().mean(1) + EPS).sqrt()
+    assert torch.all((got["post_rms"].double() - px).abs() <= 7 * U * px)
+
+
 @pytest.mark.parametrize("form", ["rows", "block", "record"])
 @pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("shift", [0, 1, 2, 4, 8])
