@@ -208,7 +208,7 @@ struct GatedGradArgs {
     float* part_p;                // [parts, H] shares of P (GROUPS: of dwp)
     float* part_amax;             // [parts]
     float* segments;              // GROUPS: [workers, 2, H] shares of P of the groups that several workers have
-    double* far_dwp;              // GROUPS, four chunks a thread: [parts, 32, threads], where neither registers nor LDS have room for it
+    double* far_dwp;              // GROUPS, WIDE: [parts, 16, kT], where neither registers nor LDS have room for it
     int rows, H, gate_rows, groups, workers;
     unsigned share;
     float res, kept_inv;
@@ -320,15 +320,16 @@ constexpr int kGradThreads = 512;       // of a row at most: 256 registers each
 // A worker (a workgroup; ONE_WAVE: a wavefront) holds a row as k_gated_norm does and loads the next row's operands before it works on one.  Its shares of
 // the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
 // workers take turns at the rows; GROUPS: each has rows next to each other, and leaves P at a group's end: dgate itself where it had the whole group.
-template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_grad(const GatedGradArgs p) {
+template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V, bool WIDE>
+__global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThreads) void k_gated_norm_grad(const GatedGradArgs p) {
+    constexpr int kT = WIDE ? 2 * kGradThreads : kGradThreads;
     constexpr bool IN_LDS = V > 1;      // dw: 64 or 128 KB
-    constexpr bool FAR = V == 4;
+    constexpr bool FAR = WIDE;
     constexpr bool TIGHT = V > 1;
     __shared__ float sh[2][16];         // each is written again only behind the other one's barrier
     __shared__ double sh_sum[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
-    __shared__ double sh_dw[IN_LDS ? V * 8 * kGradThreads : 1];
-    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !FAR ? V * 8 * kGradThreads : 1];
+    __shared__ double sh_dw[IN_LDS ? V * 8 * kT : 1];
+    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !FAR ? V * 8 * kT : 1];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
     const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
@@ -365,11 +366,12 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
     u32x4_any w[V], wp[V], gate[V];         // GROUPS: the gate is loaded where its rows begin
     float gw[TIGHT ? 1 : V][8];                  // gate * wp
     double dw[IN_LDS ? 1 : V][8], ps[V][8], dwp[GROUPS && ONE_WAVE ? V : 1][8];
-    // dwp, which changes at a group's end only
+    // dwp, which changes at a group's end only; constant distances between a thread's sums, which need no registers
+    double* far_dwp = p.far_dwp + static_cast<size_t>(blockIdx.x) * (V * 8 * kT);
     auto dwp_at = [&](int j, int i) -> double& {
         if constexpr (ONE_WAVE) return dwp[j][i];
-        else if constexpr (FAR) return p.far_dwp[(static_cast<size_t>(blockIdx.x) * V * 8 + j * 8 + i) * T + t];
-        else return sh_dwp[(j * 8 + i) * T + t];
+        else if constexpr (FAR) return far_dwp[(j * 8 + i) * kT + t];
+        else return sh_dwp[(j * 8 + i) * kT + t];
     };
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         for (int i = 0; i < 8; ++i) {
             ps[j][i] = 0.0;
             if constexpr (!TIGHT) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
-            if constexpr (IN_LDS) sh_dw[(j * 8 + i) * T + t] = 0.0;
+            if constexpr (IN_LDS) sh_dw[(j * 8 + i) * kT + t] = 0.0;
             else dw[j][i] = 0.0;
             if constexpr (GROUPS) dwp_at(j, i) = 0.0;
         }
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
     const float s = p.q ? *p.qscale : 0.0f;
     const bool s_finite = abs_bits(s) < kInf;
     float amax = 0.0f;
-    constexpr bool AHEAD = V <= 2;          // four chunks leave no registers for a second row
+    constexpr bool AHEAD = !WIDE;           // which has 128 registers, none for a second row
     Row r, next;
     Walk walk{worker, static_cast<unsigned>(p.workers), rows, static_cast<unsigned>(p.gate_rows), static_cast<unsigned>(p.groups), p.share}, then;
     unsigned row = worker;
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dy = value8<false, TAIL>(r.dy[j], i, left(j));
-                if constexpr (IN_LDS) unsafeAtomicAdd(&sh_dw[(j * 8 + i) * T + t], static_cast<double>(dy * hh[i]));
+                if constexpr (IN_LDS) unsafeAtomicAdd(&sh_dw[(j * 8 + i) * kT + t], static_cast<double>(dy * hh[i]));
                 else dw[j][i] += static_cast<double>(dy * hh[i]);
                 if constexpr (TIGHT && !IN_LDS) asm volatile("" : "+v"(dw[j][i]));         // added here, not at the row's end, to which its terms would be kept
                 dot = __builtin_fmaf(dy * pair_at(w[j], i), hh[i], dot);
@@ -499,6 +501,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         }
         if constexpr (GROUPS) {
             if (walk.last_of_piece()) {
+                if constexpr (FAR) asm volatile("" : "+s"(far_dwp));          // its addresses are made here, not kept in registers from row to row
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float o[8];
@@ -553,7 +556,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : kGradThreads) void k_gated_norm_gr
         }
     };
     leave([&](int j, int i) {
-        if constexpr (IN_LDS) return sh_dw[(j * 8 + i) * T + t];
+        if constexpr (IN_LDS) return sh_dw[(j * 8 + i) * kT + t];
         else return dw[j][i];
     }, p.part_w);
     leave([&](int j, int i) {
@@ -717,13 +720,13 @@ GatedNormArgs forward_args(const void* d_residual, const uint16_t* d_x, float re
     return p;
 }
 
-// chunks of a row that a thread has in the backward pass
-constexpr int grad_chunks(int H) { return H <= 8 * kGradThreads ? 1 : H <= 16 * kGradThreads ? 2 : 4; }
+// rows of up to kTallH: one chunk a thread; beyond, two; beyond kWideH, two and twice the threads
+constexpr int kTallH = 8 * kGradThreads, kWideH = 16 * kGradThreads;
 // Workgroups of the backward pass, as many wavefronts as k_add_norm_grad runs and at least four rows each: see grad_parts() there.
 int gated_parts(int rows, int H) {
-    const int waves = H <= kOneWaveH ? 4 : row_threads(H, grad_chunks(H)) / kWave;
+    const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kTallH ? 1 : 2) / kWave;
     const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;
-    int parts = 256 * (8 / waves);
+    int parts = 256 * (waves < 8 ? 8 / waves : 1);
     parts = parts < turns / 4 ? parts : turns / 4;
     parts = parts > 256 ? parts : 256;
     return parts < turns ? parts : turns;
@@ -744,17 +747,17 @@ GradPlan grad_plan(int rows, int H, int gate_rows) {
     g.share = static_cast<unsigned>((rows - 1) / g.workers + 1);
     g.segments = g.several && !Walk::by_groups(g.groups, g.workers);
     const size_t shares = 2 * static_cast<size_t>(g.parts) + (g.segments ? 2 * static_cast<size_t>(g.workers) : 0);
-    g.far = g.several && grad_chunks(H) == 4 ? static_cast<size_t>(g.parts) * 4 * 8 * row_threads(H, 4) * sizeof(double) : 0;
+    g.far = g.several && H > kWideH ? static_cast<size_t>(g.parts) * 2 * 8 * (2 * kGradThreads) * sizeof(double) : 0;
     g.bytes = g.far + (shares * H + g.parts) * sizeof(float);
     return g;
 }
 
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL>
 void launch_gated_grad(const GatedGradArgs& p, int parts, hipStream_t st) {
-    if (p.H <= kOneWaveH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, true, 1><<<parts, 4 * kWave, 0, st>>>(p);
-    else if (grad_chunks(p.H) == 1) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1><<<parts, row_threads(p.H, 1), 0, st>>>(p);
-    else if (grad_chunks(p.H) == 2) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2><<<parts, row_threads(p.H, 2), 0, st>>>(p);
-    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 4><<<parts, row_threads(p.H, 4), 0, st>>>(p);
+    if (p.H <= kOneWaveH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, true, 1, false><<<parts, 4 * kWave, 0, st>>>(p);
+    else if (p.H <= kTallH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1, false><<<parts, row_threads(p.H, 1), 0, st>>>(p);
+    else if (p.H <= kWideH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2, false><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2, true><<<parts, row_threads(p.H, 2), 0, st>>>(p);
 }
 
 int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, float* d_grad_scale, int accumulate, void* d_workspace,
