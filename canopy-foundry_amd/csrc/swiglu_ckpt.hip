@@ -525,7 +525,7 @@ int cf_swiglu_ckpt8_backward_quant_e5m2(const uint16_t* d_grad_out, const void* 
     p.grad8 = static_cast<uint8_t*>(d_grad8); p.grad8_t = static_cast<uint8_t*>(d_grad8_t); p.act8_t = static_cast<uint8_t*>(d_act8_t);
     p.qscale = d_qscale; p.amax = d_amax; p.act_qscale = d_act_qscale;
     const size_t tiles = static_cast<size_t>(ceil_div(rows, kTile)) * ceil_div(I, kTile);
-    if (tiles * kTileThreads >= (static_cast<size_t>(1) << 32)) return CF_ERR_UNSUPPORTED;         // a terabyte of gradients
+    if ((tiles + 8) * kTileThreads > (static_cast<size_t>(1) << 32)) return CF_ERR_UNSUPPORTED;         // a terabyte of gradients
     const unsigned grid = (static_cast<unsigned>(tiles) + 7) / 8 * 8;
     hipStream_t st = as_stream(stream);
     auto go = [&](auto rows_whole, auto lines_whole) {
