@@ -183,7 +183,36 @@ def main():
         lambda: cf.cf_add_rmsnorm_backward(x2, hsum, 0, gamma, rms, x, M, K, dr, dgamma, 0, bws, bsz.value, st))
     hbm("add_rmsnorm_backward_quant_e5m2", f"{M}x{K}", 9.0 * n,
         lambda: cf.cf_add_rmsnorm_backward_quant_e5m2(x2, hsum, 0, gamma, rms, x, M, K, dr, dgamma, 0, q, sc, amax, bws, bsz.value, st))
-    del x32, s32, dr
+    # the layer with a norm on both sides of its block, and its gated activation kept in 8 bits for the backward pass
+    gate = (0.5 + 0.2 * torch.randn(4, K, device=dev, generator=g)).to(torch.bfloat16)
+    prms = torch.empty(M, device=dev); x8 = u8(M, K); h8 = u8(M, K)
+    hbm("gated_add_rmsnorm_quantize_rows, 8-bit checkpoints", f"{M}x{K}", 9.0 * n + 8 * M,
+        lambda: cf.cf_gated_add_rmsnorm_quantize_rows(x, x2, 0, 1.0, gate, M // 4, gamma, gamma, M, K, 1e-6, 0, hsum, None, prms, rms, x8, h8, q, rs, rd, st))
+    hbm("gated_add_rmsnorm_quantize_rows, fp32 stream, 8-bit checkpoints", f"{M}x{K}", 13.0 * n + 8 * M,
+        lambda: cf.cf_gated_add_rmsnorm_quantize_rows(x32, x2, 1, 1.0, gate, M // 4, gamma, gamma, M, K, 1e-6, 0, s32, None, prms, rms, x8, h8, q, rs, rd, st))
+    dgam2 = torch.zeros(K, device=dev); dgate = torch.zeros(4, K, device=dev); dx = torch.empty_like(x)
+    for what, rpg in (("one gate", M), ("four gates", M // 4)):
+        cf.raw_cf_gated_add_rmsnorm_backward_workspace_bytes(M, K, rpg, ctypes.byref(bsz))
+        bws2 = u8(bsz.value)
+        hbm(f"gated_add_rmsnorm_backward, {what}", f"{M}x{K}", 12.0 * n,
+            lambda: cf.cf_gated_add_rmsnorm_backward(x2, hsum, x2, 0, 1.0, gate, rpg, gamma, gamma, prms, rms, x, M, K, dr, dx, None, None, None, dgam2, dgamma, dgate, 0,
+                                                     bws2, bsz.value, st))
+        hbm(f"gated_add_rmsnorm_backward_ckpt8 with E5M2 bytes, {what}", f"{M}x{K}", 9.0 * n,
+            lambda: cf.cf_gated_add_rmsnorm_backward_ckpt8(x2, h8, x8, 0, 1.0, gate, rpg, gamma, gamma, prms, rms, x, M, K, dr, None, q, sc, amax, dgam2, dgamma, dgate, 0,
+                                                           bws2, bsz.value, st))
+    gu = bf16(M, 2 * N); nn_ = M * N
+    g8 = u8(M, N); u8_ = u8(M, N); gd8 = f32(M, N // 128); ud8 = f32(M, N // 128); a8 = u8(M, N); dact = bf16(M, N)
+    asc = torch.full((1,), 8.0, device=dev)
+    hbm("swiglu_ckpt8_quantize_rows", f"{M}x{N}", 7.06 * nn_,
+        lambda: cf.cf_swiglu_ckpt8_quantize_rows(gu, gu[:, N:], 2 * N, M, N, 0, g8, gd8, u8_, ud8, a8, rs, rd, st))
+    hbm("swiglu_ckpt8_quantize_record", f"{M}x{N}", 7.06 * nn_,
+        lambda: cf.cf_swiglu_ckpt8_quantize_record(gu, gu[:, N:], 2 * N, M, N, 0, g8, gd8, u8_, ud8, a8, asc, amax, st))
+    hbm("swiglu_ckpt8_backward (bf16)", f"{M}x{N}", 8.06 * nn_,
+        lambda: cf.cf_swiglu_ckpt8_backward(dact, g8, gd8, u8_, ud8, M, N, gu, gu[:, N:], 2 * N, None, st))
+    grad8 = u8(M, 2 * N); grad8t = u8(2 * N, M); act8t = u8(N, M)
+    hbm("swiglu_ckpt8_backward_quant_e5m2, transposed operands too", f"{M}x{N}", 9.06 * nn_,
+        lambda: cf.cf_swiglu_ckpt8_backward_quant_e5m2(dact, g8, gd8, u8_, ud8, M, N, grad8, grad8t, sc, amax, act8t, asc, st))
+    del x32, s32, dr, gu, g8, u8_, a8, dact, grad8, grad8t, act8t
     if any(args.only in name for name in ("grad_norm", "grad_clip in place (given norm)")):
         grads = [torch.randn(4 * K * K + 3 * K * N, device=dev, generator=g) * 1e-3, torch.randn(K, device=dev, generator=g)]
         ptrs = torch.tensor([t.data_ptr() for t in grads], dtype=torch.int64)
