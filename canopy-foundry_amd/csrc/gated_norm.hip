@@ -37,7 +37,9 @@ struct GatedNormArgs {
 
 __device__ __forceinline__ float pair_at(const u32x4_any& v, int i) { return (i & 1) ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]); }
 
-// One row in registers, V chunks of eight elements a thread, as k_add_norm holds it: everything is read and written once.
+// One row in registers, V chunks of eight elements a thread (forward_chunks() says how many), as k_add_norm holds it: everything is read and written once.  Bound by HBM, 9 or 13
+// bytes an element with both checkpoints: 8192 x 4096 59 us on a bf16 stream (5.1 TB/s), 83 on an fp32 one (5.2), 1000 x 7168 15; a row alone takes 3.7, launch, load and two
+// reductions.  Recording a maximum adds 6 us to 8192 rows (see raise_first()).  Odd widths move whole chunks that straddle lines: 8192 x 4095 75 us.
 template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_norm(const GatedNormArgs p) {
     __shared__ double sh_post[2][16];
@@ -319,17 +321,19 @@ __device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const flo
 constexpr int kGradThreads = 512;       // of a row at most: 256 registers each
 // A worker (a workgroup; ONE_WAVE: a wavefront) holds a row as k_gated_norm does and loads the next row's operands before it works on one.  Its shares of
 // the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
-// workers take turns at the rows; GROUPS: each has rows next to each other, and leaves P at a group's end: dgate itself where it had the whole group.
+// workers take turns at the rows; GROUPS: as Walk has it, and at the end of a piece of a group P is left, dgate itself where the worker had the whole group.
+// Bound by HBM: 8192 x 4096 from bf16 rows 73 us (5.5 TB/s), from checkpoints with the E5M2 bytes 54 (5.6), and 5 for k_gated_sum.  What it took: registers.  Two sums of
+// 64 bits a column, two rows of five tensors and three weights are 256 registers for eight or sixteen columns a thread; with 1024 threads of 128 each, 2000 x 7168 (fp32 stream,
+// gates by sequence) took 159 us, with 512 of 256 94, and 64 with dw in LDS, a row ahead and Walk's order.  WIDE (H above 8192) has no room for a row ahead:
+// 2048 x 16384 114 us (3.5 TB/s).
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V, bool WIDE>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThreads) void k_gated_norm_grad(const GatedGradArgs p) {
     constexpr int kT = WIDE ? 2 * kGradThreads : kGradThreads;
-    constexpr bool IN_LDS = V > 1;      // dw: 64 or 128 KB
-    constexpr bool FAR = WIDE;
-    constexpr bool TIGHT = V > 1;
+    constexpr bool TIGHT = V > 1;       // of registers: dw in LDS, values made from the loaded elements as often as they are used
     __shared__ float sh[2][16];         // each is written again only behind the other one's barrier
     __shared__ double sh_sum[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
-    __shared__ double sh_dw[IN_LDS ? V * 8 * kT : 1];
-    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !FAR ? V * 8 * kT : 1];
+    __shared__ double sh_dw[TIGHT ? V * 8 * kT : 1];
+    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !WIDE ? V * 8 * kT : 1];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
     const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
@@ -365,19 +369,18 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
     };
     u32x4_any w[V], wp[V], gate[V];         // GROUPS: the gate is loaded where its rows begin
     float gw[TIGHT ? 1 : V][8];                  // gate * wp
-    double dw[IN_LDS ? 1 : V][8], ps[V][8], dwp[GROUPS && ONE_WAVE ? V : 1][8];
+    double dw[TIGHT ? 1 : V][8], ps[V][8], dwp[GROUPS && ONE_WAVE ? V : 1][8];
     // dwp, which changes at a group's end only; constant distances between a thread's sums, which need no registers
     double* far_dwp = p.far_dwp + static_cast<size_t>(blockIdx.x) * (V * 8 * kT);
     auto dwp_at = [&](int j, int i) -> double& {
         if constexpr (ONE_WAVE) return dwp[j][i];
-        else if constexpr (FAR) return far_dwp[(j * 8 + i) * kT + t];
+        else if constexpr (WIDE) return far_dwp[(j * 8 + i) * kT + t];
         else return sh_dwp[(j * 8 + i) * kT + t];
     };
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         w[j] = wp[j] = u32x4_any{0, 0, 0, 0};
-        gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-        if constexpr (GROUPS) gate[j] = u32x4_any{0, 0, 0, 0};
+        gate[j] = u32x4_any{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};           // 1
         if (has(j)) {
             w[j] = load_weight<TAIL>(p.weight, (t + j * T) * 8, left(j), H);
             wp[j] = load_weight<TAIL>(p.post_weight, (t + j * T) * 8, left(j), H);
@@ -388,7 +391,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         for (int i = 0; i < 8; ++i) {
             ps[j][i] = 0.0;
             if constexpr (!TIGHT) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
-            if constexpr (IN_LDS) sh_dw[(j * 8 + i) * kT + t] = 0.0;
+            if constexpr (TIGHT) sh_dw[(j * 8 + i) * kT + t] = 0.0;
             else dw[j][i] = 0.0;
             if constexpr (GROUPS) dwp_at(j, i) = 0.0;
         }
@@ -448,9 +451,8 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dy = value8<false, TAIL>(r.dy[j], i, left(j));
-                if constexpr (IN_LDS) unsafeAtomicAdd(&sh_dw[(j * 8 + i) * kT + t], static_cast<double>(dy * hh[i]));
+                if constexpr (TIGHT) unsafeAtomicAdd(&sh_dw[(j * 8 + i) * kT + t], static_cast<double>(dy * hh[i]));
                 else dw[j][i] += static_cast<double>(dy * hh[i]);
-                if constexpr (TIGHT && !IN_LDS) asm volatile("" : "+v"(dw[j][i]));         // added here, not at the row's end, to which its terms would be kept
                 dot = __builtin_fmaf(dy * pair_at(w[j], i), hh[i], dot);
             }
         }
@@ -472,7 +474,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
                 const float v = __builtin_fmaf(__builtin_fmaf(-hh[i], c, g), inv, value8<F32, TAIL>(r.dh[j], i, left(j)));
                 o[i] = v * p.res;
                 ps[j][i] += static_cast<double>(v * xh[i]);
-                if constexpr (TIGHT) asm volatile("" : "+v"(ps[j][i]));
+                if constexpr (TIGHT) asm volatile("" : "+v"(ps[j][i]));         // added here, not at the row's end, to which its terms would be kept
                 e[j][i] = v * (TIGHT ? pair_at(gate[j], i) * pair_at(wp[j], i) : gw[TIGHT ? 0 : j][i]);
                 dot = __builtin_fmaf(e[j][i], xh[i], dot);
             }
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         }
         if constexpr (GROUPS) {
             if (walk.last_of_piece()) {
-                if constexpr (FAR) asm volatile("" : "+s"(far_dwp));          // its addresses are made here, not kept in registers from row to row
+                if constexpr (WIDE) asm volatile("" : "+s"(far_dwp));          // its addresses are made here, not kept in registers from row to row
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float o[8];
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         }
     };
     leave([&](int j, int i) {
-        if constexpr (IN_LDS) return sh_dw[(j * 8 + i) * kT + t];
+        if constexpr (TIGHT) return sh_dw[(j * 8 + i) * kT + t];
         else return dw[j][i];
     }, p.part_w);
     leave([&](int j, int i) {
@@ -722,7 +724,8 @@ GatedNormArgs forward_args(const void* d_residual, const uint16_t* d_x, float re
 
 // rows of up to kTallH: one chunk a thread; beyond, two; beyond kWideH, two and twice the threads
 constexpr int kTallH = 8 * kGradThreads, kWideH = 16 * kGradThreads;
-// Workgroups of the backward pass, as many wavefronts as k_add_norm_grad runs and at least four rows each: see grad_parts() there.
+// Workgroups of the backward pass: as many as run at once with 256 registers a thread, eight wavefronts a CU (292 of seven wavefronts ran in two rounds: 8192 x 7168 196 us, 134 with
+// 256), and four rows each, or the shares cost more than the rows; but 256 where there are as many rows.
 int gated_parts(int rows, int H) {
     const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kTallH ? 1 : 2) / kWave;
     const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;

@@ -66,7 +66,10 @@ __device__ __forceinline__ float largest(const float (&a)[8]) {
 
 // A thread has V chunks of eight elements of a row, chunk c by thread c % T of the row's workgroup or, where the scale is not the whole row's, of one of its `parts`.  Sixteen
 // lanes are a group of 128 elements.  Of the two (Q_BLOCK: three) scales of a group each quarter of its lanes makes one, in the same instructions: a division takes a dozen.
-// What has been divided by its own maximum needs no clamp.
+// What has been divided by its own maximum needs no clamp, and no look for NaNs: the conversion keeps them.
+// Bound by HBM once the instructions are few enough (24 an element; with 41, divisions by every lane, clamps and looks for NaNs, 8192 x 8192 took 90 to 102 us): 7 bytes an element,
+// 8192 x 8192 80 us (5.9 TB/s) with a scale a row or a group, 91 where a maximum is recorded, 8192 x 14336 144 (5.8); 1000 x 5461 9.4.
+// A whole row wants as few chunks a thread as it can have: 1, 2, 4 of them 78.6, 82.8, 83.9 us at 4096 wide, 81.0, 83.9, 85.3 at 8192, 85 each at 14336.
 template <int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThreads) void k_swiglu_keep(const SwigluKeepArgs p) {
     __shared__ uint32_t sh[2][16];
@@ -240,7 +243,7 @@ __device__ __forceinline__ void grads8(const Raw8<false>& d, const u32x2_any& g8
     }
 }
 
-// bf16 outputs, a chunk a thread; workgroups as k_swiglu_keep's.
+// bf16 outputs, a chunk a thread; workgroups as k_swiglu_keep's.  Bound by HBM: 10 bytes an element with the activation, 8192 x 8192 114 us (5.9 TB/s).
 template <bool TAIL>
 __global__ __launch_bounds__(kKeepThreads) void k_swiglu_grad(const SwigluGradArgs p) {
     const unsigned row = p.row0 + blockIdx.x / p.parts, groups = (static_cast<unsigned>(p.I) + 127) / 128;
@@ -273,7 +276,8 @@ __device__ __forceinline__ void transpose4x4(uint32_t r0, uint32_t r1, uint32_t 
 
 typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
 
-// 8-bit outputs: a workgroup has 128 x 128 elements, a thread four rows of eight of them, whose bytes it writes along the rows and, through LDS, along the columns.
+// 8-bit outputs, 9 bytes an element, bound by HBM and by how well lines are filled: 8192 x 14336 214 us (5.0 TB/s), 2000 x 8192 42, whose transposed rows begin anywhere in a line.
+// A workgroup has 128 x 128 elements (64 columns: 250 us; 64 rows: 250; 256 rows: 215, and no better where lines are split), a thread four rows of eight of them, whose bytes it writes along the rows and, through LDS, along the columns.
 // Pieces that are whole 128-byte lines leave past the L2 (8192 x 14336: 213 us, 223 through it); where they are not (WHOLE_ROWS: of the straight outputs, WHOLE_LINES: of the transposed), the
 // L2 puts a line together from neighbouring tiles, which is why one XCD has them: 8191 x 8192 240 us past it, 153 through it, 162 with the tiles in row-major order over all XCDs.
 // LDS holds [column][128 bytes of rows] for each of the three outputs.  A wavefront's store instruction writes four bytes for each of 16 column blocks and four row blocks:

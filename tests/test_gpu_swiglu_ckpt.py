@@ -313,3 +313,29 @@ def test_gradient_against_differences(cf, dev):
         a, b = (torch.randn(g.shape, generator=gen, dtype=torch.float64) for _ in range(2))
         slope = (value(g + 1e-4 * a, u + 1e-4 * b) - value(g - 1e-4 * a, u - 1e-4 * b)) / 2e-4
         assert abs((dg * a).sum() + (du * b).sum() - slope) <= (2.0 ** -8 + 1e-5) * ((dg * a).abs().sum() + (du * b).abs().sum())
+
+
+@pytest.mark.parametrize("form", ["rows", "block", "record"])
+def test_more_rows_than_one_launch_holds(cf, dev, form):
+    """Rows of eight, 2^22 and a few: the last ones are as they are alone, forward and back."""
+    rows, I, n = (1 << 22) + 7, 8, 500
+    case(f"swiglu {form} {rows} rows of {I}")
+    g, u = (torch.randn(rows, I, device=dev).to(torch.bfloat16) for _ in range(2))
+
+    def run(g, u):
+        R = g.shape[0]
+        b, d = [torch.zeros(R, I, dtype=torch.uint8, device=dev) for _ in range(3)], [torch.zeros(R, 1, device=dev) for _ in range(4)]
+        head, kept = (g, u, I, R, I), (b[0], d[0], b[1], d[1], b[2])
+        if form == "record":
+            cf.cf_swiglu_ckpt8_quantize_record(*head, 0, *kept, torch.full((1,), 20.0, device=dev), torch.zeros(1, device=dev), stream())
+        elif form == "block":
+            cf.cf_swiglu_ckpt8_quantize_block_1x128(*head, *kept, d[2], d[3], stream())
+        else:
+            cf.cf_swiglu_ckpt8_quantize_rows(*head, 0, *kept, d[2], d[3], stream())
+        o = [torch.zeros(R, I, dtype=torch.bfloat16, device=dev) for _ in range(3)]
+        cf.cf_swiglu_ckpt8_backward(u, b[0], d[0], b[1], d[1], R, I, o[0], o[1], I, o[2], stream())
+        torch.cuda.synchronize()
+        return b + d + o
+
+    for whole, alone in zip(run(g, u), run(g[-n:].contiguous(), u[-n:].contiguous())):
+        assert torch.equal(whole[-n:], alone)
