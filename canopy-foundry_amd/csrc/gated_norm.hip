@@ -417,24 +417,18 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
             more_then = then.advance();
             if (more_then) row_then = then.row();
         }
-        if constexpr (AHEAD) {
-            r = next;
-            if (more_then) load(next, row_then);
-        } else {
-            load(r, row);
-        }
-        if constexpr (GROUPS) {
+        if constexpr (AHEAD) r = next;
+        if constexpr (GROUPS) {             // before the next row's loads, or they would be waited for with it
             if (walk.m == 0) {
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    if (has(j)) {
-                        gate[j] = load_weight<TAIL>(p.gate + static_cast<size_t>(walk.group) * H, (t + j * T) * 8, left(j), H);
-                        if constexpr (!TIGHT) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
-                        }
-                    }
+                    if (has(j)) gate[j] = load_weight<TAIL>(p.gate + static_cast<size_t>(walk.group) * H, (t + j * T) * 8, left(j), H);
             }
+        }
+        if constexpr (AHEAD) {
+            if (more_then) load(next, row_then);
+        } else {
+            load(r, row);
         }
         const size_t base = static_cast<size_t>(row) * H;
         const float inv = 1.0f / r.rms, post_inv = 1.0f / r.post_rms;
@@ -458,6 +452,14 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         }
         const float c = row_sum<ONE_WAVE>(dot, sh[0]) / static_cast<float>(H);
         dot = 0.0f;
+        if constexpr (GROUPS && !TIGHT) {
+            if (walk.m == 0) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
+            }
+        }
         float e[V][8];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
