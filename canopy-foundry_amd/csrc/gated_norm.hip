@@ -44,7 +44,7 @@ template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_norm(const GatedNormArgs p) {
     __shared__ double sh_post[2][16];
     __shared__ float sh_sum[2][16];
-    __shared__ uint32_t sh_max[4][16];
+    __shared__ uint32_t sh_max[3][16];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     unsigned row = p.row0 + blockIdx.x;
     int t = threadIdx.x;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_
     // has in fp32: a bf16 stream takes the next value where h lies next to the border of two, and through the maximum of a group one such value can be all of a scale's
     // difference (some 160 of 7 million values lie there).  x / px is x times the inverse and a correction by what that leaves.
     int e;
-    const float post_rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_post, sh_max[2], e);
+    const float post_rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_post, sh_max[1], e);
     if (t == 0 && p.post_rms) p.post_rms[row] = ldexpf(post_rms, e);
     const float post_inv = 1.0f / post_rms, divisor = post_rms < __builtin_inff() ? post_rms : 0.0f;         // infinite: 0 or NaN
 #pragma unroll
@@ -118,77 +118,68 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_
         if (p.sum && has(j)) store8_stream<F32, TAIL, !TAIL>(p.sum, base + (t + j * T) * 8, left(j), h[j]);
     }
 
-    const float rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum, sh_max[3], e);
+    const float rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_sum, sh_max[2], e);
     if (t == 0 && p.rms) p.rms[row] = ldexpf(rms, e);
     const float inv = 1.0f / rms;
     const float F = p.e5m2 ? 57344.0f : 448.0f;
-    uint32_t top[V];
+    float top[V];           // a chunk's largest |y| without its NaNs
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         keep(p.sum8, j, inv * p.kept);
-        top[j] = 0;
+        top[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             h[j][i] = h[j][i] * inv * pair_at(w[j], i);        // y from here on
-            top[j] = max(top[j], abs_bits(h[j][i]));
+            top[j] = fmaxf(top[j], fabsf(h[j][i]));
         }
         if (p.normed && has(j)) store8_bf16<TAIL>(p.normed, base + (t + j * T) * 8, left(j), h[j]);
     }
-    // the largest |y| of a chunk without its NaNs
-    auto number = [&](int j) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(h[j][i]));
-        return __float_as_uint(m);
-    };
-    auto quantize = [&](int j, float s, bool finite) {
+    // what has been divided by its own maximum needs no clamp, and the conversion keeps NaNs
+    auto quantize = [&](int j, float s) {
         if (!has(j)) return;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = h[j][i] * s;
-        store8_fp8<TAIL>(p.q, base + (t + j * T) * 8, left(j), p.e5m2, finite, v);
+        const size_t to = base + (t + j * T) * 8;
+        if constexpr (QMODE == Q_RECORD) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+            store8_fp8<TAIL>(p.q, to, left(j), p.e5m2, __all(m <= kInf), v);
+        } else {
+            store8_bytes<TAIL>(p.q, to, left(j), p.e5m2 ? convert8_fp8<true>(v) : convert8_fp8<false>(v));
+        }
     };
     if constexpr (QMODE == Q_BLOCK) {
         const int groups = (H + 127) >> 7;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            uint32_t m = max16(top[j]);
-            const bool finite = __all(m < kInf);
-            if (!finite) m = max16(number(j));
-            const float a = fmaxf(__uint_as_float(m), 1e-12f), s = F / a;
+            const float a = fmaxf(__uint_as_float(max16(__float_as_uint(top[j]))), 1e-12f), s = F / a;
             const int c = t + j * T;
             if ((c & 15) == 0 && has(j)) {
                 p.scale[static_cast<size_t>(row) * groups + (c >> 4)] = s;
                 p.descale[static_cast<size_t>(row) * groups + (c >> 4)] = a / F;
             }
-            quantize(j, s, finite);
+            quantize(j, s);
         }
     } else {
-        uint32_t m = 0;
+        float m = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) m = max(m, top[j]);
-        m = row_max<ONE_WAVE>(m, sh_max[0]);
-        bool finite = m < kInf;
-        if (!finite) {
-            uint32_t n = 0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) n = max(n, number(j));
-            m = row_max<ONE_WAVE>(n, sh_max[1]);
-        }
+        for (int j = 0; j < V; ++j) m = fmaxf(m, top[j]);
+        const uint32_t bits = row_max<ONE_WAVE>(__float_as_uint(m), sh_max[0]);
         float s, before = 0.0f;
         if constexpr (QMODE == Q_ROWS) {
-            const float a = fmaxf(__uint_as_float(m), 1e-12f);
+            const float a = fmaxf(__uint_as_float(bits), 1e-12f);
             s = F / a;
             if (t == 0) { p.scale[row] = s; p.descale[row] = a / F; }
         } else {
             s = *p.qscale;
-            if (t == 0) raise_first(p.amax, m, row, p.rows, before);
-            finite = finite && abs_bits(s) < kInf;         // 0 times infinity
+            if (t == 0) raise_first(p.amax, bits, row, p.rows, before);
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) quantize(j, s, finite);
+        for (int j = 0; j < V; ++j) quantize(j, s);
         if constexpr (QMODE == Q_RECORD) {
-            if (t == 0) raise_last(p.amax, m, row, p.rows, before);
+            if (t == 0) raise_last(p.amax, bits, row, p.rows, before);
         }
     }
 }
