@@ -39,7 +39,7 @@ __device__ __forceinline__ float pair_at(const u32x4_any& v, int i) { return (i 
 
 // One row in registers, V chunks of eight elements a thread (forward_chunks() says how many), as k_add_norm holds it: everything is read and written once.  Bound by HBM, 9 or 13
 // bytes an element with both checkpoints: 8192 x 4096 59 us on a bf16 stream (5.1 TB/s), 83 on an fp32 one (5.2), 1000 x 7168 15; a row alone takes 3.7, launch, load and two
-// reductions.  Recording a maximum adds 6 us to 8192 rows (see raise_first()).  Odd widths move whole chunks that straddle lines: 8192 x 4095 75 us.
+// reductions.  Recording a maximum adds 6 us to 8192 rows (see raise_last()).  Odd widths move whole chunks that straddle lines: 8192 x 4095 75 us.
 template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_norm(const GatedNormArgs p) {
     __shared__ double sh_post[2][16];

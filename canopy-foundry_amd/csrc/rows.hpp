@@ -319,9 +319,15 @@ __device__ __forceinline__ void raise_first(float* amax, uint32_t m, unsigned ro
     before = atomic_load_agent(amax);
     if (raises_at_once(row, rows) && __uint_as_float(m) > before) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
 }
+// Before it comes back to memory it looks at the copy in its own L2: brought there by the first who looked behind the pause, a value that the maximum has had and so a bound that most are
+// under, for which nobody waits in turn (8192 x 4096 70.1 -> 66.0 us, 16384 x 2048 75.4 -> 70.5).
+__device__ __forceinline__ bool above_l2_copy(const float* amax, uint32_t m) {
+    return __uint_as_float(m) > __hip_atomic_load(amax, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
 __device__ __forceinline__ void raise_last(float* amax, uint32_t m, unsigned row, int rows, float before) {
     if (raises_at_once(row, rows) || __uint_as_float(m) <= before) return;
     __builtin_amdgcn_s_sleep(48);           // 48 x 64 cycles
+    if (!above_l2_copy(amax, m)) return;
     if (__uint_as_float(m) > atomic_load_agent(amax)) atomicMax(reinterpret_cast<int*>(amax), static_cast<int>(m));
 }
 

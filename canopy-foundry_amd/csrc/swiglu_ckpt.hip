@@ -68,7 +68,7 @@ __device__ __forceinline__ float largest(const float (&a)[8]) {
 // lanes are a group of 128 elements.  Of the two (Q_BLOCK: three) scales of a group each quarter of its lanes makes one, in the same instructions: a division takes a dozen.
 // What has been divided by its own maximum needs no clamp, and no look for NaNs: the conversion keeps them.
 // Bound by HBM once the instructions are few enough (24 an element; with 41, divisions by every lane, clamps and looks for NaNs, 8192 x 8192 took 90 to 102 us): 7 bytes an element,
-// 8192 x 8192 80 us (5.9 TB/s) with a scale a row or a group, 91 where a maximum is recorded, 8192 x 14336 144 (5.8); 1000 x 5461 9.4.
+// 8192 x 8192 80 us (5.9 TB/s) with a scale a row or a group, 90 where a maximum is recorded, 8192 x 14336 144 (5.8); 1000 x 5461 9.4.
 // A whole row wants as few chunks a thread as it can have: 1, 2, 4 of them 78.6, 82.8, 83.9 us at 4096 wide, 81.0, 83.9, 85.3 at 8192, 85 each at 14336.
 template <int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThreads) void k_swiglu_keep(const SwigluKeepArgs p) {
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
         const uint32_t m = row_max<false>(__float_as_uint(most), sh[1]);
         if (threadIdx.x == 0) {
             if (turns > 1) {
-                atomic_max_nonneg(p.amax, __uint_as_float(m));
+                if (above_l2_copy(p.amax, m)) atomic_max_nonneg(p.amax, __uint_as_float(m));
             } else {
                 float before;
                 raise_first(p.amax, m, blockIdx.x, gridDim.x, before);
@@ -404,7 +404,7 @@ Parts row_parts(int I, int V) {
 unsigned launch_rows(unsigned parts) { return parts < (kLaunchRows >> 1) ? (kLaunchRows << 1) / parts : 1; }
 
 // Recording a maximum: a workgroup that takes two pieces in turn has one maximum to report where it had two, and one in 64 raises it after the first piece, before any
-// other looks.  8192 x 14336: one piece 154 to 159 us, two 145, three 149, four 154; as many workgroups as run at once 167; without a maximum 148.
+// other looks.  8192 x 14336: one piece 151 to 157 us, two 145, three 149, four 154; as many workgroups as run at once 167 (8192 x 8192: one 87, two 90).
 constexpr unsigned kTurnPieces = 4096;
 
 template <int QMODE, bool TAIL>
