@@ -67,7 +67,7 @@ __device__ __forceinline__ float largest(const float (&a)[8]) {
 // A thread has V chunks of eight elements of a row, chunk c by thread c % T of the row's workgroup or, where the scale is not the whole row's, of one of its `parts`.  Sixteen
 // lanes are a group of 128 elements.  Of the two (Q_BLOCK: three) scales of a group each quarter of its lanes makes one, in the same instructions: a division takes a dozen.
 // What has been divided by its own maximum needs no clamp, and no look for NaNs: the conversion keeps them.
-// Bound by HBM once the instructions are few enough (24 an element; with 41, divisions by every lane, clamps and looks for NaNs, 8192 x 8192 took 90 to 102 us): 7 bytes an element,
+// Bound by HBM once the instructions are few enough (30 an element in all; with 41, divisions by every lane, clamps and looks for NaNs, 8192 x 8192 took 90 to 102 us): 7 bytes an element,
 // 8192 x 8192 80 us (5.9 TB/s) with a scale a row or a group, 90 where a maximum is recorded, 8192 x 14336 144 (5.8); 1000 x 5461 9.4.
 // A whole row wants as few chunks a thread as it can have: 1, 2, 4 of them 78.6, 82.8, 83.9 us at 4096 wide, 81.0, 83.9, 85.3 at 8192, 85 each at 14336.
 template <int QMODE, bool TAIL, bool ONE_WAVE, int V>
