@@ -156,7 +156,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThre
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = o[i] * sa;
             u32x2_any b;
-            if (QMODE == Q_RECORD && (__any(m == __builtin_inff()) || abs_bits(qs) >= kInf)) b = pack8_fp8(e5m2, false, v);
+            if (QMODE == Q_RECORD && __any(!(m * fabsf(qs) < __builtin_inff()))) b = pack8_fp8(e5m2, false, v);
             else b = e5m2 ? convert8_fp8<true>(v) : convert8_fp8<false>(v);
             if (n > 0) store8_bytes<TAIL>(p.q, to, n, b);
         }
@@ -297,7 +297,6 @@ __global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradA
     const int c0 = static_cast<int>(group) * kTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int at = c0 + tx * 8, n = p.I - at;
     float s = *p.qscale, as = p.act8_t ? *p.act_qscale : 0.0f;
-    const bool plain = abs_bits(s) < kInf && abs_bits(as) < kInf;
     saturate_fp8(s);
     saturate_fp8(as);
     Raw8<false> d[4];
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradA
         for (int k = 0; k < 8; ++k)
             if (!TAIL || k < n) m = fmaxf(fmaxf(m, fabsf(o.dg[k])), fabsf(o.du[k]));
         most = fmaxf(most, m);
-        const bool usual = plain && !__any(fmaxf(m, largest(o.a)) == __builtin_inff());
+        const bool usual = __all(m * fabsf(s) < __builtin_inff() && largest(o.a) * fabsf(as) < __builtin_inff());       // no product an infinity
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             o.dg[k] *= s;

@@ -171,6 +171,21 @@ def test_forward_zeros_infinities_and_nans(cf, dev, I, form):
         assert got["amax"] == float("inf") and q[4, 90] == 448.0 * float(torch.sign(u[4, 90]))
 
 
+@pytest.mark.parametrize("e5m2", [0, 1])
+@pytest.mark.parametrize("I", [96, 1000])
+def test_forward_scaled_beyond_fp32(cf, dev, I, e5m2):
+    """A finite activation whose product with the given scale leaves fp32 is the format's largest value, as any that the scale takes beyond it."""
+    case(f"swiglu record beyond fp32 I={I} e5m2={e5m2}")
+    g, u = inputs(6, I, 9)
+    g[2, 7], u[2, 7] = 1e20, 1e15
+    g[4, 30], u[4, 30] = 1e20, -1e15
+    got = forward(cf, dev, g, u, "record", e5m2, qscale=1e10)
+    check_forward(got, g, u, "record", e5m2, qscale=1e10)
+    dtype, top = F8[e5m2][:2]
+    q = got["q"].view(dtype).float()
+    assert q[2, 7] == top and q[4, 30] == -top
+
+
 # ---- gradient ---------------------------------------------------------------------------------------------------------
 
 class Grad:
@@ -299,6 +314,23 @@ def test_backward_nan_and_infinity(cf, dev, rows, I):
     both = torch.cat([keep, keep], 1)
     assert torch.equal(got8[0][both], clean8[0][both]) and torch.equal(got8[1], got8[0].t()) and torch.equal(got8[2], clean8[2])
     assert torch.isnan(got8[0].view(E5M2).float()[3, 5]) and abs(float(got8[0].view(E5M2).float()[7, I + 200])) == 57344.0 and amax == float("inf")
+
+
+@pytest.mark.parametrize("rows,I", [(48, 256), (37, 333)])
+def test_backward_8_bit_scaled_beyond_fp32(cf, dev, rows, I):
+    """Finite gradients and activations whose products with the given scales leave fp32 are the formats' largest values."""
+    case(f"swiglu 8-bit gradient beyond fp32 rows={rows} I={I}")
+    x = Grad(rows, I, 6)
+    x.do[3, 5], x.do[7, 200] = 1e33, -1e33
+    got = backward8(cf, dev, x, qscale=1e10, act_qscale=1e38)
+    check_backward8(got, x, qscale=1e10, act_qscale=1e38)
+    (dg, _), (du, _), (a, _) = x.formula()
+    want = torch.cat([dg, du], 1)
+    grad, act = got[0][0].view(E5M2).float(), got[0][2].t().contiguous().view(E4M3).float()
+    far = want.abs() * 1e10 > 2.0 ** 129
+    assert far.any() and torch.equal(grad[far], 57344.0 * torch.sign(want[far]).float())
+    far = a.abs() * 1e38 > 2.0 ** 129
+    assert far.any() and torch.equal(act[far], 448.0 * torch.sign(a[far]).float())
 
 
 def test_gradient_against_differences(cf, dev):
