@@ -201,7 +201,7 @@ struct GatedGradArgs {
     float* part_p;                // [parts, H] shares of P (GROUPS: of dwp)
     float* part_amax;             // [parts]
     float* segments;              // GROUPS: [workers, 2, H] shares of P of the groups that several workers have
-    double* far_dwp;              // GROUPS, WIDE: [parts, 16, kT], where neither registers nor LDS have room for it
+    double* far_dwp;              // GROUPS, H above 8192: [parts, 16, kT], where neither registers nor LDS have room for it
     int rows, H, gate_rows, groups, workers;
     unsigned share;
     float res, kept_inv;
@@ -309,22 +309,28 @@ __device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const flo
     }
 }
 
-constexpr int kGradThreads = 512;       // of a row at most: 256 registers each
+// Threads of a row at most: 512 of 256 registers, 768 of 168, 1024 of 128.  Up to H = 8192 a thread has one or two chunks.  WIDE, up to 12288: two, and the next row's operands on a
+// bf16 stream without groups alone, elsewhere they spill (us without them and with: 9216, bf16 98 and 87, with groups 110 and 145; fp32 131 and 221; all of it with 1024 threads 110, 161
+// and 192).  WIDEST: four, with groups two, which spill either way, if little (16384, without groups: four 98, two 113; with them 247 and 222).
+enum Width { USUAL, WIDE, WIDEST };
+template <bool GROUPS, Width WIDTH>
+constexpr int kGradThreads = WIDTH == WIDE ? 768 : WIDTH == WIDEST && GROUPS ? 1024 : 512;
 // A worker (a workgroup; ONE_WAVE: a wavefront) holds a row as k_gated_norm does and loads the next row's operands before it works on one.  Its shares of
 // the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
 // workers take turns at the rows; GROUPS: as Walk has it, and at the end of a piece of a group P is left, dgate itself where the worker had the whole group.
 // Bound by HBM: 8192 x 4096 from bf16 rows 73 us (5.5 TB/s), from checkpoints with the E5M2 bytes 54 (5.6), and 5 for k_gated_sum.  What it took: registers.  Two sums of
 // 64 bits a column, two rows of five tensors and three weights are 256 registers for eight or sixteen columns a thread; with 1024 threads of 128 each, 2000 x 7168 (fp32 stream,
-// gates by sequence) took 159 us, with 512 of 256 94, and 64 with dw in LDS, a row ahead and Walk's order.  WIDE (H above 8192) has no room for a row ahead:
-// 2048 x 16384 114 us (3.5 TB/s).
-template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V, bool WIDE>
-__global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThreads) void k_gated_norm_grad(const GatedGradArgs p) {
-    constexpr int kT = WIDE ? 2 * kGradThreads : kGradThreads;
+// gates by sequence) took 159 us, with 512 of 256 94, and 64 with dw in LDS, a row ahead and Walk's order.  Above H = 8192 there is room for
+// few rows ahead, and spills cost the most: 2730 x 12288 87 us (4.6 TB/s), 2048 x 16384 98 (4.1).
+template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V, Width WIDTH>
+__global__ __launch_bounds__((ONE_WAVE ? 256 : kGradThreads<GROUPS, WIDTH>)) void k_gated_norm_grad(const GatedGradArgs p) {
+    constexpr int kT = kGradThreads<GROUPS, WIDTH>;
+    constexpr bool FAR = GROUPS && WIDTH != USUAL;
     constexpr bool TIGHT = V > 1;       // of registers: dw in LDS, values made from the loaded elements as often as they are used
     __shared__ float sh[2][16];         // each is written again only behind the other one's barrier
     __shared__ double sh_sum[ONE_WAVE ? 4 : 1][ONE_WAVE ? 512 : 1];
     __shared__ double sh_dw[TIGHT ? V * 8 * kT : 1];
-    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !WIDE ? V * 8 * kT : 1];
+    __shared__ double sh_dwp[GROUPS && !ONE_WAVE && !FAR ? V * 8 * kT : 1];
     const int H = p.H, T = ONE_WAVE ? kWave : blockDim.x;
     const int t = ONE_WAVE ? threadIdx.x & 63 : threadIdx.x;
     const unsigned worker = ONE_WAVE ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)) : blockIdx.x;
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
     double* far_dwp = p.far_dwp + static_cast<size_t>(blockIdx.x) * (V * 8 * kT);
     auto dwp_at = [&](int j, int i) -> double& {
         if constexpr (ONE_WAVE) return dwp[j][i];
-        else if constexpr (WIDE) return far_dwp[(j * 8 + i) * kT + t];
+        else if constexpr (FAR) return far_dwp[(j * 8 + i) * kT + t];
         else return sh_dwp[(j * 8 + i) * kT + t];
     };
 #pragma unroll
@@ -384,13 +390,13 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
             if constexpr (!TIGHT) gw[j][i] = pair_at(gate[j], i) * pair_at(wp[j], i);
             if constexpr (TIGHT) sh_dw[(j * 8 + i) * kT + t] = 0.0;
             else dw[j][i] = 0.0;
-            if constexpr (GROUPS) dwp_at(j, i) = 0.0;
+            if constexpr (GROUPS && !FAR) dwp_at(j, i) = 0.0;
         }
     }
     const float s = p.q ? *p.qscale : 0.0f;
     const bool s_finite = abs_bits(s) < kInf;
     float amax = 0.0f;
-    constexpr bool AHEAD = !WIDE;           // which has 128 registers, none for a second row
+    constexpr bool AHEAD = WIDTH == USUAL || (WIDTH == WIDE && !F32 && !GROUPS);            // where the registers have room for a second row
     Row r, next;
     Walk walk{worker, static_cast<unsigned>(p.workers), rows, static_cast<unsigned>(p.gate_rows), static_cast<unsigned>(p.groups), p.share}, then;
     unsigned row = worker;
@@ -399,6 +405,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         more = worker < static_cast<unsigned>(p.workers) && walk.begin();
         if (more) row = walk.row();
     }
+    unsigned pieces = 0;                    // of groups, behind the worker
     if (AHEAD && more) load(next, row);
     while (more) {
         unsigned row_then = row + p.workers;
@@ -496,12 +503,23 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         }
         if constexpr (GROUPS) {
             if (walk.last_of_piece()) {
-                if constexpr (WIDE) asm volatile("" : "+s"(far_dwp));          // its addresses are made here, not kept in registers from row to row
+                if constexpr (FAR) asm volatile("" : "+s"(far_dwp));          // its addresses are made here, not kept in registers from row to row
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dwp_at(j, i) += ps[j][i] * static_cast<double>(pair_at(gate[j], i));
+                    for (int i = 0; i < 8; ++i) {
+                        const double term = ps[j][i] * static_cast<double>(pair_at(gate[j], i));
+                        if constexpr (FAR) {                // the first piece finds nothing there, the last leaves the share
+                            const double sum = pieces == 0 ? term : dwp_at(j, i) + term;
+                            if (more_then) dwp_at(j, i) = sum;
+                            o[i] = static_cast<float>(sum);
+                        } else {
+                            dwp_at(j, i) += term;
+                        }
+                    }
+                    if constexpr (FAR)
+                        if (!more_then && has(j)) store8_f32<TAIL>(p.part_p + static_cast<size_t>(worker) * H, (t + j * T) * 8, left(j), o);
                     if (has(j)) {
                         const int at = (t + j * T) * 8;
                         if (walk.whole) {
@@ -522,6 +540,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
 #pragma unroll
                     for (int i = 0; i < 8; ++i) ps[j][i] = 0.0;
                 }
+                ++pieces;
             }
             walk = then;
         }
@@ -554,10 +573,12 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : WIDE ? 2 * kGradThreads : kGradThr
         if constexpr (TIGHT) return sh_dw[(j * 8 + i) * kT + t];
         else return dw[j][i];
     }, p.part_w);
-    leave([&](int j, int i) {
-        if constexpr (GROUPS) return dwp_at(j, i);
-        else return ps[j][i];
-    }, p.part_p);
+    if (!FAR || pieces == 0)
+        leave([&](int j, int i) {
+            if constexpr (FAR) return 0.0;
+            else if constexpr (GROUPS) return dwp_at(j, i);
+            else return ps[j][i];
+        }, p.part_p);
     if (p.q) {
         __syncthreads();
         const uint32_t m = row_max<false>(__float_as_uint(amax), reinterpret_cast<uint32_t*>(sh[0]));
@@ -715,8 +736,8 @@ GatedNormArgs forward_args(const void* d_residual, const uint16_t* d_x, float re
     return p;
 }
 
-// rows of up to kTallH: one chunk a thread; beyond, two; beyond kWideH, two and twice the threads
-constexpr int kTallH = 8 * kGradThreads, kWideH = 16 * kGradThreads;
+// rows of up to kTallH: one chunk a thread; up to kWideH, two; the widest as kGradThreads has it
+constexpr int kTallH = 8 * kGradThreads<false, USUAL>, kUsualH = 2 * kTallH, kWideH = 16 * kGradThreads<false, WIDE>;
 // Workgroups of the backward pass: as many as run at once with 256 registers a thread, eight wavefronts a CU (292 of seven wavefronts ran in two rounds: 8192 x 7168 196 us, 134 with
 // 256), and four rows each, or the shares cost more than the rows; but 256 where there are as many rows.
 int gated_parts(int rows, int H) {
@@ -743,17 +764,21 @@ GradPlan grad_plan(int rows, int H, int gate_rows) {
     g.share = static_cast<unsigned>((rows - 1) / g.workers + 1);
     g.segments = g.several && !Walk::by_groups(g.groups, g.workers);
     const size_t shares = 2 * static_cast<size_t>(g.parts) + (g.segments ? 2 * static_cast<size_t>(g.workers) : 0);
-    g.far = g.several && H > kWideH ? static_cast<size_t>(g.parts) * 2 * 8 * (2 * kGradThreads) * sizeof(double) : 0;
+    const size_t threads = H > kWideH ? kGradThreads<true, WIDEST> : kGradThreads<true, WIDE>;
+    g.far = g.several && H > kUsualH ? static_cast<size_t>(g.parts) * 2 * 8 * threads * sizeof(double) : 0;
     g.bytes = g.far + (shares * H + g.parts) * sizeof(float);
     return g;
 }
 
+template <bool GROUPS>
+constexpr int kWidestChunks = GROUPS ? 2 : 4;
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL>
 void launch_gated_grad(const GatedGradArgs& p, int parts, hipStream_t st) {
-    if (p.H <= kOneWaveH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, true, 1, false><<<parts, 4 * kWave, 0, st>>>(p);
-    else if (p.H <= kTallH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1, false><<<parts, row_threads(p.H, 1), 0, st>>>(p);
-    else if (p.H <= kWideH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2, false><<<parts, row_threads(p.H, 2), 0, st>>>(p);
-    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2, true><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+    if (p.H <= kOneWaveH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, true, 1, USUAL><<<parts, 4 * kWave, 0, st>>>(p);
+    else if (p.H <= kTallH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 1, USUAL><<<parts, row_threads(p.H, 1), 0, st>>>(p);
+    else if (p.H <= kUsualH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2, USUAL><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+    else if (p.H <= kWideH) k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, 2, WIDE><<<parts, row_threads(p.H, 2), 0, st>>>(p);
+    else k_gated_norm_grad<F32, KEPT, GROUPS, TAIL, false, kWidestChunks<GROUPS>, WIDEST><<<parts, row_threads(p.H, kWidestChunks<GROUPS>), 0, st>>>(p);
 }
 
 int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, float* d_grad_scale, int accumulate, void* d_workspace,

@@ -316,6 +316,16 @@ def test_backward(cf, dev, rows, H, gate_rows, f32, kept):
 
 @pytest.mark.parametrize("kept", [False, True])
 @pytest.mark.parametrize("f32", [0, 1])
+@pytest.mark.parametrize("rows,H,gate_rows", [(300, 9216, 0), (300, 9216, 7), (600, 9001, 1), (700, 8200, 100), (2300, 8200, 1), (515, 12288, 2), (300, 12290, 0), (515, 13001, 250),
+                                              (600, 16384, 0), (600, 16384, 3)])
+def test_backward_of_wide_rows_with_several_a_workgroup(cf, dev, rows, H, gate_rows, f32, kept):
+    case(f"gated norm gradient rows={rows} H={H} gate_rows={gate_rows} f32={f32} kept={kept}")
+    g = Grad(rows, H, f32, gate_rows, 1.25, kept, rows + H)
+    check_backward(backward(cf, dev, g, ["both", "e5m2", "bf16"][(rows + f32) % 3]), g)
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("f32", [0, 1])
 @pytest.mark.parametrize("shift", [1, 2, 4])
 def test_backward_accumulates_in_place_at_any_alignment_and_without_a_stream_gradient(cf, dev, f32, shift, kept):
     for rows, H, gate_rows in ((40, 1032, 13), (7, 333, 1), (9, 4096, 9), (1100, 40, 300), (12, 10000, 5)):
