@@ -69,7 +69,8 @@ __device__ __forceinline__ float largest(const float (&a)[8]) {
 // What has been divided by its own maximum needs no clamp, and no look for NaNs: the conversion keeps them.
 // Bound by HBM once the instructions are few enough (30 an element in all; with 41, divisions by every lane, clamps and looks for NaNs, 8192 x 8192 took 90 to 102 us): 7 bytes an element,
 // 8192 x 8192 80 us (5.9 TB/s) with a scale a row or a group, 90 where a maximum is recorded, 8192 x 14336 144 (5.8); 1000 x 5461 9.4.
-// A whole row wants as few chunks a thread as it can have: 1, 2, 4 of them 78.6, 82.8, 83.9 us at 4096 wide, 81.0, 83.9, 85.3 at 8192, 85 each at 14336.
+// A whole row wants as few chunks a thread as it can have: 1, 2, 4 of them 78.6, 82.8, 83.9 us at 4096 wide, 81.0, 83.9, 85.3 at 8192, 85 each at 14336; 2048 x 18432
+// with three 50, with four 65.  Beyond 24576 a row of four fills a CU and its phases follow each other (2048 x 28672 88 us, 4.7 TB/s; a second one there would spill: 136).
 template <int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : QMODE == Q_ROWS ? 1024 : kKeepThreads) void k_swiglu_keep(const SwigluKeepArgs p) {
     __shared__ uint32_t sh[2][16];
@@ -417,6 +418,7 @@ int launch_keep(SwigluKeepArgs p, hipStream_t st) {
             if (p.I <= kOneWaveH) k_swiglu_keep<QMODE, TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
             else if (p.I <= kOneChunkH) k_swiglu_keep<QMODE, TAIL, false, 1><<<n, row_threads(p.I, 1), 0, st>>>(p);
             else if (p.I <= 2 * kOneChunkH) k_swiglu_keep<QMODE, TAIL, false, 2><<<n, row_threads(p.I, 2), 0, st>>>(p);
+            else if (p.I <= 3 * kOneChunkH) k_swiglu_keep<QMODE, TAIL, false, 3><<<n, row_threads(p.I, 3), 0, st>>>(p);
             else k_swiglu_keep<QMODE, TAIL, false, 4><<<n, row_threads(p.I, 4), 0, st>>>(p);
         } else {
             p.total = n * cut.parts;

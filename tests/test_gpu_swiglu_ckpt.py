@@ -124,6 +124,14 @@ def test_forward_any_alignment_and_stride(cf, dev, form, shift):
         check_forward(forward(cf, dev, g, u, form, 0, shift), g, u, form, 0)
 
 
+@pytest.mark.parametrize("e5m2", [0, 1])
+@pytest.mark.parametrize("rows,I", [(3, 16392), (2, 17001), (300, 24576), (2, 24577), (2, 32761)])
+def test_forward_wide_rows(cf, dev, rows, I, e5m2):
+    case(f"swiglu rows={rows} I={I} e5m2={e5m2}")
+    g, u = inputs(rows, I, rows * 7 + I)
+    check_forward(forward(cf, dev, g, u, "rows", e5m2), g, u, "rows", e5m2)
+
+
 @pytest.mark.parametrize("form", ["block", "record"])
 def test_forward_wider_than_a_row_in_registers(cf, dev, form):
     g, u = inputs(3, 70001, 5)
