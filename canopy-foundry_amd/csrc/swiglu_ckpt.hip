@@ -224,6 +224,7 @@ struct SwigluGradArgs {
     float* amax;
     int rows, I;
     unsigned row0, parts;
+    unsigned tile0, tiles;          // k_swiglu_grad8: the launch's first tile, and how many it has
 };
 
 // what eight elements give: dg, du and the activation
@@ -284,14 +285,15 @@ typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
 // LDS holds [column][128 bytes of rows] for each of the three outputs.  A wavefront's store instruction writes four bytes for each of 16 column blocks and four row blocks:
 // the 16-byte pieces of a column are xor-swizzled by the column block, and the upper eight blocks store their columns in swapped pairs, so that 64 lanes hit 64 banks.
 constexpr int kTile = 128, kTileThreads = 512;
+constexpr unsigned kLaunchTiles = (1u << 23) - 8;       // a launch has fewer than 2^32 threads
 template <bool TAIL, bool WHOLE_ROWS, bool WHOLE_LINES>
 __global__ __launch_bounds__(kTileThreads) void k_swiglu_grad8(const SwigluGradArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t tile[3][kTile * kTile];
     __shared__ uint32_t sh[16];
-    // the eight XCDs, which take workgroups in turn, each have an eighth of the tiles, in strips of a few column tiles and down the rows within one
+    // the eight XCDs, which take workgroups in turn, each have an eighth of the launch's tiles, in strips of a few column tiles and down the rows within one
     const unsigned across = (static_cast<unsigned>(p.I) + kTile - 1) / kTile, rows = p.rows, down = (rows + kTile - 1) / kTile;
-    const unsigned total = across * down, each = (total + 7) / 8, index = blockIdx.x % 8 * each + blockIdx.x / 8;
-    if (blockIdx.x / 8 >= each || index >= total) return;
+    const unsigned each = (p.tiles + 7) / 8, here = blockIdx.x % 8 * each + blockIdx.x / 8, index = p.tile0 + here;
+    if (blockIdx.x / 8 >= each || here >= p.tiles) return;
     constexpr unsigned kStrip = WHOLE_LINES ? 8 : 4;
     const unsigned strip = index / (kStrip * down) * kStrip, rest = index % (kStrip * down), wide = across - strip < kStrip ? across - strip : kStrip;
     const unsigned r0 = rest / wide * kTile, group = strip + rest % wide;
@@ -530,13 +532,16 @@ int cf_swiglu_ckpt8_backward_quant_e5m2(const uint16_t* d_grad_out, const void* 
     p.grad8 = static_cast<uint8_t*>(d_grad8); p.grad8_t = static_cast<uint8_t*>(d_grad8_t); p.act8_t = static_cast<uint8_t*>(d_act8_t);
     p.qscale = d_qscale; p.amax = d_amax; p.act_qscale = d_act_qscale;
     const size_t tiles = static_cast<size_t>(ceil_div(rows, kTile)) * ceil_div(I, kTile);
-    if ((tiles + 8) * kTileThreads > (static_cast<size_t>(1) << 32)) return CF_ERR_UNSUPPORTED;         // a terabyte of gradients
-    const unsigned grid = (static_cast<unsigned>(tiles) + 7) / 8 * 8;
+    if (tiles >= static_cast<size_t>(1) << 31) return CF_ERR_UNSUPPORTED;         // some 2^45 elements: 70 terabytes of d_grad_out
     hipStream_t st = as_stream(stream);
     auto go = [&](auto rows_whole, auto lines_whole) {
         constexpr bool ROWS = decltype(rows_whole)::value, LINES = decltype(lines_whole)::value;
-        if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
-        else k_swiglu_grad8<false, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+        for (p.tile0 = 0; p.tile0 < tiles; p.tile0 += kLaunchTiles) {
+            p.tiles = tiles - p.tile0 < kLaunchTiles ? static_cast<unsigned>(tiles) - p.tile0 : kLaunchTiles;
+            const unsigned grid = (p.tiles + 7) / 8 * 8;
+            if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+            else k_swiglu_grad8<false, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+        }
     };
     const std::true_type yes{};
     const std::false_type no{};
