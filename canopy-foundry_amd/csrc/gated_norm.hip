@@ -7,6 +7,7 @@
 //
 // Backward, per row:  g = dy * w,  D = dh + (g - hh * mean(g * hh)) / p,  dr = T(res * D),  e = D * gate * wp,  dx = (e - xh * mean(e * xh)) / px;
 // over the rows:  dw = sum(dy * hh);  over a gate's rows:  P = sum(D * xh),  dgate = wp * P;  over the gates:  dwp = sum(gate * P).
+#include "gated_norm_plan.hpp"
 #include "rows.hpp"
 
 #include <cmath>
@@ -254,9 +255,8 @@ struct Walk {
     unsigned group, start, m, n, others, first_n, last_n, lead;
     unsigned whole;                     // the group is this worker's alone
 
-    __host__ __device__ static bool by_groups(unsigned groups, unsigned workers) { return groups >= 8ull * workers; }
     __device__ __forceinline__ bool begin() {
-        if (by_groups(groups, workers)) {
+        if (whole_groups(groups, workers)) {
             group = worker;
         } else {
             if (static_cast<unsigned long long>(worker) * share >= rows) return false;
@@ -272,7 +272,7 @@ struct Walk {
         m = lead = others = last_n = 0;
         n = first_n = end - start;
         whole = 1;
-        if (by_groups(groups, workers)) return true;
+        if (whole_groups(groups, workers)) return true;
         const unsigned k0 = start / share, k1 = (end - 1) / share, mine = worker * share;
         if (start >= mine + share) return false;
         if (k0 == k1) return true;
@@ -291,7 +291,7 @@ struct Walk {
     __device__ __forceinline__ bool last_of_piece() const { return m + 1 == n; }
     __device__ __forceinline__ bool advance() {
         if (++m < n) return true;
-        group += by_groups(groups, workers) ? workers : 1;
+        group += whole_groups(groups, workers) ? workers : 1;
         return piece();
     }
 };
@@ -309,12 +309,6 @@ __device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const flo
     }
 }
 
-// Threads of a row at most: 512 of 256 registers, 768 of 168, 1024 of 128.  Up to H = 8192 a thread has one or two chunks.  WIDE, up to 12288: two, and the next row's operands on a
-// bf16 stream without groups alone, elsewhere they spill (us without them and with: 9216, bf16 98 and 87, with groups 110 and 145; fp32 131 and 221; all of it with 1024 threads 110, 161
-// and 192).  WIDEST: four, with groups two, which spill either way, if little (16384, without groups: four 98, two 113; with them 247 and 222).
-enum Width { USUAL, WIDE, WIDEST };
-template <bool GROUPS, Width WIDTH>
-constexpr int kGradThreads = WIDTH == WIDE ? 768 : WIDTH == WIDEST && GROUPS ? 1024 : 512;
 // A worker (a workgroup; ONE_WAVE: a wavefront) holds a row as k_gated_norm does and loads the next row's operands before it works on one.  Its shares of
 // the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
 // workers take turns at the rows; GROUPS: as Walk has it, and at the end of a piece of a group P is left, dgate itself where the worker had the whole group.
@@ -736,40 +730,6 @@ GatedNormArgs forward_args(const void* d_residual, const uint16_t* d_x, float re
     return p;
 }
 
-// rows of up to kTallH: one chunk a thread; up to kWideH, two; the widest as kGradThreads has it
-constexpr int kTallH = 8 * kGradThreads<false, USUAL>, kUsualH = 2 * kTallH, kWideH = 16 * kGradThreads<false, WIDE>;
-// Workgroups of the backward pass: as many as run at once with 256 registers a thread, eight wavefronts a CU (292 of seven wavefronts ran in two rounds: 8192 x 7168 196 us, 134 with
-// 256), and four rows each, or the shares cost more than the rows; but 256 where there are as many rows.
-int gated_parts(int rows, int H) {
-    const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kTallH ? 1 : 2) / kWave;
-    const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;
-    int parts = 256 * (waves < 8 ? 8 / waves : 1);
-    parts = parts < turns / 4 ? parts : turns / 4;
-    parts = parts > 256 ? parts : 256;
-    return parts < turns ? parts : turns;
-}
-struct GradPlan {
-    int parts, workers, groups;         // groups: 0 = no gate
-    bool several, segments;             // several groups; some of them in several workers' rows
-    unsigned share;                     // rows of a worker
-    size_t far, bytes;
-};
-GradPlan grad_plan(int rows, int H, int gate_rows) {
-    GradPlan g{};
-    if (rows == 0 || H == 0) return g;
-    g.parts = gated_parts(rows, H);
-    g.groups = gate_rows > 0 ? (rows - 1) / gate_rows + 1 : 0;
-    g.several = g.groups > 1;
-    g.workers = H <= kOneWaveH ? (4 * g.parts < rows ? 4 * g.parts : rows) : g.parts;
-    g.share = static_cast<unsigned>((rows - 1) / g.workers + 1);
-    g.segments = g.several && !Walk::by_groups(g.groups, g.workers);
-    const size_t shares = 2 * static_cast<size_t>(g.parts) + (g.segments ? 2 * static_cast<size_t>(g.workers) : 0);
-    const size_t threads = H > kWideH ? kGradThreads<true, WIDEST> : kGradThreads<true, WIDE>;
-    g.far = g.several && H > kUsualH ? static_cast<size_t>(g.parts) * 2 * 8 * threads * sizeof(double) : 0;
-    g.bytes = g.far + (shares * H + g.parts) * sizeof(float);
-    return g;
-}
-
 template <bool GROUPS>
 constexpr int kWidestChunks = GROUPS ? 2 : 4;
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL>
@@ -831,8 +791,7 @@ int gated_grad(GatedGradArgs p, bool kept, int f32, float* d_grad_post_scale, fl
     s.part_w = p.part_w; s.part_p = p.part_p; s.part_amax = p.part_amax; s.segments = p.segments; s.gate = p.gate; s.post_weight = p.post_weight;
     s.dgate = p.dgate; s.amax = p.q ? p.amax : nullptr; s.rows = p.rows; s.gate_rows = p.gate_rows; s.parts = plan.parts; s.share = plan.share;
     s.groups = plan.several ? 0 : plan.groups; s.accumulate_gate = p.accumulate_gate;
-    // a group has some workers / groups segments
-    s.shares = plan.workers >= 16 * plan.groups ? 32 : plan.workers >= 4 * plan.groups ? 8 : 2;
+    s.shares = plan.shares;
     const unsigned segment_blocks = plan.segments ? static_cast<unsigned>(plan.groups) * ceil_div(p.H, 4 * kSumThreads / s.shares) : 0;
     k_gated_sum<<<2 * s.sum_blocks + (s.amax ? 1 : 0) + segment_blocks, kSumThreads, 0, st>>>(s);
     return launch_status();

@@ -2,9 +2,11 @@
 // every row.
 #pragma once
 #include "common.hpp"
+#include "row_threads.hpp"
 
 namespace cf {
 
+static_assert(kRowWave == kWave);
 constexpr int kMaxH = 16384;
 
 enum { Q_ROWS = 0, Q_BLOCK = 1, Q_RECORD = 2 };
@@ -338,10 +340,6 @@ inline int check_shape(int rows, int H) {
     return H > kMaxH ? CF_ERR_UNSUPPORTED : 0;
 }
 inline bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
-
-// threads of a row, V chunks each
-constexpr int row_threads(int H, int V) { return ((H + 7) / 8 + kWave * V - 1) / (kWave * V) * kWave; }
-constexpr int kOneWaveH = 8 * kWave, kOneChunkH = 8 * 1024;
 
 constexpr unsigned kLaunchRows = 1u << 21;             // a launch has fewer than 2^32 threads
 
