@@ -402,8 +402,8 @@ Parts row_parts(int I, int V) {
     const unsigned each = (chunks + parts * V - 1) / (parts * V);
     return {parts, (each + kWave - 1) / kWave * kWave};
 }
-// rows of a launch: fewer than 2^32 threads
-unsigned launch_rows(unsigned parts) { return parts < (kLaunchRows >> 1) ? (kLaunchRows << 1) / parts : 1; }
+// rows of a launch: fewer than 2^32 threads; a row of fewer than 2^30 elements has 2^18 parts at most
+unsigned launch_rows(unsigned parts) { return (kLaunchRows << 1) / parts; }
 
 // Recording a maximum: a workgroup that takes two pieces in turn has one maximum to report where it had two, and one in 64 raises it after the first piece, before any
 // other looks.  8192 x 14336: one piece 151 to 157 us, two 145, three 149, four 154; as many workgroups as run at once 167 (8192 x 8192: one 87, two 90).
