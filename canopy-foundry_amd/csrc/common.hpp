@@ -134,6 +134,18 @@ __device__ __forceinline__ float e5m2_to_f32(uint8_t b) {
     return __uint_as_float(__float_as_uint(mag) | sign);
 }
 
+// ---- 4 x 4 bytes transposed: rows r0..r3 hold bytes n0..n3; returns columns: c[j] = {r0.bj, r1.bj, r2.bj, r3.bj}
+__device__ __forceinline__ void transpose4x4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t (&c)[4]) {
+    const uint32_t t0 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);
+    const uint32_t t1 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+    const uint32_t u0 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
+    const uint32_t u1 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+    c[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
+    c[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
+    c[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
+    c[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
+}
+
 // ---- 64-lane wavefront reductions ------------------------------------------
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll

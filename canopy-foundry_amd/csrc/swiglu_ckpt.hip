@@ -264,18 +264,6 @@ __global__ __launch_bounds__(kKeepThreads) void k_swiglu_grad(const SwigluGradAr
     if (p.act) store8_bf16<TAIL>(p.act, from, n, o.a);
 }
 
-// rows r0..r3 hold bytes n0..n3; returns columns: c[j] = {r0.bj, r1.bj, r2.bj, r3.bj}
-__device__ __forceinline__ void transpose4x4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t (&c)[4]) {
-    const uint32_t t0 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);
-    const uint32_t t1 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
-    const uint32_t u0 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
-    const uint32_t u1 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-    c[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
-    c[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
-    c[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
-    c[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
-}
-
 typedef uint32_t u32x4_byte __attribute__((ext_vector_type(4), aligned(1)));
 
 // 8-bit outputs, 9 bytes an element, bound by HBM and by how well lines are filled: 8192 x 14336 214 us (5.0 TB/s), 2000 x 8192 42, whose transposed rows begin anywhere in a line.

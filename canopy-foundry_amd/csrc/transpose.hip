@@ -26,18 +26,6 @@ constexpr int kTile = 128;
 // parity, i.e. sit in different halves.
 constexpr int kPitch = kTile;
 
-// rows r0..r3 hold bytes n0..n3; returns columns: c[j] = {r0.bj, r1.bj, r2.bj, r3.bj}
-__device__ __forceinline__ void transpose4x4(uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3, uint32_t c[4]) {
-    const uint32_t t0 = __builtin_amdgcn_perm(r1, r0, 0x05010400u);
-    const uint32_t t1 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
-    const uint32_t u0 = __builtin_amdgcn_perm(r3, r2, 0x05010400u);
-    const uint32_t u1 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
-    c[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
-    c[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
-    c[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
-    c[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
-}
-
 // 8 consecutive source elements of one row -> 8 bytes
 template <bool QUANT>
 __device__ __forceinline__ uint2 load_row8(const void* src, size_t elem_index, float s) {
