@@ -33,3 +33,27 @@ def test_many_groups_stay_in_range(plan):
         assert p["groups"] == -(-rows // gate_rows) and p["workers"] * p["share"] >= rows
         assert p["segments"] == (1 < p["groups"] < 8 * p["workers"])
         assert p["shares"] == (32 if p["workers"] >= 16 * p["groups"] else 8 if p["workers"] >= 4 * p["groups"] else 2)
+
+
+def width_class(H):
+    """A wavefront a row, one chunk a thread, two, two of the wide kernel, the widest."""
+    return sum(H > most for most in (512, 4096, 8192, 12288))
+
+
+def test_the_gpu_tests_reach_both_orders_at_every_width(plan):
+    """Whole groups (eight a worker and more), pieces of groups that several workers have, one gate and none; a change of the plan that takes an order out of its tests shows here."""
+    import test_gpu_gated_norm_groups as groups
+    import test_gpu_gated_norm_sums as sums
+    many = plan(groups.SHAPES)
+    assert all(p["several"] and not p["segments"] and p["groups"] >= 8 * p["workers"] for p in many)
+    assert {width_class(H) for _, H, _ in groups.SHAPES} == set(range(5))
+    assert {width_class(H) for rows, H, n in groups.SHAPES if n > 1 and rows % n} >= {0, 1, 2, 3}          # a last group cut short
+    for rows, H in sums.SHAPES:
+        none, one, some, each = plan([(rows, H, n if n is not None else rows) for n in sums.GATE_ROWS])
+        assert not none["several"] and not one["several"] and one["groups"] == 1
+        assert some["segments"] and 300 >= 3 * some["share"] and some["share"] >= 30          # pieces, and rows enough for 32 bits to show
+        assert each["several"] and not each["segments"]
+    assert {width_class(H) for _, H in sums.SHAPES} == set(range(5))
+    wide = dict(zip(groups.WIDE, plan(groups.WIDE)))
+    assert all(rows > p["parts"] for (rows, _, _), p in wide.items())
+    assert {(p["groups"] > 1, p["segments"]) for p in wide.values()} == {(False, 0), (True, 1), (True, 0)}
