@@ -39,7 +39,7 @@ struct GatedNormArgs {
 __device__ __forceinline__ float pair_at(const u32x4_any& v, int i) { return (i & 1) ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]); }
 
 // One row in registers, V chunks of eight elements a thread (forward_chunks() says how many), as k_add_norm holds it: everything is read and written once.  Bound by HBM, 9 or 13
-// bytes an element with both checkpoints: 8192 x 4096 59 us on a bf16 stream (5.1 TB/s), 83 on an fp32 one (5.2), 1000 x 7168 15; a row alone takes 3.7, launch, load and two
+// bytes an element with both checkpoints: 8192 x 4096 59 us on a bf16 stream (5.1 TB/s), 83 on an fp32 one (5.2), 1000 x 7168 13 to 14.5; a row alone takes 3.2, launch, load and two
 // reductions.  Recording a maximum adds 6 us to 8192 rows (see raise_last()).  Odd widths move whole chunks that straddle lines: 8192 x 4095 75 us.
 template <bool F32, int QMODE, bool TAIL, bool ONE_WAVE, int V>
 __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_norm(const GatedNormArgs p) {
@@ -313,8 +313,8 @@ __device__ __forceinline__ void store8_f32(float* p, size_t at, int n, const flo
 // the sums over rows are kept in 64 bits and rounded to fp32 once on their way through memory, as in k_add_norm_grad.  Without groups of rows
 // workers take turns at the rows; GROUPS: as Walk has it, and at the end of a piece of a group P is left, dgate itself where the worker had the whole group.
 // Bound by HBM: 8192 x 4096 from bf16 rows 73 us (5.5 TB/s), from checkpoints with the E5M2 bytes 54 (5.6), and 5 for k_gated_sum.  What it took: registers.  Two sums of
-// 64 bits a column, two rows of five tensors and three weights are 256 registers for eight or sixteen columns a thread; with 1024 threads of 128 each, 2000 x 7168 (fp32 stream,
-// gates by sequence) took 159 us, with 512 of 256 94, and 64 with dw in LDS, a row ahead and Walk's order.  Above H = 8192 there is room for
+// 64 bits a column, two rows of five tensors and three weights for eight or sixteen columns a thread: with 1024 threads of 128 registers, 2000 x 7168 (fp32 stream,
+// gates by sequence) took 159 us, with 512 of 256 94, and 64 with dw in LDS, a row ahead and Walk's order, for which 129 to 209 registers are enough.  Above H = 8192 there is room for
 // few rows ahead, and spills cost the most: 2730 x 12288 87 us (4.6 TB/s), 2048 x 16384 98 (4.1).
 template <bool F32, bool KEPT, bool GROUPS, bool TAIL, bool ONE_WAVE, int V, Width WIDTH>
 __global__ __launch_bounds__((ONE_WAVE ? 256 : kGradThreads<GROUPS, WIDTH>)) void k_gated_norm_grad(const GatedGradArgs p) {
@@ -676,7 +676,7 @@ float kept_scale(int H) {
 }
 
 // Chunks of a row that a thread has.  Two reductions follow each other here, which many rows hide best with some four workgroups a CU, whole rows behind each other's;
-// a row alone wants as many threads as it can have.  1, 2, 4 chunks, us, rows of both checkpoints, 33.6 M elements (the first line: kernel alone):
+// a row alone wants as many threads as it can have.  1, 2, 4 chunks, us, rows of both checkpoints, 33.6 M elements (the first line: one row, by events over many calls):
 //     1 row of 4096, bf16       3.7   4.4   5.8             H = 1024, f32     82.5  82.6  85.0
 //     H = 1024, bf16           60.3  57.3  68.8             H = 4096, f32     82.9  83.9  89.3
 //     H = 4096, bf16           61.4  58.5  61.0             H = 5120, f32     93.5  86.2  88.8
@@ -684,6 +684,9 @@ float kept_scale(int H) {
 //     H = 6144, bf16           73.8  65.1  60.6             H = 12288, f32      -   91.1 100.0
 //     H = 7168, bf16           78.5  65.2  61.4             H = 16384, f32      -   91.5  94.0
 //     H = 12288, bf16            -   63.7  74.2             H = 16384, bf16     -   70.9  63.3
+//     H = 8200, bf16             -   72.2  78.0             H = 13312, bf16     -   75.6  65.0
+//     H = 10240, bf16            -   66.3  69.6             H = 14336, bf16     -   77.4  64.0
+// Four are ahead from somewhere between 12288 and 13312 on, the rule's border lies above that.
 int forward_chunks(int rows, int H, bool f32) {
     if (rows <= 256 && H <= kOneChunkH) return 1;
     return !f32 && ((H >= 5120 && H <= kOneChunkH) || H > 14336) ? 4 : 2;

@@ -6,7 +6,7 @@
 
 namespace cf {
 
-// Threads of a row at most: 512 of 256 registers, 768 of 168, 1024 of 128.  Up to H = 8192 a thread has one or two chunks.  WIDE, up to 12288: two, and the next row's operands on a
+// Threads of a row at most: 512 of up to 256 registers, 768 of 168, 1024 of 128.  Up to H = 8192 a thread has one or two chunks.  WIDE, up to 12288: two, and the next row's operands on a
 // bf16 stream without groups alone, elsewhere they spill (us without them and with: 9216, bf16 98 and 87, with groups 110 and 145; fp32 131 and 221; all of it with 1024 threads 110, 161
 // and 192).  WIDEST: four, with groups two, which spill either way, if little (16384, without groups: four 98, two 113; with them 247 and 222).
 enum Width { USUAL, WIDE, WIDEST };
@@ -18,8 +18,13 @@ constexpr bool whole_groups(unsigned groups, unsigned workers) { return groups >
 
 // rows of up to kTallH: one chunk a thread; up to kWideH, two; the widest as kGradThreads has it
 constexpr int kTallH = 8 * kGradThreads<false, USUAL>, kUsualH = 2 * kTallH, kWideH = 16 * kGradThreads<false, WIDE>;
-// Workgroups of the backward pass: as many as run at once with 256 registers a thread, eight wavefronts a CU (292 of seven wavefronts ran in two rounds: 8192 x 7168 196 us, 134 with
-// 256), and four rows each, or the shares cost more than the rows; but 256 where there are as many rows.
+// Workgroups of the backward pass: eight wavefronts a CU, which all kernels have registers for (292 workgroups of seven ran in two rounds: 8192 x 7168 196 us, 134 with 256), and four
+// rows each, or the shares cost more than the rows; but 256 where there are as many rows.  Many kernels have registers for twelve wavefronts, whose additional shares mostly cost
+// more than they bring above H = 256.  8 and 12, us, 16.8 M elements, bf16 rows, dx as bf16:
+//                          no gate         four gates                                no gate         four gates
+//     H = 256            51.2   47.5      61.9   73.7            H = 1536          43.3   51.2      46.2   48.6
+//     H = 512            43.4   45.1      53.1   57.7            H = 2048          43.5   46.9      50.9   49.3
+//     H = 1024           44.3   46.7      53.1   56.3            H = 2048, f32     62.6   62.8      66.8   73.9
 inline int gated_parts(int rows, int H) {
     const int waves = H <= kOneWaveH ? 4 : row_threads(H, H <= kTallH ? 1 : 2) / kRowWave;
     const int turns = H <= kOneWaveH ? (rows - 1) / 4 + 1 : rows;

@@ -394,7 +394,13 @@ Parts row_parts(int I, int V) {
 unsigned launch_rows(unsigned parts) { return (kLaunchRows << 1) / parts; }
 
 // Recording a maximum: a workgroup that takes two pieces in turn has one maximum to report where it had two, and one in 64 raises it after the first piece, before any
-// other looks.  8192 x 14336: one piece 151 to 157 us, two 145, three 149, four 154; as many workgroups as run at once 167 (8192 x 8192: one 87, two 90).
+// other looks.  8192 x 14336: one piece 151 to 157 us, two 145, three 149, four 154; as many workgroups as run at once 167.  One and two elsewhere, us with the maximum's clearing:
+//                 4096 wide       6144            8192            11008           14336           16384
+//     1000 rows  11.1   10.6    16.7   13.9    17.1   15.4    22.6   20.4    25.5   24.4    29.6   27.5
+//     2048       18.2   15.7    24.4   22.7    29.7   28.6    38.1   35.1    44.4   42.4    48.6   47.2
+//     4096       31.3   28.8    40.2   37.4    49.3   49.1    64.8   61.4    80.5   75.6    85.0   86.6
+//     8192       51.1   48.8    69.9   66.1    87.3   90.7     118    114     153    145     157    165
+// So two are ahead below kTurnPieces as well, and one at powers of two from 8192 wide on with many rows: the rule goes by the number of pieces alone and takes neither.
 constexpr unsigned kTurnPieces = 4096;
 
 template <int QMODE, bool TAIL>
