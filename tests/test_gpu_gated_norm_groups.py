@@ -110,3 +110,24 @@ def test_wide_rows_accumulate(cf, dev, rows, H, gate_rows, f32, kept):
         else:
             assert torch.equal(got["dgate"], start["dgate"])
             check_backward(host(got), host(g), host(start), accumulate)
+
+
+def test_more_groups_than_an_int_times_sixteen(cf, dev):
+    """A gate for each of 2^27 rows and a few: the last ones give what they give alone; the rest are zeros, so that the sums over rows are those rows' too."""
+    rows, H, n = (1 << 27) + 5, 8, 700
+    case(f"gated norm gradient rows={rows} H={H} gate_rows=1")
+    g = Grad(dev, n, H, 0, 1, 1.25, True, 3)
+    want = backward(cf, dev, g, "both")
+    big = object.__new__(Grad)
+    big.a = Layer.__new__(Layer)
+    a, b = g.a, big.a
+    at_the_end = lambda t, fill=0.0: torch.cat([torch.full((rows - n, *t.shape[1:]), fill, dtype=t.dtype, device=dev), t])  # noqa: E731
+    bits = lambda t: at_the_end(t.view(torch.uint8)).view(E4M3)  # noqa: E731
+    b.rows, b.H, b.f32, b.gate_rows, b.res, b.wp, b.w, b.gate, b.r = rows, H, 0, 1, 1.25, a.wp, a.w, at_the_end(a.gate), a.r
+    big.kept, big.rms, big.post_rms, big.dy, big.dh, big.h, big.x = True, at_the_end(g.rms, 1.0), at_the_end(g.post_rms, 1.0), at_the_end(g.dy), at_the_end(g.dh), bits(g.h), bits(g.x)
+    got = backward(cf, dev, big, "both")
+    for k in ("dr", "dx", "q", "dgate"):
+        assert torch.equal(got[k][rows - n:], want[k]) and not bool(got[k][:rows - n].any()), k
+    assert got["amax"] == want["amax"]
+    for k in ("dw", "dwp"):         # the same terms in other shares, each of which is rounded once, and so is the sum
+        assert float((got[k].double() - want[k].double()).abs().max()) <= 2.0 ** -22 * n * float(want[k].abs().max())

@@ -53,3 +53,41 @@ def test_more_tiles_than_one_launch_holds(cf, dev, rows, I):
             assert torch.equal(grad[end], one) and torch.equal(grad_t[:, end], one_t) and torch.equal(act_t[:, end], one_act)
     for lines in (grad.view(2, I), grad_t.view(2, I), act_t.view(1, I)) if wide else (grad.t(), grad_t, act_t):
         assert not bool(lines[:, n:ends[1].start].any())
+
+
+@pytest.mark.parametrize("form", ["block", "record"])
+@pytest.mark.parametrize("rows,I", [(1, (1 << 30) - 1), ((1 << 30) + 200, 1)])
+def test_the_other_forms_run_there(cf, dev, rows, I, form):
+    """The forward pass and the bf16 gradient of the same sizes: their ends as alone."""
+    case(f"swiglu {form} {rows} x {I}")
+    n, wide = 1024, I > 1
+    ends = [slice(0, n), slice((max(rows, I) - n) // 128 * 128, max(rows, I))]
+    gen = torch.Generator(device=dev).manual_seed(4)
+    at = lambda end: (slice(None), end) if wide else (end, slice(None))  # noqa: E731
+    slots = lambda end: (slice(None), slice(end.start // 128, -(-end.stop // 128))) if wide else at(end)  # noqa: E731
+    g, u, do = (torch.zeros(rows, I, dtype=torch.bfloat16, device=dev) for _ in range(3))
+    for end in ends:
+        for t in (g, u, do):
+            t[at(end)] = torch.randn(t[at(end)].shape, device=dev, generator=gen).to(torch.bfloat16)
+
+    def run(g, u, do):
+        rows, I = g.shape
+        G = (I + 127) // 128
+        b8, d = [torch.zeros(rows, I, dtype=torch.uint8, device=dev) for _ in range(3)], [torch.zeros(rows, G, device=dev) for _ in range(4 if form == "block" else 2)]
+        amax = torch.zeros(1, device=dev)
+        if form == "block":
+            cf.cf_swiglu_ckpt8_quantize_block_1x128(g, u, I, rows, I, b8[0], d[0], b8[1], d[1], b8[2], d[2], d[3], stream())
+        else:
+            cf.cf_swiglu_ckpt8_quantize_record(g, u, I, rows, I, 0, b8[0], d[0], b8[1], d[1], b8[2], torch.full((1,), ACT_SCALE, device=dev), amax, stream())
+        o = [torch.zeros(rows, I, dtype=torch.bfloat16, device=dev) for _ in range(3)]
+        cf.cf_swiglu_ckpt8_backward(do, b8[0], d[0], b8[1], d[1], rows, I, o[0], o[1], I, o[2], stream())
+        torch.cuda.synchronize()
+        return b8 + o, d, float(amax)
+
+    values, scales, amax = run(g, u, do)
+    most = 0.0
+    for end in ends:
+        v, s, m = run(*(t[at(end)].contiguous() for t in (g, u, do)))
+        most = max(most, m)
+        assert all(torch.equal(a[at(end)], b) for a, b in zip(values, v)) and all(torch.equal(a[slots(end)], b) for a, b in zip(scales, s))
+    assert amax == most
