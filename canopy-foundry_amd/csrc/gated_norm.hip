@@ -94,7 +94,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_
         store8_bytes<TAIL>(to, base + (t + j * T) * 8, left(j), convert8_fp8<false>(v));
     };
 
-    // Each operation up to h is rounded to fp32 as it is written, and the root mean square comes from the threads' sums added in 64 bits, so that h has the bits that the formula
+    // Each operation up to h is rounded to fp32 as it is written, the mean of the squares from a 64-bit sum, so that h has the bits that the formula
     // has in fp32: a bf16 stream takes the next value where h lies next to the border of two, and through the maximum of a group one such value can be all of a scale's
     // difference (some 160 of 7 million values lie there).  x / px is x times the inverse and a correction by what that leaves.
     int e;

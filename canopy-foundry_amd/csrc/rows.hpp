@@ -275,23 +275,27 @@ __device__ __forceinline__ double row_sum(double v, double* sh) {
 
 // The root mean square of a row that its threads hold in chunks of eight, V each: sqrt(mean(h^2) + eps) = 2^e times what is returned, with the row scaled by
 // 2^-e, which h / rms does not see.  e is 0 but where squares leave fp32 (|h| of 1e19 and more, or of 1e-15 and less under as small an eps): then the sum is taken once
-// more of the scaled row.  A row that holds infinities or NaNs stays as it is.  SUM: the type in which the threads' sums are added up.  `sh`: two sums, `sh_max`: one maximum, as row_sum() and row_max() ask.
+// more of the scaled row.  A row that holds infinities or NaNs stays as it is.  SUM: the type of the sum; the mean, eps's addition and the root are one rounding to fp32 each.  `sh`: two sums, `sh_max`: one maximum, as row_sum() and row_max() ask.
 template <bool ONE_WAVE, int V, typename SUM>
 __device__ __forceinline__ float row_rms(float (&h)[V][8], int H, float eps, SUM (*sh)[16], uint32_t* sh_max, int& e) {
     auto mean_square = [&](SUM* s) {
-        float ss = 0.0f;
+        SUM ss = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            float part = 0.0f;
+            SUM part = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) part = __builtin_fmaf(h[j][i], h[j][i], part);
+            for (int i = 0; i < 8; ++i) {
+                const SUM v = h[j][i];
+                if constexpr (sizeof(SUM) == 8) part = __builtin_fma(v, v, part);
+                else part = __builtin_fmaf(v, v, part);
+            }
             ss += part;
         }
-        return row_sum<ONE_WAVE>(static_cast<SUM>(ss), s) / static_cast<SUM>(H);
+        return static_cast<float>(row_sum<ONE_WAVE>(ss, s) / static_cast<SUM>(H));
     };
-    SUM mean = mean_square(sh[0]) + eps;
+    float mean = mean_square(sh[0]) + eps;
     e = 0;
-    if (!(mean >= static_cast<SUM>(1e-30f) && mean < static_cast<SUM>(__builtin_inff()))) {
+    if (!(mean >= 1e-30f && mean < __builtin_inff())) {
         uint32_t m = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j)
@@ -308,8 +312,7 @@ __device__ __forceinline__ float row_rms(float (&h)[V][8], int H, float eps, SUM
             mean = mean_square(sh[1]) + ldexpf(eps, -2 * e);
         }
     }
-    if constexpr (sizeof(SUM) == 8) return static_cast<float>(sqrt(mean));
-    else return sqrtf(mean);
+    return sqrtf(mean);
 }
 
 // Raising one maximum from every row.  Atomics on one address take turns, and the rows that run first all find the value they start from: with an

@@ -269,8 +269,8 @@ int cf_add_rmsnorm_backward_quant_e5m2(const uint16_t* d_grad_normed, const void
  * For the backward pass the caller keeps h and x, or in their place the normalised rows in 8 bits: d_x8 = e4m3(xh * S), d_sum8 = e4m3(hh * S) [rows, H], null = not
  * wanted, with S the largest power of two with S * sqrt(H) <= 448, which no element of a normalised row can leave; S depends on H alone.  They round at
  * 2^-4 of the element or at 2^-10 / S, whichever is more; a NaN is NaN.  d_x8 and d_sum8 overlap no other argument.
- * Up to h every operation is one rounding to fp32, in the order written.  The order in which a row is summed follows from H, the stream's type and whether there are
- * more than 256 rows: a row alone may differ in its last bits from the same row in a batch.
+ * Up to h every operation is one rounding to fp32, in the order written, and the mean of x^2 one of a sum in 64 bits.  The order in which a row is summed
+ * follows from H, the stream's type and whether there are more than 256 rows: a row alone may differ in its last bits from the same row in a batch.
  * q and its scales, alignments, magnitudes, NaNs, eps and H <= 16384: as cf_add_rmsnorm_quantize_*.  residual_scale is finite, else CF_ERR_INVALID_ARG. */
 
 /* Per-row scales (no counterpart, as above; the scale's formula is that of kernels/fp8.cu:37-39,49). */
