@@ -699,8 +699,8 @@ int launch_gated_norm(GatedNormArgs p, hipStream_t st) {
         const int V = forward_chunks(p.rows, p.H, F32);
         if (p.H <= kOneWaveH) k_gated_norm<F32, QMODE, TAIL, true, 1><<<(n + 3) / 4, 4 * kWave, 0, st>>>(p);
         else if (V == 1) k_gated_norm<F32, QMODE, TAIL, false, 1><<<n, row_threads(p.H, 1), 0, st>>>(p);
-        else if (V == 2) k_gated_norm<F32, QMODE, TAIL, false, 2><<<n, row_threads(p.H, 2), 0, st>>>(p);
-        else k_gated_norm<F32, QMODE, TAIL, false, 4><<<n, row_threads(p.H, 4), 0, st>>>(p);
+        else if (F32 || V == 2) k_gated_norm<F32, QMODE, TAIL, false, 2><<<n, row_threads(p.H, 2), 0, st>>>(p);
+        else if constexpr (!F32) k_gated_norm<F32, QMODE, TAIL, false, 4><<<n, row_threads(p.H, 4), 0, st>>>(p);
     }
     return launch_status();
 }

@@ -533,8 +533,13 @@ int cf_swiglu_ckpt8_backward_quant_e5m2(const uint16_t* d_grad_out, const void* 
         for (p.tile0 = 0; p.tile0 < tiles; p.tile0 += kLaunchTiles) {
             p.tiles = tiles - p.tile0 < kLaunchTiles ? static_cast<unsigned>(tiles) - p.tile0 : kLaunchTiles;
             const unsigned grid = (p.tiles + 7) / 8 * 8;
-            if (rows % 16 != 0 || I % 8 != 0) k_swiglu_grad8<true, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
-            else k_swiglu_grad8<false, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+            if constexpr (!(ROWS && LINES)) {           // whole tiles have no tails
+                if (rows % 16 != 0 || I % 8 != 0) {
+                    k_swiglu_grad8<true, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
+                    continue;
+                }
+            }
+            k_swiglu_grad8<false, ROWS, LINES><<<grid, kTileThreads, 0, st>>>(p);
         }
     };
     const std::true_type yes{};
