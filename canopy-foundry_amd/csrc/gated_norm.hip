@@ -96,7 +96,7 @@ __global__ __launch_bounds__(ONE_WAVE ? 256 : V == 4 ? 512 : 1024) void k_gated_
 
     // Each operation up to h is rounded to fp32 as it is written, the mean of the squares from a 64-bit sum, so that h has the bits that the formula
     // has in fp32: a bf16 stream takes the next value where h lies next to the border of two, and through the maximum of a group one such value can be all of a scale's
-    // difference (some 160 of 7 million values lie there).  x / px is x times the inverse and a correction by what that leaves.
+    // difference (some 160 of 7 million values lie there).  The squares in 64 bits cost nothing that shows: 8192 x 4096 58.8 us without, 59.2 with them, 1000 x 7168 14.3 and 13.5.  x / px is x times the inverse and a correction by what that leaves.
     int e;
     const float post_rms = row_rms<ONE_WAVE, V>(h, H, p.eps, sh_post, sh_max[1], e);
     if (t == 0 && p.post_rms) p.post_rms[row] = ldexpf(post_rms, e);
